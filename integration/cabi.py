@@ -10,7 +10,7 @@ import os
 import re
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-HEADERS = ("teeny_b200.h", "teeny_qwen3.h", "teeny_hybrid.h")
+HEADERS = ("teeny_b200.h", "teeny_qwen3.h", "teeny_hybrid.h", "teeny_cache8.h")
 RUST_FILE = os.path.join(ROOT, "integration", "teeny-cuda", "src", "b200.rs")
 BEGIN, END = "// ---- generated from include/*.h: begin ----", "// ---- generated from include/*.h: end ----"
 
@@ -26,11 +26,11 @@ TYPES = {
     "teeny_qwen3*": "*mut TeenyQwen3", "teeny_qwen3**": "*mut *mut TeenyQwen3",
     "const teeny_hybrid_config*": "*const TeenyHybridConfig", "const teeny_hybrid_layer*": "*const TeenyHybridLayer",
     "const teeny_hybrid_branch*": "*const TeenyHybridBranch", "teeny_hybrid*": "*mut TeenyHybrid",
-    "teeny_hybrid**": "*mut *mut TeenyHybrid",
+    "teeny_hybrid**": "*mut *mut TeenyHybrid", "const teeny_cache8_shape*": "*const TeenyCache8Shape",
 }
 STRUCT_NAMES = {"teeny_attn_shape": "TeenyAttnShape", "teeny_qwen3_config": "TeenyQwen3Config",
                 "teeny_hybrid_config": "TeenyHybridConfig", "teeny_hybrid_layer": "TeenyHybridLayer",
-                "teeny_hybrid_branch": "TeenyHybridBranch"}
+                "teeny_hybrid_branch": "TeenyHybridBranch", "teeny_cache8_shape": "TeenyCache8Shape"}
 OPAQUE = {"teeny_qwen3": "TeenyQwen3", "teeny_hybrid": "TeenyHybrid"}
 
 

@@ -113,6 +113,16 @@ pub struct TeenyHybridBranch {
     pub softcap: f32,
     pub rot_scale: f32,
 }
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct TeenyCache8Shape {
+    pub slots: c_int,
+    pub kv_heads: c_int,
+    pub max_cached: c_int,
+    pub dim: c_int,
+    pub vdim: c_int,
+    pub block: c_int,
+}
 /// Opaque runner handle (`teeny_qwen3`).
 #[repr(C)]
 pub struct TeenyQwen3 {
@@ -290,6 +300,11 @@ extern "C" {
     pub fn teeny_head_linear(f32: c_int, x: *const c_void, ldx: c_longlong, x_head: c_longlong, w: *const c_void, y: *mut c_void, ldy: c_longlong, y_head: c_longlong, heads: c_int, n: c_int, k: c_int, rows: c_int, rot_dims: c_int, rot_off: c_int, inv_freq: *const f32, rot_scale: f32, seqs: *const c_int, n_seqs: c_int, stream: CUstream) -> c_int;
     pub fn teeny_latent_attention_scratch_bytes(vdim: c_int) -> usize;
     pub fn teeny_latent_attention(f32: c_int, q: *const c_void, ldq: c_longlong, rows: c_int, cache: *const c_void, slots: c_int, max_cached: c_int, out: *mut c_void, ldo: c_longlong, heads: c_int, dim: c_int, vdim: c_int, score_scale: f32, scratch: *mut c_void, scratch_bytes: usize, seqs: *const c_int, n_seqs: c_int, max_len: c_int, stream: CUstream) -> c_int;
+    pub fn teeny_cache8_append(f32: c_int, shape: *const TeenyCache8Shape, k: *mut c_void, v: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, weights: *mut f32, k_new: *const c_void, ldk: c_longlong, v_new: *const c_void, ldv: c_longlong, rows: c_int, seqs: *const c_int, host_seqs: *const c_int, n_seqs: c_int, max_len: c_int, stream: CUstream) -> c_int;
+    pub fn teeny_cache8_attention_scratch_bytes(shape: *const TeenyCache8Shape, f32: c_int, heads: c_int, rows: c_int, n_seqs: c_int, max_len: c_int, with_weights: c_int) -> usize;
+    pub fn teeny_cache8_attention(f32: c_int, shape: *const TeenyCache8Shape, k: *const c_void, v: *const c_void, k_scale: *const f32, v_scale: *const f32, weights: *mut f32, weight_decay: f32, q: *const c_void, ldq: c_longlong, out: *mut c_void, ldo: c_longlong, rows: c_int, heads: c_int, score_scale: f32, softcap: f32, sink: *const f32, gate: *const c_void, ldg: c_longlong, lse: *mut f32, scratch: *mut c_void, scratch_bytes: usize, seqs: *const c_int, host_seqs: *const c_int, n_seqs: c_int, max_len: c_int, stream: CUstream) -> c_int;
+    pub fn teeny_cache8_evict_scratch_bytes(shape: *const TeenyCache8Shape, n_seqs: c_int, keep: c_int) -> usize;
+    pub fn teeny_cache8_evict(shape: *const TeenyCache8Shape, k: *mut c_void, v: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, weights: *mut f32, keep: c_int, recent: c_int, kept: *mut c_int, scratch: *mut c_void, scratch_bytes: usize, seqs: *const c_int, host_seqs: *const c_int, n_seqs: c_int, stream: CUstream) -> c_int;
 }
 // ---- generated from include/*.h: end ----
 

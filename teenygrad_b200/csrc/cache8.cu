@@ -1,0 +1,406 @@
+// The 8-bit key/value cache: appending tokens, evicting them, and the entry points of teeny_cache8.h.
+//
+// Scales are powers of two, so that holding a code at another scale is a shift of its exponent, exact unless the result leaves E4M3's
+// normal range.  A block's scale is 2^k with the smallest k >= -126 for which its largest number is at most 448 * 2^k.
+#include <cstdlib>
+
+#include "../../include/teeny_cache8.h"
+#include "common.cuh"
+#include "kernels.h"
+
+namespace teeny {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Exponent of the scale for numbers up to amax (finite, >= 0): 448 = 1.75 * 2^8.
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const unsigned u = __float_as_uint(amax);
+  return max(-126, static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0));
+}
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<unsigned>(k + 127) << 23); }  // -126 <= k <= 127
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float m = fabsf(x);
+  return m < INFINITY ? m : 0.0f;
+}
+// four numbers, none of them beyond 448 after scaling, as E4M3 (round to nearest even; what is not finite becomes NaN)
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
+  auto one = [&](float x) { return fabsf(x) < INFINITY ? x * inv : __uint_as_float(0x7fffffffu); };
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(one(a), one(b)), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(one(c), one(d)), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+__device__ __forceinline__ float4 decode4(uint32_t w) {
+  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
+  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ uint4 rescale16(uint4 w, float factor) {
+  uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 x = decode4(r[i]);
+    r[i] = encode4(x.x, x.y, x.z, x.w, factor);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// 16 numbers of a row; vec: 16-byte pieces
+__device__ __forceinline__ void load16(const bf16* p, bool vec, float (&x)[16]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 w = reinterpret_cast<const uint4*>(p)[i];
+      const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { x[8 * i + 2 * e] = bf16_lo(r[e]); x[8 * i + 2 * e + 1] = bf16_hi(r[e]); }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __bfloat162float(p[e]);
+  }
+}
+__device__ __forceinline__ void load16(const float* p, bool vec, float (&x)[16]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 w = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = w.x; x[4 * i + 1] = w.y; x[4 * i + 2] = w.z; x[4 * i + 3] = w.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = p[e];
+  }
+}
+__device__ __forceinline__ float block_max(float v, float* sh) {
+  v = warp_max(v);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float m = sh[0];
+  for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) m = fmaxf(m, sh[w]);
+  return m;
+}
+
+// One CTA for the new tokens of one entry in one block of the cache: blockIdx = (block counted from the entry's first, 2 * head + (values), entry).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) cache8_append_kernel(const Cache8 c, const Cache8Append a, const SeqDesc* seqs, int max_len, int vec) {
+  __shared__ float sh[kThreads / 32];
+  pdl_wait();
+  const SeqDesc sq = seqs[blockIdx.z];
+  if (!cache8_fits(sq, c, a.rows, max_len)) return;
+  const int head = blockIdx.y >> 1, of_v = blockIdx.y & 1, d = of_v ? c.V : c.D, per = d / 16;
+  const int b = sq.pos / c.B + blockIdx.x, begin = max(sq.pos, b * c.B), end = min(sq.pos + sq.len, (b + 1) * c.B);
+  if (begin >= end) return;
+  const size_t sh_row = static_cast<size_t>(sq.slot) * c.H + head;
+  uint8_t* codes = (of_v ? c.v : c.k) + sh_row * c.cap * d;
+  float* scales = (of_v ? c.vs : c.ks) + sh_row * c.blocks;
+  const long long ld = of_v ? a.ldv : a.ldk;
+  const T* src = static_cast<const T*>(of_v ? a.v : a.k) + (sq.row0 + begin - sq.pos) * ld + head * d;
+  const bool older = begin > b * c.B;
+  const float was = older ? scales[b] : 0.0f;
+  const int chunks = (end - begin) * per;
+  float amax = 0.0f;
+  for (int i = threadIdx.x; i < chunks; i += kThreads) {
+    float x[16];
+    load16(src + i / per * ld + i % per * 16, vec, x);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_abs(x[e]));
+  }
+  amax = block_max(amax, sh);
+  const float fresh = pow2(scale_exponent(amax)), scale = older ? fmaxf(fresh, was) : fresh;
+  const float inv = pow2(127 - static_cast<int>(__float_as_uint(scale) >> 23));
+  for (int i = threadIdx.x; i < chunks; i += kThreads) {
+    float x[16];
+    load16(src + i / per * ld + i % per * 16, vec, x);
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = encode4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3], inv);
+    reinterpret_cast<uint4*>(codes + static_cast<size_t>(begin) * d)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (older && scale != was) {
+    uint4* old = reinterpret_cast<uint4*>(codes + static_cast<size_t>(b) * c.B * d);
+    for (int i = threadIdx.x; i < (begin - b * c.B) * per; i += kThreads) old[i] = rescale16(old[i], was * inv);
+  }
+  if (threadIdx.x == 0) scales[b] = scale;
+  if (!of_v && c.w)
+    for (int t = begin + threadIdx.x; t < end; t += kThreads) c.w[sh_row * c.cap + t] = 0.0f;
+}
+
+// ---- eviction ----
+// Weights as unsigned numbers of the same order, NaN the least, zeros of both signs the same.
+__device__ __forceinline__ unsigned order_key(float w) {
+  if (w != w) return 0u;
+  const unsigned u = w == 0.0f ? 0u : __float_as_uint(w);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+constexpr int kSelThreads = 1024, kBins = 2048;
+
+// The kept tokens of one (entry, head), in order.  The smallest kept weight is found by digits, 11, 11 and 10 bits from the top: a histogram of
+// the next digit of the keys that agree with the digits found so far.
+__global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8 c, int keep, int recent, int* kept, const SeqDesc* seqs) {
+  __shared__ int hist[kBins], sums[32], found[2], warp_gt[32], warp_eq[32];
+  const int head = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  const SeqDesc sq = seqs[blockIdx.y];
+  int* out = kept + (static_cast<size_t>(blockIdx.y) * c.H + head) * keep;
+  const bool ok = sq.slot >= 0 && sq.slot < c.slots && sq.pos >= 0 && sq.pos <= c.cap;
+  const int len = ok ? sq.pos : 0;
+  if (len <= keep) {
+    for (int i = tid; i < keep; i += kSelThreads) out[i] = i < len ? i : -1;
+    return;
+  }
+  const float* w = c.w + (static_cast<size_t>(sq.slot) * c.H + head) * c.cap;
+  const int cand = len - recent, want = keep - recent;
+  unsigned prefix = 0;
+  int left = want;  // of the keys that agree with the prefix, the `left` largest are kept
+  if (want > 0) {
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < cand; i += kSelThreads) {
+        const unsigned key = order_key(w[i]);
+        if (pass == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1);
+      }
+      __syncthreads();
+      // counts from the largest digit down: thread t has digits 2047 - 2t and 2046 - 2t
+      const int hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
+      int run = hi + lo;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += up;
+      }
+      if (lane == 31) sums[warp] = run;
+      __syncthreads();
+      int above = run - hi - lo;
+      for (int k = 0; k < warp; ++k) above += sums[k];
+      if (above < left && left <= above + hi) { found[0] = kBins - 1 - 2 * tid; found[1] = above; }
+      else if (above + hi < left && left <= above + hi + lo) { found[0] = kBins - 2 - 2 * tid; found[1] = above + hi; }
+      __syncthreads();
+      prefix = prefix << bits | static_cast<unsigned>(found[0]);
+      left -= found[1];
+      __syncthreads();
+    }
+  }
+  // each warp has a stretch of the candidates: count, then write behind what the warps before keep
+  const int stretch = (cand + 31) / 32, first = min(cand, warp * stretch), last = min(cand, first + stretch);
+  int gt = 0, eq = 0;
+  for (int i = first; i < last; i += 32) {
+    const unsigned key = i + lane < last ? order_key(w[i + lane]) : 0u;
+    const bool in = i + lane < last && want > 0;
+    gt += __popc(__ballot_sync(0xffffffffu, in && key > prefix));
+    eq += __popc(__ballot_sync(0xffffffffu, in && key == prefix));
+  }
+  if (lane == 0) { warp_gt[warp] = gt; warp_eq[warp] = eq; }
+  __syncthreads();
+  int above = 0, ties = 0;
+  for (int k = 0; k < warp; ++k) { above += warp_gt[k]; ties += warp_eq[k]; }
+  for (int i = first; i < last; i += 32) {
+    const unsigned key = i + lane < last ? order_key(w[i + lane]) : 0u;
+    const bool in = i + lane < last && want > 0;
+    const unsigned g = __ballot_sync(0xffffffffu, in && key > prefix), e = __ballot_sync(0xffffffffu, in && key == prefix);
+    const unsigned below = (1u << lane) - 1;
+    const int tie = ties + __popc(e & below), at = above + __popc(g & below) + min(tie, left);
+    if ((g >> lane & 1) || ((e >> lane & 1) && tie < left)) out[at] = i + lane;
+    above += __popc(g);
+    ties += __popc(e);
+  }
+  for (int i = tid; i < recent; i += kSelThreads) out[want + i] = cand + i;
+}
+
+// Kept tokens to the front, block by block in order: a kept token's row is never before its place, so a block's rows are read before any
+// write reaches them.  One CTA for the keys or the values of an (entry, head).
+__global__ void __launch_bounds__(kThreads) cache8_compact_kernel(const Cache8 c, int keep, const int* kept, const SeqDesc* seqs) {
+  __shared__ float sh[kThreads / 32];
+  constexpr int kMost = kCache8Block * kCache8Head / 16 / kThreads;
+  pdl_wait();
+  const SeqDesc sq = seqs[blockIdx.y];
+  if (sq.slot < 0 || sq.slot >= c.slots || sq.pos < 0 || sq.pos > c.cap) return;
+  const int head = blockIdx.x >> 1, of_v = blockIdx.x & 1, d = of_v ? c.V : c.D, per = d / 16, len = min(sq.pos, keep);
+  const size_t sh_row = static_cast<size_t>(sq.slot) * c.H + head;
+  uint8_t* codes = (of_v ? c.v : c.k) + sh_row * c.cap * d;
+  float* scales = (of_v ? c.vs : c.ks) + sh_row * c.blocks;
+  float* w = c.w + sh_row * c.cap;
+  const int* index = kept + (static_cast<size_t>(blockIdx.y) * c.H + head) * keep;
+  for (int t0 = 0; t0 < len; t0 += c.B) {
+    const int tokens = min(c.B, len - t0), chunks = tokens * per;
+    uint4 x[kMost];
+    float s[kMost], amax = 0.0f, wt = 0.0f;
+#pragma unroll
+    for (int m = 0; m < kMost; ++m) {
+      const int i = threadIdx.x + m * kThreads;
+      if (i >= chunks) break;
+      const int from = index[t0 + i / per];
+      x[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from) * d + i % per * 16);
+      s[m] = scales[from / c.B];
+      const uint32_t r[4] = {x[m].x, x[m].y, x[m].z, x[m].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 y = decode4(r[e]);
+        amax = fmaxf(amax, s[m] * fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
+      }
+    }
+    if (!of_v && threadIdx.x < tokens) wt = w[index[t0 + threadIdx.x]];
+    amax = block_max(amax, sh);
+    const float scale = pow2(scale_exponent(amax)), inv = pow2(127 - static_cast<int>(__float_as_uint(scale) >> 23));
+#pragma unroll
+    for (int m = 0; m < kMost; ++m) {
+      const int i = threadIdx.x + m * kThreads;
+      if (i >= chunks) break;
+      reinterpret_cast<uint4*>(codes + static_cast<size_t>(t0) * d)[i] = rescale16(x[m], s[m] * inv);
+    }
+    if (threadIdx.x == 0) scales[t0 / c.B] = scale;
+    if (!of_v && threadIdx.x < tokens) w[t0 + threadIdx.x] = wt;
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+int cache8_append(const Cache8& c, const Cache8Append& a, const SeqDesc* seqs, int n_seqs, int max_len, cudaStream_t st) {
+  const int size = a.f32 ? 4 : 2;
+  const uintptr_t rows16 = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | static_cast<uintptr_t>(a.ldk * size) |
+                           static_cast<uintptr_t>(a.ldv * size);
+  const int vec = (rows16 & 15) == 0;
+  const dim3 grid((max_len + c.B - 2) / c.B + 1, 2 * c.H, n_seqs);
+  if (a.f32) launch_kernel(cache8_append_kernel<float>, grid, dim3(kThreads), 0, st, 1, c, a, seqs, max_len, vec);
+  else launch_kernel(cache8_append_kernel<bf16>, grid, dim3(kThreads), 0, st, 1, c, a, seqs, max_len, vec);
+  return static_cast<int>(cudaGetLastError());
+}
+
+size_t cache8_evict_scratch_bytes(const Cache8&, int, int) { return 0; }
+
+int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void*, const SeqDesc* seqs, int n_seqs, cudaStream_t st) {
+  launch_kernel(cache8_select_kernel, dim3(c.H, n_seqs), dim3(kSelThreads), 0, st, 1, c, keep, recent, kept, seqs);
+  launch_kernel(cache8_compact_kernel, dim3(2 * c.H, n_seqs), dim3(kThreads), 0, st, 1, c, keep, static_cast<const int*>(kept), seqs);
+  return static_cast<int>(cudaGetLastError());
+}
+
+namespace {
+
+bool cache_of(const teeny_cache8_shape* s, Cache8* c) {
+  if (!s || s->slots <= 0 || s->kv_heads <= 0 || s->kv_heads > 16384 || s->max_cached <= 0 || s->max_cached > (1 << 30) || s->dim <= 0 ||
+      s->dim > kCache8Head || s->dim % 16 || s->vdim <= 0 || s->vdim > kCache8Head || s->vdim % 16 ||
+      (s->block != 16 && s->block != 32 && s->block != 64 && s->block != 128))
+    return false;
+  *c = Cache8{nullptr, nullptr, nullptr, nullptr, nullptr, s->slots, s->kv_heads, s->max_cached, s->dim, s->vdim, s->block,
+              (s->max_cached + s->block - 1) / s->block};
+  return true;
+}
+int bind_cache(Cache8* c, void* k, void* v, float* ks, float* vs, float* w) {
+  if (!k || !v || !ks || !vs) return TEENY_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return TEENY_ERR_ALIGNMENT;
+  c->k = static_cast<uint8_t*>(k);
+  c->v = static_cast<uint8_t*>(v);
+  c->ks = ks;
+  c->vs = vs;
+  c->w = w;
+  return TEENY_OK;
+}
+// The host's copy of a step table, where the caller has one.  once: a slot may come only once (with by_len: in entries that have tokens).
+int check_table(const SeqDesc* t, int n, const Cache8& c, bool once, bool by_len) {
+  unsigned char* seen = once && n > 1 ? static_cast<unsigned char*>(calloc((static_cast<size_t>(c.slots) + 7) / 8, 1)) : nullptr;
+  if (once && n > 1 && !seen) return TEENY_ERR_BAD_ARG;
+  int rc = TEENY_OK;
+  for (int i = 0; i < n && rc == TEENY_OK; ++i) {
+    if (t[i].slot < 0 || t[i].slot >= c.slots) { rc = TEENY_ERR_BAD_ARG; break; }
+    if (!seen || (by_len && t[i].len == 0)) continue;
+    unsigned char& byte = seen[t[i].slot >> 3];
+    const unsigned char bit = static_cast<unsigned char>(1u << (t[i].slot & 7));
+    if (byte & bit) rc = TEENY_ERR_BAD_ARG;
+    byte |= bit;
+  }
+  free(seen);
+  return rc;
+}
+// (an entry without tokens does nothing)
+bool all_fit(const SeqDesc* t, int n, const Cache8& c, int rows, int max_len) {
+  for (int i = 0; i < n; ++i)
+    if (!cache8_fits(t[i], c, rows, max_len) && !(t[i].len == 0 && t[i].pos >= 0 && t[i].pos <= c.cap)) return false;
+  return true;
+}
+bool step_sizes(int rows, int n_seqs, int max_len) { return rows > 0 && n_seqs > 0 && n_seqs <= 65535 && max_len > 0; }
+
+}  // namespace
+}  // namespace teeny
+
+using namespace teeny;
+
+extern "C" {
+
+int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void* v, float* k_scale, float* v_scale, float* weights,
+                        const void* k_new, long long ldk, const void* v_new, long long ldv, int rows, const int* seqs,
+                        const int* host_seqs, int n_seqs, int max_len, teeny_stream_t stream) {
+  Cache8 c;
+  if (!cache_of(shape, &c) || !k_new || !v_new || !seqs || !step_sizes(rows, n_seqs, max_len) ||
+      ldk < static_cast<long long>(c.H) * c.D || ldv < static_cast<long long>(c.H) * c.V)
+    return TEENY_ERR_BAD_ARG;
+  if (const int rc = bind_cache(&c, k, v, k_scale, v_scale, weights)) return rc;
+  if (const SeqDesc* host = reinterpret_cast<const SeqDesc*>(host_seqs)) {
+    if (!all_fit(host, n_seqs, c, rows, max_len)) return TEENY_ERR_BAD_ARG;
+    if (const int rc = check_table(host, n_seqs, c, true, true)) return rc;
+  }
+  const Cache8Append a{f32 != 0, k_new, v_new, ldk, ldv, rows};
+  return cache8_append(c, a, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, max_len, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int f32, int heads, int rows, int n_seqs, int max_len,
+                                            int with_weights) {
+  Cache8 c;
+  if (!cache_of(shape, &c) || heads <= 0 || heads % c.H || !step_sizes(rows, n_seqs, max_len)) return 0;
+  return cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, with_weights != 0);
+}
+
+int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void* k, const void* v, const float* k_scale,
+                           const float* v_scale, float* weights, float weight_decay, const void* q, long long ldq, void* out,
+                           long long ldo, int rows, int heads, float score_scale, float softcap, const float* sink, const void* gate,
+                           long long ldg, float* lse, void* scratch, size_t scratch_bytes, const int* seqs, const int* host_seqs,
+                           int n_seqs, int max_len, teeny_stream_t stream) {
+  Cache8 c;
+  if (!cache_of(shape, &c) || !q || !out || !seqs || !step_sizes(rows, n_seqs, max_len) || heads <= 0 || heads % c.H ||
+      ldq < static_cast<long long>(heads) * c.D || ldo < static_cast<long long>(heads) * c.V ||
+      (gate && ldg < static_cast<long long>(heads) * c.V) || !(softcap >= 0.0f) || !(score_scale == score_scale))
+    return TEENY_ERR_BAD_ARG;
+  if (const int rc = bind_cache(&c, const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scale), const_cast<float*>(v_scale), weights))
+    return rc;
+  const SeqDesc* host = reinterpret_cast<const SeqDesc*>(host_seqs);
+  if (host) {
+    if (!all_fit(host, n_seqs, c, rows, max_len)) return TEENY_ERR_BAD_ARG;
+    if (const int rc = check_table(host, n_seqs, c, weights != nullptr, true)) return rc;
+  }
+  const size_t need = cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, weights != nullptr);
+  if (need && (!scratch || scratch_bytes < need)) return TEENY_ERR_SCRATCH;
+  if (reinterpret_cast<uintptr_t>(scratch) & 15) return TEENY_ERR_ALIGNMENT;
+  const Cache8Attn a{f32 != 0, q, ldq, out, ldo, rows, heads, score_scale, softcap, sink, gate, ldg, lse, weights != nullptr, weight_decay,
+                     scratch, scratch_bytes};
+  return cache8_attention(c, a, reinterpret_cast<const SeqDesc*>(seqs), host, n_seqs, max_len, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t teeny_cache8_evict_scratch_bytes(const teeny_cache8_shape* shape, int n_seqs, int keep) {
+  Cache8 c;
+  if (!cache_of(shape, &c) || n_seqs <= 0 || n_seqs > 65535 || keep <= 0 || keep > c.cap) return 0;
+  return cache8_evict_scratch_bytes(c, n_seqs, keep);
+}
+
+int teeny_cache8_evict(const teeny_cache8_shape* shape, void* k, void* v, float* k_scale, float* v_scale, float* weights, int keep,
+                       int recent, int* kept, void* scratch, size_t scratch_bytes, const int* seqs, const int* host_seqs, int n_seqs,
+                       teeny_stream_t stream) {
+  Cache8 c;
+  if (!cache_of(shape, &c) || !weights || !kept || !seqs || n_seqs <= 0 || n_seqs > 65535 || keep <= 0 || keep > c.cap || recent < 0 || recent > keep)
+    return TEENY_ERR_BAD_ARG;
+  if (const int rc = bind_cache(&c, k, v, k_scale, v_scale, weights)) return rc;
+  if (const SeqDesc* host = reinterpret_cast<const SeqDesc*>(host_seqs)) {
+    for (int i = 0; i < n_seqs; ++i)
+      if (host[i].pos < 0 || host[i].pos > c.cap) return TEENY_ERR_BAD_ARG;
+    if (const int rc = check_table(host, n_seqs, c, true, false)) return rc;
+  }
+  const size_t need = cache8_evict_scratch_bytes(c, n_seqs, keep);
+  if (need && (!scratch || scratch_bytes < need)) return TEENY_ERR_SCRATCH;
+  if (reinterpret_cast<uintptr_t>(scratch) & 15) return TEENY_ERR_ALIGNMENT;
+  return cache8_evict(c, keep, recent, kept, scratch, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -506,4 +506,46 @@ int glu_interleaved_f32(const float* gu, long long ld, float* out, long long ldo
 int argmax_f32(const float* logits, long long ld, float* best_val, int* best_idx, int rows, int cols, cudaStream_t st);
 int f32_to_bf16(const float* x, bf16* y, long long n, cudaStream_t st);
 
+// ---- 8-bit key/value cache (cache8.cu, cache8_attention.cu; layout in teeny_cache8.h) ----
+struct Cache8 {
+  uint8_t *k, *v;
+  float *ks, *vs, *w;  // scales; weights or null
+  int slots, H, cap, D, V, B, blocks;  // B tokens a block, `blocks` of them a slot and head
+};
+constexpr int kCache8Head = 128;   // largest dim and vdim
+constexpr int kCache8Block = 128;  // largest block
+// An entry that the kernels leave out: they read and write nothing of it.
+__host__ __device__ inline bool cache8_fits(const SeqDesc& s, const Cache8& c, int rows, int max_len) {
+  return s.slot >= 0 && s.slot < c.slots && s.pos >= 0 && s.len > 0 && s.len <= max_len && s.len <= c.cap && s.pos <= c.cap - s.len &&
+         s.row0 >= 0 && s.row0 <= rows - s.len;
+}
+struct Cache8Append {
+  int f32;
+  const void *k, *v;  // [rows, ld], heads side by side
+  long long ldk, ldv;
+  int rows;
+};
+int cache8_append(const Cache8& c, const Cache8Append& a, const SeqDesc* seqs, int n_seqs, int max_len, cudaStream_t st);
+struct Cache8Attn {
+  int f32;
+  const void* q;
+  long long ldq;
+  void* out;
+  long long ldo;
+  int rows, Hq;
+  float scale, softcap;
+  const float* sink;
+  const void* gate;
+  long long ldg;
+  float* lse;      // [rows, Hq] or null
+  int weights;     // add to the cache's weights
+  float decay;
+  void* scratch;
+  size_t scratch_bytes;
+};
+size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights);
+int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int max_len, cudaStream_t st);
+size_t cache8_evict_scratch_bytes(const Cache8& c, int n_seqs, int keep);
+int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, int n_seqs, cudaStream_t st);
+
 }  // namespace teeny

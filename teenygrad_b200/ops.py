@@ -9,7 +9,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import lib, check, AttnShape
+from ._lib import lib, check, AttnShape, Cache8Shape
 
 _BF16, _F32 = torch.bfloat16, torch.float32
 
@@ -537,3 +537,154 @@ def latent_attention(q, cache, vdim, score_scale, seqs, max_len, out=None, scrat
                                      out.stride(0), q.shape[1], q.shape[2], vdim, float(score_scale), _ptr(scratch),
                                      0 if scratch is None else scratch.numel(), _ptr(seqs), seqs.shape[0], max_len, _stream()), "latent_attention")
     return out
+
+
+# ---- the 8-bit key/value cache (include/teeny_cache8.h) ----
+class StepTable:
+    """A step's entries on the device (``seqs`` int32 [n, 4]) and in host memory (``host``), with what the calls need to know of
+    them.  A program that advances ``seqs`` on the device (a replayed graph) passes the table all the same: the kernels go by
+    ``seqs``, the host's copy serves the checks of arguments and the choice of kernels when a call is made or captured."""
+
+    def __init__(self, entries, device="cuda"):
+        rows = [tuple(int(x) for x in e) for e in entries]
+        if not rows or any(len(e) != 4 for e in rows):
+            raise ValueError("a step table is a list of (slot, position, first row, tokens)")
+        self.n, self.longest = len(rows), max(e[3] for e in rows)
+        self.seqs = torch.tensor(rows, dtype=torch.int32, device=device)
+        self.host = (C.c_int * (4 * self.n))(*[x for e in rows for x in e])
+
+
+def step_table(entries, device="cuda"):
+    """Entries of a step for the ``cache8_*`` calls: (slot, position of the first token, first row, tokens) each."""
+    return StepTable(entries, device)
+
+
+class Cache8:
+    """Keys and values in 8 bits: ``k`` [slots, kv_heads, max_len, dim] and ``v`` [.., vdim] float8_e4m3fn with a power-of-two scale
+    for each ``block`` tokens and kv head, ``k_scale`` / ``v_scale`` f32 [slots, kv_heads, ceil(max_len / block)].  ``weights`` f32 [slots,
+    kv_heads, max_len] or None: the attention weight that every cached token received."""
+
+    def __init__(self, k, v, k_scale, v_scale, block, weights=None):
+        slots, heads, cap, dim = k.shape
+        blocks = (cap + block - 1) // block
+        for t, dtype, shape, name in ((k, torch.float8_e4m3fn, (slots, heads, cap, dim), "k"),
+                                      (v, torch.float8_e4m3fn, (slots, heads, cap, v.shape[-1]), "v"),
+                                      (k_scale, _F32, (slots, heads, blocks), "k_scale"), (v_scale, _F32, (slots, heads, blocks), "v_scale"),
+                                      (weights, _F32, (slots, heads, cap), "weights")):
+            if t is None and name == "weights":
+                continue
+            _req(t, dtype, name)
+            if tuple(t.shape) != shape or not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"{name} must be a contiguous tensor of shape {shape} on {k.device}")
+        if block not in (16, 32, 64, 128) or dim % 16 or v.shape[-1] % 16 or not 0 < dim <= 128 or not 0 < v.shape[-1] <= 128:
+            raise ValueError("blocks are of 16, 32, 64 or 128 tokens, head sizes multiples of 16 up to 128")
+        self.k, self.v, self.k_scale, self.v_scale, self.weights, self.block, self.device = k, v, k_scale, v_scale, weights, block, k.device
+        self.shape = Cache8Shape(slots, heads, cap, dim, v.shape[-1], block)
+
+
+def cache8(slots, kv_heads, max_len, dim, vdim=None, block=64, weights=False, device="cuda"):
+    """An empty Cache8."""
+    vdim, blocks = dim if vdim is None else vdim, (max_len + block - 1) // block
+    of = lambda dtype, *shape: torch.zeros(slots, kv_heads, *shape, dtype=dtype, device=device)  # noqa: E731
+    return Cache8(of(torch.uint8, max_len, dim).view(torch.float8_e4m3fn), of(torch.uint8, max_len, vdim).view(torch.float8_e4m3fn),
+                  of(_F32, blocks), of(_F32, blocks), block, of(_F32, max_len) if weights else None)
+
+
+def _on(device, **tensors):
+    """Everything a call gets lies on the cache's device, which is the current one (the call goes to its current stream)."""
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device}, it is on {t.device}")
+
+
+def _head_rows(t, heads, dim, name):
+    """``t`` [rows, heads, dim] whose heads lie side by side -> distance of its rows."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim):
+        raise ValueError(f"{name} must be [rows, {heads}, {dim}] with its heads side by side")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * dim)
+
+
+def cache8_append(cache, k, v, table):
+    """Tokens k [rows, kv_heads, dim] and v [rows, kv_heads, vdim] (bf16 or f32) of the table's entries into the cache at their
+    positions.  The scale of a block that already holds older tokens of the sequence never shrinks, and they are held at the new
+    one; the new tokens' weights are set to zero."""
+    s = cache.shape
+    _on(cache.device, k=k, v=v, table=table.seqs)
+    _req(v, k.dtype, "v")
+    ldk, ldv = _head_rows(k, s.kv_heads, s.dim, "k"), _head_rows(v, s.kv_heads, s.vdim, "v")
+    if k.shape[0] != v.shape[0]:
+        raise ValueError("k and v have different numbers of rows")
+    check(lib.teeny_cache8_append(_f32_flag(k), s, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(cache.weights),
+                                  _ptr(k), ldk, _ptr(v), ldv, k.shape[0], _ptr(table.seqs), table.host, table.n, table.longest, _stream()),
+          "cache8_append")
+
+
+def cache8_attention_scratch(cache, table, q, weights=False):
+    """Scratch for calls with this many entries and rows (None: they need none).  Calls in one stream may share it."""
+    n = lib.teeny_cache8_attention_scratch_bytes(cache.shape, _f32_flag(q), q.shape[1], q.shape[0], table.n, table.longest, int(weights))
+    return torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+
+
+def cache8_attention(q, cache, score_scale, table, softcap=0.0, sink=None, gate=None, weight_decay=None, lse=None, out=None, scratch=None):
+    """Causal attention of the entries' tokens q [rows, heads, dim] (bf16 or f32) over the cache, which holds their own keys and values
+    already; ``softcap``, ``sink`` f32 [heads] and ``gate`` [rows, heads * vdim] as in cached_attention.  With ``weight_decay`` every live token's
+    weight becomes weight_decay * weight + the probabilities it got (0.0: those alone).  ``lse`` f32 [rows, heads] receives the logarithms of the
+    softmax denominators.  Returns [rows, heads, vdim]."""
+    s = cache.shape
+    _on(cache.device, q=q, table=table.seqs, sink=sink, gate=gate, lse=lse, out=out, scratch=scratch)
+    f32, heads = _f32_flag(q), q.shape[1]
+    ldq = _head_rows(q, heads, s.dim, "q")
+    rows = q.shape[0]
+    if out is None:
+        out = torch.zeros(rows, heads, s.vdim, dtype=q.dtype, device=q.device)
+    ldo = _head_rows(_req(out, q.dtype, "out"), heads, s.vdim, "out")
+    ldg = 0
+    if gate is not None:
+        if _req(gate, q.dtype, "gate").shape != (rows, heads * s.vdim) or gate.stride(1) != 1:
+            raise ValueError(f"gate must be [{rows}, {heads * s.vdim}]")
+        ldg = gate.stride(0) if rows > 1 else heads * s.vdim
+    if out.shape[0] != rows:
+        raise ValueError(f"out must have {rows} rows")
+    if sink is not None and (_req(sink, _F32, "sink").shape != (heads,) or not sink.is_contiguous()):
+        raise ValueError(f"sink must be [{heads}]")
+    if lse is not None and (_req(lse, _F32, "lse").shape != (rows, heads) or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous [{rows}, {heads}]")
+    count = weight_decay is not None
+    if count and cache.weights is None:
+        raise ValueError("this cache has no weights")
+    if scratch is None:
+        scratch = cache8_attention_scratch(cache, table, q, count)
+    check(lib.teeny_cache8_attention(f32, s, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale),
+                                     _ptr(cache.weights) if count else None, float(weight_decay) if count else 0.0, _ptr(q), ldq, _ptr(out), ldo,
+                                     rows, heads, float(score_scale), float(softcap), _ptr(sink), _ptr(gate), ldg, _ptr(lse), _ptr(scratch),
+                                     scratch.numel() if scratch is not None else 0, _ptr(table.seqs), table.host, table.n, table.longest,
+                                     _stream()), "cache8_attention")
+    return out
+
+
+def cache8_evict_scratch(cache, table, keep):
+    n = lib.teeny_cache8_evict_scratch_bytes(cache.shape, table.n, keep)
+    return torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+
+
+def cache8_evict(cache, table, keep, recent, kept=None, scratch=None):
+    """Thins out the slots of the table's entries, (slot, live tokens, 0, 0) each: every kv head keeps its last ``recent`` tokens and the ones with
+    the largest weights of the others, ``keep`` in all, moved to the front in their order.  The slot's next token goes to position min(live
+    tokens, keep).  Returns the kept tokens' indices before, int32 [entries, kv_heads, keep], -1 behind the last."""
+    s = cache.shape
+    if cache.weights is None:
+        raise ValueError("this cache has no weights")
+    shape = (table.n, s.kv_heads, keep)
+    if kept is None:
+        kept = torch.empty(shape, dtype=torch.int32, device=cache.device)
+    elif _req(kept, torch.int32, "kept").shape != shape or not kept.is_contiguous():
+        raise ValueError(f"kept must be a contiguous {shape}")
+    if scratch is None:
+        scratch = cache8_evict_scratch(cache, table, keep)
+    _on(cache.device, table=table.seqs, kept=kept, scratch=scratch)
+    check(lib.teeny_cache8_evict(s, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(cache.weights), keep, recent,
+                                 _ptr(kept), _ptr(scratch), scratch.numel() if scratch is not None else 0, _ptr(table.seqs), table.host,
+                                 table.n, _stream()), "cache8_evict")
+    return kept
