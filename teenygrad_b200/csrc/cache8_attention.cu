@@ -1,4 +1,20 @@
-// Causal attention over the 8-bit key/value cache (layout in teeny_cache8.h).
+// Causal attention over the 8-bit key/value cache (layout in teeny_cache8.h) for any number of query rows, and the weights that the cached tokens
+// receive.
+//
+// Both products run on E4M3 operands as they lie in the cache (mma.sync m16n8k32, f32 sums), which needs no conversion of keys and values: of
+// a 16-row tile, rows 0-7 hold the first E4M3 term of eight query rows and rows 8-15 the second, x = t0 + t1 / 16, which is a bf16
+// number exactly (each term has four of its eight bits; a row is scaled so that its largest number is in [128, 256), below 2^-20 of that a
+// rest is cut).  f32 rows take three such tiles, six terms.  The two halves of a sum lie in the same thread's registers.  Probabilities are split
+// the same way, relative to the largest one of the 32 keys that a warp takes at a time, so that no product depends on how far a
+// key is below the row's maximum.  Scales of key blocks multiply the scores; those of value blocks, relative to the larger one of the 32
+// keys, the probabilities.
+//
+// The call is bound by reading the cache.  A producer warp keeps a ring of 32 KB stages in flight (128 keys and their values by TMA, their scales by
+// 4-byte asynchronous copies on the same barrier); a consumer warp owns 32 keys of a tile.  Work is divided evenly by tiles: entry after
+// entry, head after head, row group after row group, each CTA takes the same number of consecutive tiles of all of them, whatever the
+// lengths.  A sequence that lies in several CTAs' shares leaves partial results in scratch, at most two for each CTA, which a second kernel adds.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "mma.cuh"
@@ -7,109 +23,827 @@ namespace teeny {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kTile = 128;                     // keys of a stage
+constexpr int kBox = kTile * kCache8Head;      // 16 KB: their keys, or their values (narrower heads are filled up with zeros by the copies)
+constexpr int kGroups = kTile / 16;            // scales are kept for groups of 16 keys
+constexpr int kStage = 2 * kBox;
 
+// Variant of the kernel: TP tiles of two terms each (1: bf16, 3: f32), MT x 8 query rows, NG groups of four consumer warps.  Eight bf16 rows fit 168
+// registers, with two CTAs of five warps on an SM; more rows, and f32's, take one CTA with two groups, to which the producer's warpgroup leaves its registers
+// (128 * 40 + 256 * 224 of the 384 * 168 that the CTA has).
+template <int TP, int MT, int NG>
+struct Variant {
+  static constexpr int kRows = 8 * MT, kWarps = 4 * NG, kThreads = NG == 1 ? 160 : 384;
+  static constexpr int kStages = NG == 1 ? 3 : 6;
+  static constexpr int kScales = kStages * kStage;                        // f32 [stages][2][kGroups]
+  static constexpr int kQ = kScales + kStages * 2 * kGroups * 4;          // uint4 [MT][TP][4 steps][32 lanes]
+  static constexpr int kMerge = kQ + MT * TP * 4 * 32 * 16;               // f32 [kWarps / 2][32 values][32 lanes]
+  static constexpr int kML = kMerge + kWarps / 2 * 32 * 32 * 4;           // f32 [kWarps][kRows][2]
+  static constexpr int kNan = kML + kWarps * kRows * 8;                   // int [128]
+  static constexpr int kBars = kNan + 128 * 4;
+  static constexpr int kBytes = kBars + 2 * kStages * 8 + 1024;
+  static_assert(kBytes <= (NG == 1 ? 115600 : 232000), "shared memory");
+};
+
+__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 halves(unsigned short two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// The first E4M3 term of two numbers; x, y become what is left of them, times 16.
+__device__ __forceinline__ unsigned short take_term(float& x, float& y) {
+  const unsigned short t = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+  const float2 f = halves(t);
+  x = (x - f.x) * 16.0f;
+  y = (y - f.y) * 16.0f;
+  return t;
+}
 __device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ void store_one(bf16* p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void store_one(float* p, float x) { *p = x; }
-__device__ __forceinline__ float4 decode4(uint32_t w) {
-  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
-  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ float capped(float s, float softcap) { return softcap > 0.0f ? softcap * tanhf(s / softcap) : s; }
 
-// One CTA of four warps for a (row, query head); warp w takes the keys w, w + 4, .., lane l the dimensions 4l .. 4l + 3.
-template <typename T>
-__global__ void __launch_bounds__(128) cache8_rows_kernel(const Cache8 c, const Cache8Attn a, const SeqDesc* seqs, int max_len, float* lse_out) {
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][kCache8Head];
-  pdl_wait();
-  const SeqDesc sq = seqs[blockIdx.y];
-  const int i = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, hk = h / (a.Hq / c.H);
-  if (!cache8_fits(sq, c, a.rows, max_len) || i >= sq.len) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, live = sq.pos + i + 1;
-  const size_t row = sq.row0 + i, head = static_cast<size_t>(sq.slot) * c.H + hk;
-  float q[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) q[e] = 4 * lane < c.D ? load_one(static_cast<const T*>(a.q) + row * a.ldq + h * c.D + 4 * lane + e) : 0.0f;
-  for (int j = warp; j < live; j += 4) {
-    float s = 0.0f;
-    if (4 * lane < c.D) {
-      const float4 x = decode4(*reinterpret_cast<const uint32_t*>(c.k + (head * c.cap + j) * c.D + 4 * lane));
-      s = q[0] * x.x + q[1] * x.y + q[2] * x.z + q[3] * x.w;
-    }
-    s = capped(warp_sum(s) * c.ks[head * c.blocks + j / c.B] * a.scale, a.softcap);
-    const float top = fmaxf(m, s), old = m == -INFINITY ? 0.0f : expf(m - top), p = expf(s - top);
-    m = top;
-    l = l * old + p;
-    if (4 * lane < c.V) {
-      const float4 x = decode4(*reinterpret_cast<const uint32_t*>(c.v + (head * c.cap + j) * c.V + 4 * lane));
-      const float pv = p * c.vs[head * c.blocks + j / c.B];
-      o[0] = o[0] * old + pv * x.x; o[1] = o[1] * old + pv * x.y; o[2] = o[2] * old + pv * x.z; o[3] = o[3] * old + pv * x.w;
-    }
-  }
-  if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sm_o[warp][4 * lane + e] = o[e];
-  __syncthreads();
-  float top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3])), sum = 0.0f, x = 0.0f;
-  const int d = threadIdx.x;
-  for (int w = 0; w < 4; ++w) {
-    const float f = sm_m[w] == -INFINITY ? 0.0f : expf(sm_m[w] - top);
-    sum += sm_l[w] * f;
-    x += sm_o[w][d] * f;
-  }
-  if (a.sink) sum += expf(a.sink[h] - top);
-  if (lse_out && d == 0) lse_out[row * a.Hq + h] = top + logf(sum);
-  if (d >= c.V) return;
-  x /= sum;
-  if (a.gate) x *= sigmoid_f(load_one(static_cast<const T*>(a.gate) + row * a.ldg + h * c.V + d));
-  store_one(static_cast<T*>(a.out) + row * a.ldo + h * c.V + d, x);
+struct Shared {  // what a call's kernels share
+  Cache8 c;
+  Cache8Attn a;
+  const SeqDesc* seqs;
+  int n_seqs, max_len, G;
+  float scale_log2, two_over_cap, cap_l2;
+  float* part_o;   // [2 * CTAs][rows of a unit][128]
+  float* part_ml;  // [2 * CTAs][rows of a unit][2]
+  float* lse2;     // [rows][Hq], base 2, or null
+  float* scores;   // [entries][Hq][cap] base 2, or null
+  int parts;       // CTAs of the main kernel
+  int vec_q, vec_o;
+  int* err;
+};
+
+// Tiles of an entry: its units are (head, row group), each over all its tiles.
+struct EntryShape { int tiles, groups; long long all; };
+__device__ __forceinline__ EntryShape entry_shape(const Shared& s, const SeqDesc& sq, int rows) {
+  EntryShape e{0, 0, 0};
+  if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return e;
+  e.tiles = (sq.pos + sq.len + kTile - 1) / kTile;
+  e.groups = static_cast<int>((static_cast<long long>(sq.len) * s.G + rows - 1) / rows);
+  e.all = static_cast<long long>(e.tiles) * e.groups * s.c.H;
+  return e;
+}
+// CTA p's share of the tiles; with fewer tiles than CTAs the first ones take one each (no share between two others is ever empty).
+__device__ __forceinline__ long long share_begin(long long total, int part, int parts) {
+  return total <= parts ? min(total, static_cast<long long>(part)) : total * part / parts;
 }
 
-// A warp for a (key, kv head): the probabilities that the entry's rows gave it, from the rows' lse.
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Output element of query head h in row `row`: o unnormalised, l the row sum (with the sink's part).
 template <typename T>
-__global__ void __launch_bounds__(128) cache8_weights_kernel(const Cache8 c, const Cache8Attn a, const SeqDesc* seqs, int max_len, const float* lse) {
-  pdl_wait();
-  const SeqDesc sq = seqs[blockIdx.z];
-  if (!cache8_fits(sq, c, a.rows, max_len)) return;
-  const int hk = blockIdx.y, lane = threadIdx.x & 31, group = a.Hq / c.H;
-  for (int j = blockIdx.x * 4 + (threadIdx.x >> 5); j < sq.pos + sq.len; j += gridDim.x * 4) {
-    const size_t head = static_cast<size_t>(sq.slot) * c.H + hk;
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (4 * lane < c.D) x = decode4(*reinterpret_cast<const uint32_t*>(c.k + (head * c.cap + j) * c.D + 4 * lane));
-    const float scale = c.ks[head * c.blocks + j / c.B] * a.scale;
-    float sum = 0.0f;
-    for (int i = max(0, j - sq.pos); i < sq.len; ++i)
-      for (int g = 0; g < group; ++g) {
-        const size_t row = sq.row0 + i;
-        const T* q = static_cast<const T*>(a.q) + row * a.ldq + (hk * group + g) * c.D + 4 * lane;
-        float s = 0.0f;
-        if (4 * lane < c.D) s = load_one(q) * x.x + load_one(q + 1) * x.y + load_one(q + 2) * x.z + load_one(q + 3) * x.w;
-        sum += expf(capped(warp_sum(s) * scale, a.softcap) - lse[row * a.Hq + hk * group + g]);
+__device__ __forceinline__ float finished(const Shared& s, size_t row, int h, int d, float o, float inv) {
+  o *= inv;
+  if (s.a.gate) o *= sigmoid_f(load_one(static_cast<const T*>(s.a.gate) + row * s.a.ldg + static_cast<size_t>(h) * s.c.V + d));
+  return o;
+}
+__device__ __forceinline__ void note_lse(const Shared& s, size_t row, int h, float lse2) {
+  if (s.lse2) s.lse2[row * s.a.Hq + h] = lse2;
+  if (s.a.lse) s.a.lse[row * s.a.Hq + h] = lse2 * kLn2;
+}
+// 16 finished numbers of a row
+__device__ __forceinline__ void store16(bf16* p, const float (&x)[16], bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
+                                                  pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) store_one(p + i, x[i]);
+  }
+}
+__device__ __forceinline__ void store16(float* p, const float (&x)[16], bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = x[i];
+  }
+}
+
+// Terms of one query row, of which this lane (c = lane % 4) has the dimensions 32 c .. 32 c + 31, as the words of a lane's A fragments: word w of the
+// steps' eight is dimensions 32 c + 4 w ..; term[t][w].  Returns the factor that takes a sum of terms back (base-2 scores).
+template <typename T, int TERMS>
+__device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool vec, int c, float scale_log2, uint32_t (&term)[TERMS][8]) {
+  float x[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = 0.0f;
+  if (valid) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d0 = 32 * c + 16 * h;
+      if (d0 >= dim) continue;
+      if (vec && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + d0 + 8 * i);
+          const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { x[16 * h + 8 * i + 2 * e] = bf16_lo(r[e]); x[16 * h + 8 * i + 2 * e + 1] = bf16_hi(r[e]); }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[16 * h + i] = load_one(q + d0 + i);
       }
-    float* w = c.w + head * c.cap + j;
-    if (lane == 0) *w = a.decay == 0.0f ? sum : a.decay * *w + sum;
+    }
+  }
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const int p = split_scale_exponent(amax);
+  const float up = exp2f(static_cast<float>(p));
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    // (an infinity would saturate: it has to stay what it is, not a number of E4M3's range)
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = fabsf(x[4 * w + e]) < INFINITY ? x[4 * w + e] * up : __uint_as_float(0x7fffffffu);
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      const uint32_t lo = take_term(y[0], y[1]), hi = take_term(y[2], y[3]);
+      term[t][w] = lo | hi << 16;
+    }
+  }
+  return exp2f(static_cast<float>(-p)) * scale_log2;
+}
+
+template <typename T, int TP, int MT, int NG>
+__global__ void __launch_bounds__(Variant<TP, MT, NG>::kThreads, NG == 1 ? 2 : 1)
+cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Shared s) {
+  using V = Variant<TP, MT, NG>;
+  constexpr int R = V::kRows, W = V::kWarps;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long sm_first[3];  // total tiles, entry of this CTA's first tile, tiles of that entry before it
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  auto full_bar = [&](int st) { return base + V::kBars + 8u * st; };
+  auto empty_bar = [&](int st) { return base + V::kBars + 8u * (V::kStages + st); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+    for (int st = 0; st < V::kStages; ++st) {
+      mbar_init(full_bar(st), 1 + 2 * kGroups);
+      mbar_init(empty_bar(st), 4);
+    }
+    mbar_fence_init();
+  }
+  pdl_wait();
+  if (warp == 0) {
+    long long total = 0;
+    for (int e = lane; e < s.n_seqs; e += 32) total += entry_shape(s, s.seqs[e], R).all;
+    total = warp_sum_ll(total);
+    const long long t0 = share_begin(total, blockIdx.x, s.parts);
+    long long before = 0;
+    for (int e0 = 0; e0 < s.n_seqs; e0 += 32) {
+      const long long mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
+      long long run = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += up;
+      }
+      const long long end = before + run;
+      if (mine > 0 && t0 >= end - mine && t0 < end) {
+        sm_first[1] = e0 + lane;
+        sm_first[2] = t0 - (end - mine);
+      }
+      before = __shfl_sync(0xffffffffu, end, 31);
+      if (before > t0) break;
+    }
+    if (lane == 0) sm_first[0] = total;
+  }
+  __syncthreads();
+  const long long total = sm_first[0], t0 = share_begin(total, blockIdx.x, s.parts), t1 = share_begin(total, blockIdx.x + 1, s.parts);
+  if (t0 >= t1) return;
+
+  // body(entry, its table row, head, row group, first and last tile, whole unit?, first segment?) for every piece of this CTA's share
+  auto walk = [&](auto&& body) {
+    long long done = t0, at = sm_first[2];
+    for (int e = static_cast<int>(sm_first[1]); done < t1; ++e, at = 0) {
+      const SeqDesc sq = s.seqs[e];
+      const EntryShape es = entry_shape(s, sq, R);
+      while (at < es.all && done < t1) {
+        const int unit = static_cast<int>(at / es.tiles), j0 = static_cast<int>(at - static_cast<long long>(unit) * es.tiles);
+        const int j1 = static_cast<int>(min(static_cast<long long>(es.tiles), j0 + (t1 - done)));
+        const int hk = unit / es.groups, rg = unit - hk * es.groups;
+        // keys that the group's last row sees
+        const int last = min(sq.len - 1, static_cast<int>((static_cast<long long>(rg) * R + R - 1) / s.G)), limit = sq.pos + last + 1;
+        if (!body(e, sq, hk, rg, j0, min(j1, (limit + kTile - 1) / kTile), limit, j0 == 0 && j1 == es.tiles, done == t0)) return;
+        at += j1 - j0;
+        done += j1 - j0;
+      }
+    }
+  };
+
+  if (warp >= W) {
+    // ---------------- producer ----------------
+    if (NG > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp > W) return;
+    int st = 0;
+    uint32_t ph = 0;
+    walk([&](int, const SeqDesc& sq, int hk, int, int j0, int j1, int limit, bool, bool) {
+      const size_t srow = (static_cast<size_t>(sq.slot) * s.c.H + hk) * s.c.blocks;
+      for (int j = j0; j < j1; ++j) {
+        if (!mbar_wait(empty_bar(st), ph ^ 1, s.err, DEVERR_ATTN_PRODUCER)) return false;
+        const int key0 = j * kTile;
+        if (lane < 2 * kGroups) {
+          const int key = key0 + 16 * (lane & (kGroups - 1));
+          const float* src = (lane < kGroups ? s.c.ks : s.c.vs) + srow + (key < limit ? key / s.c.B : 0);
+          const uint32_t bytes = key < limit ? 4 : 0;  // (0: zero is written; blocks behind the last key may hold anything)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n\tcp.async.mbarrier.arrive.noinc.shared::cta.b64 [%3];"
+                       ::"r"(base + V::kScales + (st * 2 * kGroups + lane) * 4), "l"(src), "r"(bytes), "r"(full_bar(st)) : "memory");
+        }
+        if (lane == 0) {
+          mbar_expect_tx(full_bar(st), kStage);
+          tma_load_4d(base + st * kStage, &tmap_k, full_bar(st), 0, key0, hk, sq.slot);
+          tma_load_4d(base + st * kStage + kBox, &tmap_v, full_bar(st), 0, key0, hk, sq.slot);
+        }
+        if (++st == V::kStages) { st = 0; ph ^= 1; }
+      }
+      return true;
+    });
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  if (NG > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+  const int g = lane >> 2, c = lane & 3, quarter = warp & 3, ng = warp >> 2;
+  float* sm_ml = reinterpret_cast<float*>(gen + V::kML);
+  int* sm_nan = reinterpret_cast<int*>(gen + V::kNan);
+  int count = 0;  // tiles of this CTA so far
+  walk([&](int e, const SeqDesc& sq, int hk, int rg, int j0, int j1, int limit, bool whole, bool first) {
+    // ---- query terms: row tile mt by warp mt (mod W), into shared memory as A fragments ----
+    float factor[MT];
+    int rows_limit[MT];  // keys that this lane's rows see
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const long long r = static_cast<long long>(rg) * R + mt * 8 + g;
+      const int i = static_cast<int>(r / s.G), h = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+      const bool valid = i < sq.len;
+      rows_limit[mt] = valid ? sq.pos + i + 1 : limit;
+      if (mt % W == warp) {
+        uint32_t term[2 * TP][8];
+        const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(h) * s.c.D;
+        const float f = split_row<T, 2 * TP>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
+#pragma unroll
+        for (int tp = 0; tp < TP; ++tp)
+#pragma unroll
+          for (int step = 0; step < 4; ++step)
+            reinterpret_cast<uint4*>(gen + V::kQ)[((mt * TP + tp) * 4 + step) * 32 + lane] =
+                make_uint4(term[2 * tp][2 * step], term[2 * tp + 1][2 * step], term[2 * tp][2 * step + 1], term[2 * tp + 1][2 * step + 1]);
+        if (c == 0) sm_ml[mt * 8 + g] = f;
+      }
+    }
+    for (int d = threadIdx.x; d < 128; d += 32 * W) sm_nan[d] = 0x7fffffff;
+    named_barrier_sync(1, 32 * W);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) factor[mt] = sm_ml[mt * 8 + g];
+
+    float m[MT], l[MT];
+    f32x2 acc[MT][16];  // dimensions 32 c + n and 32 c + 16 + n
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt] = -INFINITY;
+      l[mt] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) acc[mt][n] = 0ull;
+    }
+    bool ok = true;
+    for (int j = j0; j < j1; ++j, ++count) {
+      if (NG > 1 && count % NG != ng) continue;
+      const int st = count % V::kStages;
+      if (!mbar_wait(full_bar(st), count / V::kStages & 1, s.err, DEVERR_ATTN_SOFTMAX)) { ok = false; break; }
+      const int kb = j * kTile + 32 * quarter;
+      if (kb < limit) {
+        const uint32_t kt = base + st * kStage + (32 * quarter + g) * 128, vt = base + st * kStage + kBox + 32 * quarter * 128;
+        const uint32_t sc = base + V::kScales + st * 2 * kGroups * 4 + 2 * quarter * 4;
+        const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + kGroups * 4), vs1 = lds32(sc + kGroups * 4 + 4);
+        const bool masked = kb + 32 > sq.pos + 1;
+        // ---- scores: key 8 t + g of the warp's 32 is column g of block t; lane c reads the dimensions whose terms it holds of the query ----
+        uint4 kw[4][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) kw[t][h] = lds128(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
+        uint4 pf[MT][TP];
+        float alpha[MT], beta[MT];
+        const float vmax = fmaxf(vs0, vs1);
+        float r0 = 256.0f, r1 = 256.0f;
+        if (vs0 != vs1) {
+          const float inv = vmax > 0.0f ? 256.0f / vmax : 0.0f;
+          r0 = vs0 * inv;
+          r1 = vs1 * inv;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float x[4][2];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) x[t][0] = x[t][1] = 0.0f;
+#pragma unroll
+          for (int tp = TP - 1; tp >= 0; --tp) {
+            uint4 qa[4];
+#pragma unroll
+            for (int step = 0; step < 4; ++step) qa[step] = lds128(base + V::kQ + (((mt * TP + tp) * 4 + step) * 32 + lane) * 16);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma_e4m3_16832(d, qa[0], kw[t][0].x, kw[t][0].y);
+              mma_e4m3_16832(d, qa[1], kw[t][0].z, kw[t][0].w);
+              mma_e4m3_16832(d, qa[2], kw[t][1].x, kw[t][1].y);
+              mma_e4m3_16832(d, qa[3], kw[t][1].z, kw[t][1].w);
+              x[t][0] = fmaf(x[t][0], 1.0f / 256.0f, fmaf(d[2], 0.0625f, d[0]));
+              x[t][1] = fmaf(x[t][1], 1.0f / 256.0f, fmaf(d[3], 0.0625f, d[1]));
+            }
+          }
+          const float f0 = factor[mt] * ks0, f1 = factor[mt] * ks1;
+          float top = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              float y = x[t][z] * (t < 2 ? f0 : f1);
+              if (s.cap_l2 > 0.0f) y = softcap_log2(y, s.two_over_cap, s.cap_l2);
+              if (masked && kb + 8 * t + 2 * c + z >= rows_limit[mt]) y = -INFINITY;
+              x[t][z] = y;
+              top = fmaxf(top, y);
+            }
+          if (s.scores) {
+            const int r = rg * R + mt * 8 + g;  // (single tokens: a row is a query head of the group)
+            if (r < s.G) {
+              float* to = s.scores + (static_cast<size_t>(e) * s.a.Hq + hk * s.G + r) * s.c.cap + kb + 2 * c;
+#pragma unroll
+              for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int z = 0; z < 2; ++z)
+                  if (!masked || kb + 8 * t + 2 * c + z < limit) to[8 * t + z] = x[t][z];
+            }
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float from = top == -INFINITY ? 0.0f : top, m_new = fmaxf(m[mt], top), to = m_new == -INFINITY ? 0.0f : m_new;
+          alpha[mt] = ex2(m[mt] - to);
+          beta[mt] = ex2(top - to);
+          m[mt] = m_new;
+          float sum = 0.0f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              x[t][z] = ex2(x[t][z] - from);
+              sum += x[t][z];
+              x[t][z] *= t < 2 ? r0 : r1;
+            }
+          l[mt] = fmaf(l[mt], alpha[mt], sum * beta[mt]);
+          beta[mt] *= vmax * (1.0f / 256.0f);
+          // A fragments of the values' product: keys 2c, 2c + 1 of blocks 0, 1 (then 2, 3)
+#pragma unroll
+          for (int tp = 0; tp < TP; ++tp) {
+            uint32_t w[2][2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t lo = take_term(x[2 * half][0], x[2 * half][1]), hi = take_term(x[2 * half + 1][0], x[2 * half + 1][1]);
+                w[z][half] = lo | hi << 16;
+              }
+            pf[mt][tp] = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
+          }
+        }
+        // ---- values: lane (g, c) reads the dimensions 16 g .. 16 g + 15 of the keys whose probabilities it holds; transposed by bytes they are the
+        // B fragments of 16 blocks of eight dimensions {16 g + n} ----
+        uint4 vw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+          vw[i] = lds128(vt + row * 128 + ((g ^ (row & 7)) << 4));
+        }
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = kb + 2 * c + (i & 1) + 8 * (i >> 1);
+            if (key >= limit) vw[i] = make_uint4(0u, 0u, 0u, 0u);  // stale rows may hold NaN, and 0 * NaN is NaN
+            if (sq.len > 1) {
+              // a NaN value counts only for the rows that see its key: noted, and put back when the rows are finished
+              uint32_t* word = &vw[i].x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if ((((word[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u)
+                  for (int b = 0; b < 4; ++b)
+                    if ((word[k] >> (8 * b) & 0x7fu) == 0x7fu) {
+                      word[k] &= ~(0xffu << (8 * b));
+                      atomicMin(&sm_nan[16 * g + 4 * k + b], key);
+                    }
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t b[2][4];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a0 = (&vw[4 * half].x)[k], a1 = (&vw[4 * half + 1].x)[k], a2 = (&vw[4 * half + 2].x)[k], a3 = (&vw[4 * half + 3].x)[k];
+            const uint32_t l01 = __byte_perm(a0, a1, 0x5140), h01 = __byte_perm(a0, a1, 0x7362);
+            const uint32_t l23 = __byte_perm(a2, a3, 0x5140), h23 = __byte_perm(a2, a3, 0x7362);
+            b[half][0] = __byte_perm(l01, l23, 0x5410);
+            b[half][1] = __byte_perm(l01, l23, 0x7632);
+            b[half][2] = __byte_perm(h01, h23, 0x5410);
+            b[half][3] = __byte_perm(h01, h23, 0x7632);
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const f32x2 al = pack2(alpha[mt], alpha[mt]), be = pack2(beta[mt], beta[mt]), sixteenth = pack2(0.0625f, 0.0625f);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              f32x2 o = 0ull;
+#pragma unroll
+              for (int tp = TP - 1; tp >= 0; --tp) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_e4m3_16832(d, pf[mt][tp], b[0][n], b[1][n]);
+                const f32x2 both = fma2(pack2(d[2], d[3]), sixteenth, pack2(d[0], d[1]));
+                o = tp == TP - 1 ? both : fma2(o, pack2(1.0f / 256.0f, 1.0f / 256.0f), both);
+              }
+              acc[mt][4 * k + n] = fma2(acc[mt][4 * k + n], al, mul2(o, be));
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_bar(st));
+    }
+    if (!ok) return false;
+
+    // ---- the warps' parts together ----
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 1);
+      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 2);
+    }
+    named_barrier_sync(1, 32 * W);  // (sm_ml held the rows' factors)
+    if (c == 0)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        sm_ml[(warp * R + mt * 8 + g) * 2] = m[mt];
+        sm_ml[(warp * R + mt * 8 + g) * 2 + 1] = l[mt];
+      }
+    named_barrier_sync(1, 32 * W);
+    f32x2* merge = reinterpret_cast<f32x2*>(gen + V::kMerge);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r8 = mt * 8 + g;
+      float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm_ml[(w * R + r8) * 2]);
+      const float to = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int w = 0; w < W; ++w) ll = fmaf(sm_ml[(w * R + r8) * 2 + 1], ex2(sm_ml[(w * R + r8) * 2] - to), ll);
+      const float f = ex2(m[mt] - to);
+#pragma unroll
+      for (int n = 0; n < 16; ++n) acc[mt][n] = mul2(acc[mt][n], pack2(f, f));
+#pragma unroll
+      for (int half = W / 2; half > 0; half >>= 1) {
+        if (warp >= half && warp < 2 * half)
+#pragma unroll
+          for (int n = 0; n < 16; ++n) merge[((warp - half) * 16 + n) * 32 + lane] = acc[mt][n];
+        named_barrier_sync(1, 32 * W);
+        if (warp < half)
+#pragma unroll
+          for (int n = 0; n < 16; ++n) acc[mt][n] = fma2(merge[(warp * 16 + n) * 32 + lane], pack2(1.0f, 1.0f), acc[mt][n]);
+        if (half > 1 || MT > 1) named_barrier_sync(1, 32 * W);
+      }
+      if (warp != 0) continue;
+      float o[2][16];
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        const float2 v = unpack2(acc[mt][n]);
+        o[0][n] = v.x;
+        o[1][n] = v.y;
+      }
+      if (sq.len > 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            if (rows_limit[mt] > sm_nan[32 * c + 16 * h + n]) o[h][n] = __uint_as_float(0x7fffffffu);
+      }
+      if (!whole) {
+        const size_t slot = (2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1)) * R + r8;
+        if (c == 0) {
+          s.part_ml[slot * 2] = mm;
+          s.part_ml[slot * 2 + 1] = ll;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) store16(s.part_o + slot * 128 + 32 * c + 16 * h, o[h], true);
+        continue;
+      }
+      const long long r = static_cast<long long>(rg) * R + r8;
+      const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+      if (i >= sq.len) continue;
+      const size_t row = static_cast<size_t>(sq.row0) + i;
+      if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
+      if (c == 0) note_lse(s, row, hq, mm + log2f(ll));
+      const float inv = 1.0f / ll;
+      T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d0 = 32 * c + 16 * h;
+        if (d0 >= s.c.V) continue;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) o[h][n] = finished<T>(s, row, hq, d0 + n, o[h][n], inv);
+        store16(out + d0, o[h], s.vec_o);
+      }
+    }
+    named_barrier_sync(1, 32 * W);  // the next unit writes what was read here
+    return true;
+  });
+}
+
+// Adds the parts of the units that lie in several CTAs' shares: one CTA for a unit, a warp for a row (mod 8), a lane for four dimensions.
+template <typename T>
+__global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_constant__ Shared s, int rows, int max_groups) {
+  __shared__ long long sums[8][2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int e = blockIdx.x / (s.c.H * max_groups), unit = blockIdx.x % (s.c.H * max_groups), hk = unit / max_groups, rg = unit % max_groups;
+  pdl_wait();
+  const SeqDesc sq = s.seqs[e];
+  const EntryShape es = entry_shape(s, sq, rows);
+  if (rg >= es.groups) return;
+  long long before = 0, total = 0;
+  for (int i = threadIdx.x; i < s.n_seqs; i += 256) {
+    const long long t = entry_shape(s, s.seqs[i], rows).all;
+    total += t;
+    if (i < e) before += t;
+  }
+  before = warp_sum_ll(before);
+  total = warp_sum_ll(total);
+  if (lane == 0) { sums[warp][0] = before; sums[warp][1] = total; }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) { before += sums[w][0]; total += sums[w][1]; }
+  const long long u0 = before + (static_cast<long long>(hk) * es.groups + rg) * es.tiles, u1 = u0 + es.tiles;
+  auto owner = [&](long long tile) { return static_cast<int>(total <= s.parts ? tile : ((tile + 1) * s.parts - 1) / total); };
+  const int c0 = owner(u0), c1 = owner(u1 - 1);
+  if (c0 == c1) return;
+  const int slot0 = 2 * c0 + (share_begin(total, c0, s.parts) == u0 ? 0 : 1);
+  for (int r8 = warp; r8 < rows; r8 += 8) {
+    const long long r = static_cast<long long>(rg) * rows + r8;
+    const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+    if (i >= sq.len) break;
+    auto place = [&](int part) { return static_cast<size_t>(part == c0 ? slot0 : 2 * part) * rows + r8; };
+    float mm = -INFINITY, ll = 0.0f;
+    for (int p = c0 + lane; p <= c1; p += 32) mm = fmaxf(mm, s.part_ml[place(p) * 2]);
+    mm = warp_max(mm);
+    const float to = mm == -INFINITY ? 0.0f : mm;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = c0; p <= c1; ++p) {
+      const float pm = s.part_ml[place(p) * 2];
+      if (pm == -INFINITY && s.part_ml[place(p) * 2 + 1] == 0.0f) continue;  // no key of this row: nothing was written but that
+      const float f = ex2(pm - to);
+      const float4 x = *reinterpret_cast<const float4*>(s.part_o + place(p) * 128 + 4 * lane);
+      ll = fmaf(s.part_ml[place(p) * 2 + 1], f, ll);
+      o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+    }
+    const size_t row = static_cast<size_t>(sq.row0) + i;
+    if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
+    if (lane == 0) note_lse(s, row, hq, mm + log2f(ll));
+    const float inv = 1.0f / ll;
+    T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 4 * lane;
+    if (4 * lane >= s.c.V) continue;
+    const float y[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int d = 0; d < 4; ++d) store_one(out + d, finished<T>(s, row, hq, 4 * lane + d, y[d], inv));
   }
 }
+
+// Weights of single tokens' calls, from the scores that the attention kernel left: blockIdx = (share of the keys, kv head, entry).
+__global__ void __launch_bounds__(256) cache8_weights_kernel(const __grid_constant__ Shared s) {
+  pdl_wait();
+  const int e = blockIdx.z, hk = blockIdx.y;
+  const SeqDesc sq = s.seqs[e];
+  if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return;
+  float* w = s.c.w + (static_cast<size_t>(sq.slot) * s.c.H + hk) * s.c.cap;
+  const float* x = s.scores + (static_cast<size_t>(e) * s.a.Hq + hk * s.G) * s.c.cap;
+  const float* z = s.lse2 + static_cast<size_t>(sq.row0) * s.a.Hq + hk * s.G;
+  for (int j = blockIdx.x * 256 + threadIdx.x; j <= sq.pos; j += gridDim.x * 256) {
+    float sum = 0.0f;
+    for (int h = 0; h < s.G; ++h) sum += ex2(x[static_cast<size_t>(h) * s.c.cap + j] - z[h]);
+    w[j] = s.a.decay == 0.0f ? sum : fmaf(s.a.decay, w[j], sum);
+  }
+}
+
+// Weights of calls with several tokens: the scores once more, from the rows' lse.  A warp takes 32 keys of a (kv head, entry) and goes through the
+// rows eight at a time.
+template <typename T, int TP>
+__global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_constant__ Shared s) {
+  pdl_wait();
+  const int e = blockIdx.z, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const SeqDesc sq = s.seqs[e];
+  if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return;
+  const int live = sq.pos + sq.len;
+  const size_t head = static_cast<size_t>(sq.slot) * s.c.H + hk;
+  for (int kb = (blockIdx.x * 4 + warp) * 32; kb < live; kb += gridDim.x * 128) {
+    uint4 kw[4][2];
+    float ks[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int key = kb + 8 * t + g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d0 = 16 * (2 * c + h);
+        kw[t][h] = key < live && d0 < s.c.D ? *reinterpret_cast<const uint4*>(s.c.k + (head * s.c.cap + key) * s.c.D + d0) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    ks[0] = s.c.ks[head * s.c.blocks + kb / s.c.B];
+    ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + (kb + 16) / s.c.B] : 0.0f;
+    float sum[4][2] = {};
+    const long long rows = static_cast<long long>(sq.len) * s.G;
+    for (long long r0 = static_cast<long long>(max(0, kb - sq.pos)) * s.G / 8 * 8; r0 < rows; r0 += 8) {
+      const long long r = r0 + g;
+      const int i = static_cast<int>(min(r, rows - 1) / s.G), hq = hk * s.G + static_cast<int>(min(r, rows - 1) - static_cast<long long>(i) * s.G);
+      const size_t row = static_cast<size_t>(sq.row0) + i;
+      uint32_t term[2 * TP][8];
+      const float f = split_row<T, 2 * TP>(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c,
+                                           s.scale_log2, term);
+      const float z = s.lse2[row * s.a.Hq + hq];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float x[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int tp = TP - 1; tp >= 0; --tp) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int step = 0; step < 4; ++step) {
+            const uint4 a = make_uint4(term[2 * tp][2 * step], term[2 * tp + 1][2 * step], term[2 * tp][2 * step + 1], term[2 * tp + 1][2 * step + 1]);
+            const uint4& k = kw[t][step >> 1];
+            mma_e4m3_16832(d, a, step & 1 ? k.z : k.x, step & 1 ? k.w : k.y);
+          }
+          x[0] = fmaf(x[0], 1.0f / 256.0f, fmaf(d[2], 0.0625f, d[0]));
+          x[1] = fmaf(x[1], 1.0f / 256.0f, fmaf(d[3], 0.0625f, d[1]));
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float v = x[y] * (f * ks[t >> 1]);
+          if (s.cap_l2 > 0.0f) v = softcap_log2(v, s.two_over_cap, s.cap_l2);
+          if (r < rows && kb + 8 * t + 2 * c + y <= sq.pos + i) sum[t][y] += ex2(v - z);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum[t][y] += __shfl_xor_sync(0xffffffffu, sum[t][y], o);
+        const int key = kb + 8 * t + 2 * c + y;
+        float* w = s.c.w + head * s.c.cap + key;
+        if (g == 0 && key < live) *w = s.a.decay == 0.0f ? sum[t][y] : fmaf(s.a.decay, *w, sum[t][y]);
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct Plan {
+  int mt, parts, groups;
+  size_t part_o, part_ml, lse2, scores, bytes;
+};
+int row_tiles(int f32, int G, int max_len) {
+  // as few passes over the keys as rows allow, and no more row tiles than those need
+  const int most = f32 ? 2 : 4;
+  const long long rows = static_cast<long long>(G) * max_len, passes = (rows + 8 * most - 1) / (8 * most);
+  return static_cast<int>((rows + 8 * passes - 1) / (8 * passes));
+}
+Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights) {
+  Plan p{};
+  const int G = Hq / c.H;
+  p.mt = row_tiles(f32, G, max_len);
+  p.groups = static_cast<int>((static_cast<long long>(G) * max_len + 8 * p.mt - 1) / (8 * p.mt));
+  p.parts = sm_count() * (!f32 && p.mt == 1 ? 2 : 1);  // (the CTAs that are resident at once)
+  auto take = [&](size_t n) { const size_t at = p.bytes; p.bytes += (n + 255) / 256 * 256; return at; };
+  p.part_o = take(static_cast<size_t>(2) * p.parts * 8 * p.mt * 128 * 4);
+  p.part_ml = take(static_cast<size_t>(2) * p.parts * 8 * p.mt * 2 * 4);
+  p.lse2 = weights ? take(static_cast<size_t>(rows) * Hq * 4) : 0;
+  p.scores = weights && max_len == 1 ? take(static_cast<size_t>(n_seqs) * Hq * c.cap * 4) : 0;
+  return p;
+}
+
+template <typename F>
+void for_variant(int f32, int mt, F&& f) {
+  if (f32) {
+    if (mt == 1) f(cache8_attention_kernel<float, 3, 1, 2>, Variant<3, 1, 2>{});
+    else f(cache8_attention_kernel<float, 3, 2, 2>, Variant<3, 2, 2>{});
+  } else {
+    if (mt == 1) f(cache8_attention_kernel<bf16, 1, 1, 1>, Variant<1, 1, 1>{});
+    else if (mt == 2) f(cache8_attention_kernel<bf16, 1, 2, 2>, Variant<1, 2, 2>{});
+    else if (mt == 3) f(cache8_attention_kernel<bf16, 1, 3, 2>, Variant<1, 3, 2>{});
+    else f(cache8_attention_kernel<bf16, 1, 4, 2>, Variant<1, 4, 2>{});
+  }
+}
+int prepare() {
+  static std::atomic<unsigned long long> done{0};  // one bit per device; threads may race to set it
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && (done.load(std::memory_order_acquire) >> dev) & 1ull) return 0;
+  cudaError_t e = cudaSuccess;
+  for (int f32 = 0; f32 < 2; ++f32)
+    for (int mt = 1; mt <= (f32 ? 2 : 4); ++mt)
+      for_variant(f32, mt, [&](auto kernel, auto v) {
+        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(v)::kBytes);
+        if (e == cudaSuccess) e = rc;
+      });
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return 0;
+}
+int encode_codes(CUtensorMap* map, const uint8_t* base, int d, const Cache8& c) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(c.cap), static_cast<uint64_t>(c.H), static_cast<uint64_t>(c.slots)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(d) * c.cap, static_cast<uint64_t>(d) * c.cap * c.H};
+  const uint32_t box[4] = {kCache8Head, kTile, 1, 1};
+  return encode_tensor_map_u8(map, base, 4, dims, strides, box);
+}
+struct PdlScope {  // kernels of a call behind its first one start their set-up while it ends
+  bool was = pdl_enabled();
+  PdlScope() { pdl_set_enabled(true); }
+  ~PdlScope() { pdl_set_enabled(was); }
+};
 
 }  // namespace
 
-size_t cache8_attention_scratch_bytes(const Cache8&, int, int Hq, int rows, int, int, bool weights) {
-  return weights ? static_cast<size_t>(rows) * Hq * 4 : 0;
+size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights) {
+  return plan_of(c, f32, Hq, rows, n_seqs, max_len, weights).bytes;
 }
 
 int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc*, int n_seqs, int max_len, cudaStream_t st) {
-  float* lse = a.lse ? a.lse : a.weights ? static_cast<float*>(a.scratch) : nullptr;
-  const dim3 grid(static_cast<unsigned>(max_len) * a.Hq, n_seqs);
-  if (a.f32) launch_kernel(cache8_rows_kernel<float>, grid, dim3(128), 0, st, 1, c, a, seqs, max_len, lse);
-  else launch_kernel(cache8_rows_kernel<bf16>, grid, dim3(128), 0, st, 1, c, a, seqs, max_len, lse);
+  if (const int rc = prepare()) return rc;
+  const Plan p = plan_of(c, a.f32, a.Hq, a.rows, n_seqs, max_len, a.weights != 0);
+  CUtensorMap mk, mv;
+  if (const int rc = encode_codes(&mk, c.k, c.D, c)) return rc;
+  if (const int rc = encode_codes(&mv, c.v, c.V, c)) return rc;
+  Shared s{};
+  s.c = c;
+  s.a = a;
+  s.seqs = seqs;
+  s.n_seqs = n_seqs;
+  s.max_len = max_len;
+  s.G = a.Hq / c.H;
+  s.scale_log2 = a.scale * kLog2e;
+  if (a.softcap > 0.0f) {
+    s.two_over_cap = 2.0f / a.softcap;
+    s.cap_l2 = a.softcap * kLog2e;
+  }
+  uint8_t* scratch = static_cast<uint8_t*>(a.scratch);
+  s.part_o = reinterpret_cast<float*>(scratch + p.part_o);
+  s.part_ml = reinterpret_cast<float*>(scratch + p.part_ml);
+  if (a.weights) s.lse2 = reinterpret_cast<float*>(scratch + p.lse2);
+  if (a.weights && max_len == 1) s.scores = reinterpret_cast<float*>(scratch + p.scores);
+  s.parts = p.parts;
+  const int size = a.f32 ? 4 : 2;
+  s.vec_q = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.ldq * size)) & 15) == 0;
+  s.vec_o = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) & 15) == 0;
+  s.err = device_error_word();
+  if (!s.err) return TEENY_ERR_DRIVER;
+  for_variant(a.f32, p.mt, [&](auto kernel, auto v) {
+    using V = decltype(v);
+    launch_kernel(kernel, dim3(p.parts), dim3(V::kThreads), V::kBytes, st, 1, mk, mv, s);
+  });
+  const PdlScope behind;
+  const dim3 units(static_cast<unsigned>(n_seqs) * c.H * p.groups);
+  if (a.f32) launch_kernel(cache8_combine_kernel<float>, units, dim3(256), 0, st, 1, s, 8 * p.mt, p.groups);
+  else launch_kernel(cache8_combine_kernel<bf16>, units, dim3(256), 0, st, 1, s, 8 * p.mt, p.groups);
   if (a.weights) {
-    const dim3 wgrid(512, c.H, n_seqs);
-    if (a.f32) launch_kernel(cache8_weights_kernel<float>, wgrid, dim3(128), 0, st, 1, c, a, seqs, max_len, static_cast<const float*>(lse));
-    else launch_kernel(cache8_weights_kernel<bf16>, wgrid, dim3(128), 0, st, 1, c, a, seqs, max_len, static_cast<const float*>(lse));
+    const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
+    const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
+    if (max_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);
+    else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float, 3>, grid, dim3(128), 0, st, 1, s);
+    else launch_kernel(cache8_rows_weights_kernel<bf16, 1>, grid, dim3(128), 0, st, 1, s);
   }
   return static_cast<int>(cudaGetLastError());
 }
