@@ -9,10 +9,11 @@
 // key is below the row's maximum.  Scales of key blocks multiply the scores; those of value blocks, relative to the larger one of the 32
 // keys, the probabilities.
 //
-// The call is bound by reading the cache.  A producer warp keeps a ring of 32 KB stages in flight (128 keys and their values by TMA, their scales by
-// 4-byte asynchronous copies on the same barrier); a consumer warp owns 32 keys of a tile.  Work is divided evenly by tiles: entry after
-// entry, head after head, row group after row group, each CTA takes the same number of consecutive tiles of all of them, whatever the
-// lengths.  A sequence that lies in several CTAs' shares leaves partial results in scratch, at most two for each CTA, which a second kernel adds.
+// The call is bound by reading the cache.  Every warp works alone: it takes slices of 32 keys of one sequence and head, and keeps the next ones in
+// flight itself (keys and values by TMA, their scales by 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry
+// after entry, head after head, row group after row group, each warp takes the same number of consecutive slices of all of them, whatever
+// the lengths.  A sequence that lies in several warps' shares leaves partial results in scratch, at most two for each warp, which a
+// second kernel adds.  No warp waits for another.
 #include <atomic>
 
 #include "common.cuh"
@@ -24,32 +25,36 @@ namespace teeny {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kTile = 128;                     // keys of a stage
-constexpr int kBox = kTile * kCache8Head;      // 16 KB: their keys, or their values (narrower heads are filled up with zeros by the copies)
-constexpr int kGroups = kTile / 16;            // scales are kept for groups of 16 keys
+constexpr int kSlice = 32;                     // keys that a warp takes at a time
+constexpr int kBox = kSlice * kCache8Head;     // 4 KB: their keys, or their values (narrower heads are filled up with zeros by the copies)
 constexpr int kStage = 2 * kBox;
+constexpr int kWarps = 4;                      // of a CTA
 
-// Variant of the kernel: TP tiles of two terms each (1: bf16, 3: f32), MT x 8 query rows, NG groups of four consumer warps.  Eight bf16 rows fit 168
-// registers, with two CTAs of five warps on an SM; more rows, and f32's, take one CTA with two groups, to which the producer's warpgroup leaves its registers
-// (128 * 40 + 256 * 224 of the 384 * 168 that the CTA has).
-template <int TP, int MT, int NG>
+// Variant of the kernel: TP tiles of two terms each (1: bf16, 3: f32), MT x 8 query rows.  Eight bf16 rows fit 168 registers, which twelve warps
+// of an SM can have; with more rows it is eight warps.
+template <int TP, int MT>
 struct Variant {
-  static constexpr int kRows = 8 * MT, kWarps = 4 * NG, kThreads = NG == 1 ? 160 : 384;
-  static constexpr int kStages = NG == 1 ? 3 : 6;
-  static constexpr int kScales = kStages * kStage;                        // f32 [stages][2][kGroups]
-  static constexpr int kQ = kScales + kStages * 2 * kGroups * 4;          // uint4 [MT][TP][4 steps][32 lanes]
-  static constexpr int kMerge = kQ + MT * TP * 4 * 32 * 16;               // f32 [kWarps / 2][32 values][32 lanes]
-  static constexpr int kML = kMerge + kWarps / 2 * 32 * 32 * 4;           // f32 [kWarps][kRows][2]
-  static constexpr int kNan = kML + kWarps * kRows * 8;                   // int [128]
+  static constexpr int kRows = 8 * MT, kSmall = TP * MT == 1, kCtas = kSmall ? 3 : 2, kStages = 2;
+  // a warp's part of shared memory: stages, scales f32 [stages][4], query terms uint4 [MT][TP][4 steps][32 lanes] (in registers when there is one tile
+  // of them), int [128] first NaN value of each dimension, barriers
+  static constexpr int kScales = kStages * kStage;
+  static constexpr int kQ = kScales + kStages * 16;
+  static constexpr int kNan = kQ + (kSmall ? 0 : MT * TP * 4 * 32 * 16);
   static constexpr int kBars = kNan + 128 * 4;
-  static constexpr int kBytes = kBars + 2 * kStages * 8 + 1024;
-  static_assert(kBytes <= (NG == 1 ? 115600 : 232000), "shared memory");
+  static constexpr int kWarpBytes = (kBars + kStages * 8 + 1023) / 1024 * 1024;
+  static constexpr int kBytes = kWarps * kWarpBytes + 1024;
+  static_assert((kBytes + 1024) * kCtas <= 233472, "shared memory");
 };
 
 __device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_e4m3_16832_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {  // the sum starts here
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
@@ -84,29 +89,31 @@ struct Shared {  // what a call's kernels share
   const SeqDesc* seqs;
   int n_seqs, max_len, G;
   float scale_log2, two_over_cap, cap_l2;
-  float* part_o;   // [2 * CTAs][rows of a unit][128]
-  float* part_ml;  // [2 * CTAs][rows of a unit][2]
+  float* part_o;   // [2 * warps][rows of a unit][128]
+  float* part_ml;  // [2 * warps][rows of a unit][2]
   float* lse2;     // [rows][Hq], base 2, or null
   float* scores;   // [entries][Hq][cap] base 2, or null
-  int parts;       // CTAs of the main kernel
+  int parts;       // warps of the main kernel
   int vec_q, vec_o;
   int* err;
 };
 
-// Tiles of an entry: its units are (head, row group), each over all its tiles.
-struct EntryShape { int tiles, groups; long long all; };
+// Slices of an entry: its units are (head, row group), each over all its slices.
+struct EntryShape { int slices, groups; long long all; };
 __device__ __forceinline__ EntryShape entry_shape(const Shared& s, const SeqDesc& sq, int rows) {
   EntryShape e{0, 0, 0};
   if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return e;
-  e.tiles = (sq.pos + sq.len + kTile - 1) / kTile;
+  e.slices = (sq.pos + sq.len + kSlice - 1) / kSlice;
   e.groups = static_cast<int>((static_cast<long long>(sq.len) * s.G + rows - 1) / rows);
-  e.all = static_cast<long long>(e.tiles) * e.groups * s.c.H;
+  e.all = static_cast<long long>(e.slices) * e.groups * s.c.H;
   return e;
 }
-// CTA p's share of the tiles; with fewer tiles than CTAs the first ones take one each (no share between two others is ever empty).
-__device__ __forceinline__ long long share_begin(long long total, int part, int parts) {
-  return total <= parts ? min(total, static_cast<long long>(part)) : total * part / parts;
+// Where warp w's share begins; no share takes less than kLeast slices, and none between two others is empty.
+constexpr int kLeast = 2;
+__device__ __forceinline__ int shares(const Shared& s, long long total) {
+  return static_cast<int>(min(static_cast<long long>(s.parts), (total + kLeast - 1) / kLeast));
 }
+__device__ __forceinline__ long long share_begin(long long total, int part, int parts) { return total * part / parts; }
 
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
@@ -195,35 +202,72 @@ __device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool
   return exp2f(static_cast<float>(-p)) * scale_log2;
 }
 
-template <typename T, int TP, int MT, int NG>
-__global__ void __launch_bounds__(Variant<TP, MT, NG>::kThreads, NG == 1 ? 2 : 1)
+// One (entry, head, row group) as far as it lies in a warp's share.
+struct Piece {
+  SeqDesc sq;
+  int e, slices, groups, hk, rg, j, end, limit;  // slices j .. end - 1; limit: keys that the group's last row sees
+  bool whole, first;
+};
+__device__ __forceinline__ void piece_range(const Shared& s, Piece& p, int rows, int j0, long long left) {
+  p.j = j0;
+  const int stop = static_cast<int>(min(static_cast<long long>(p.slices), j0 + left));
+  p.whole = j0 == 0 && stop == p.slices;
+  const int last = static_cast<int>(min(static_cast<long long>(p.sq.len) * s.G, (static_cast<long long>(p.rg) + 1) * rows) - 1) / s.G;
+  p.limit = p.sq.pos + last + 1;
+  p.end = stop;
+}
+// to the next unit, of which `left` slices may be taken
+__device__ __forceinline__ void next_piece(const Shared& s, Piece& p, int rows, long long left) {
+  if (++p.rg == p.groups) {
+    p.rg = 0;
+    if (++p.hk == s.c.H) {
+      p.hk = 0;
+      EntryShape es;
+      do {
+        p.sq = s.seqs[++p.e];
+        es = entry_shape(s, p.sq, rows);
+      } while (es.all == 0);
+      p.slices = es.slices;
+      p.groups = es.groups;
+    }
+  }
+  p.first = false;
+  piece_range(s, p, rows, 0, left);
+}
+
+template <typename T, int TP, int MT>
+__global__ void __launch_bounds__(32 * kWarps, Variant<TP, MT>::kCtas)
 cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Shared s) {
-  using V = Variant<TP, MT, NG>;
-  constexpr int R = V::kRows, W = V::kWarps;
+  using V = Variant<TP, MT>;
+  constexpr int R = V::kRows, ST = V::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ long long sm_first[3];  // total tiles, entry of this CTA's first tile, tiles of that entry before it
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  auto full_bar = [&](int st) { return base + V::kBars + 8u * st; };
-  auto empty_bar = [&](int st) { return base + V::kBars + 8u * (V::kStages + st); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t offset = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw) + warp * V::kWarpBytes;
+  const uint32_t base = smem_u32(smem_raw) + offset;
+  uint8_t* gen = smem_raw + offset;
+  if (lane == 0) {
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
-    for (int st = 0; st < V::kStages; ++st) {
-      mbar_init(full_bar(st), 1 + 2 * kGroups);
-      mbar_init(empty_bar(st), 4);
-    }
+    for (int st = 0; st < ST; ++st) mbar_init(base + V::kBars + 8 * st, 1 + 4);
     mbar_fence_init();
   }
+  __syncwarp();
   pdl_wait();
-  if (warp == 0) {
+  // ---- this warp's share ----
+  const int part = blockIdx.x * kWarps + warp;
+  Piece load;
+  long long left;  // slices of the share that are still to be loaded
+  {
     long long total = 0;
     for (int e = lane; e < s.n_seqs; e += 32) total += entry_shape(s, s.seqs[e], R).all;
     total = warp_sum_ll(total);
-    const long long t0 = share_begin(total, blockIdx.x, s.parts);
-    long long before = 0;
-    for (int e0 = 0; e0 < s.n_seqs; e0 += 32) {
+    const int parts = shares(s, total);
+    if (part >= parts) return;
+    const long long t0 = share_begin(total, part, parts);
+    left = share_begin(total, part + 1, parts) - t0;
+    long long before = 0, at = 0;
+    int found = -1;
+    for (int e0 = 0; found < 0; e0 += 32) {
       const long long mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
       long long run = mine;
 #pragma unroll
@@ -232,101 +276,78 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         if (lane >= o) run += up;
       }
       const long long end = before + run;
-      if (mine > 0 && t0 >= end - mine && t0 < end) {
-        sm_first[1] = e0 + lane;
-        sm_first[2] = t0 - (end - mine);
-      }
+      const unsigned who = __ballot_sync(0xffffffffu, mine > 0 && t0 >= end - mine && t0 < end);
       before = __shfl_sync(0xffffffffu, end, 31);
-      if (before > t0) break;
+      if (!who) continue;
+      const int src = __ffs(who) - 1;
+      found = e0 + src;
+      at = t0 - __shfl_sync(0xffffffffu, end - mine, src);
     }
-    if (lane == 0) sm_first[0] = total;
+    load.e = found;
+    load.sq = s.seqs[found];
+    const EntryShape es = entry_shape(s, load.sq, R);
+    load.slices = es.slices;
+    load.groups = es.groups;
+    const long long unit = at / es.slices;
+    load.hk = static_cast<int>(unit / es.groups);
+    load.rg = static_cast<int>(unit - static_cast<long long>(load.hk) * es.groups);
+    load.first = true;
+    piece_range(s, load, R, static_cast<int>(at - unit * es.slices), left);
   }
-  __syncthreads();
-  const long long total = sm_first[0], t0 = share_begin(total, blockIdx.x, s.parts), t1 = share_begin(total, blockIdx.x + 1, s.parts);
-  if (t0 >= t1) return;
-
-  // body(entry, its table row, head, row group, first and last tile, whole unit?, first segment?) for every piece of this CTA's share
-  auto walk = [&](auto&& body) {
-    long long done = t0, at = sm_first[2];
-    for (int e = static_cast<int>(sm_first[1]); done < t1; ++e, at = 0) {
-      const SeqDesc sq = s.seqs[e];
-      const EntryShape es = entry_shape(s, sq, R);
-      while (at < es.all && done < t1) {
-        const int unit = static_cast<int>(at / es.tiles), j0 = static_cast<int>(at - static_cast<long long>(unit) * es.tiles);
-        const int j1 = static_cast<int>(min(static_cast<long long>(es.tiles), j0 + (t1 - done)));
-        const int hk = unit / es.groups, rg = unit - hk * es.groups;
-        // keys that the group's last row sees
-        const int last = min(sq.len - 1, static_cast<int>((static_cast<long long>(rg) * R + R - 1) / s.G)), limit = sq.pos + last + 1;
-        if (!body(e, sq, hk, rg, j0, min(j1, (limit + kTile - 1) / kTile), limit, j0 == 0 && j1 == es.tiles, done == t0)) return;
-        at += j1 - j0;
-        done += j1 - j0;
-      }
+  Piece p = load;
+  long long rest = left;  // slices of the share that are still to be computed
+  int issued = 0, count = 0;
+  auto load_next = [&]() {
+    if (left == 0) return;
+    if (load.j == load.end) next_piece(s, load, R, left);
+    const int st = issued & (ST - 1), key0 = load.j * kSlice;
+    const uint32_t bar = base + V::kBars + 8 * st;
+    if (lane < 4) {  // scales of the slice's two groups of 16 keys; blocks behind the last key may hold anything: zero is written
+      const int key = key0 + 16 * (lane & 1);
+      const uint32_t bytes = key < load.limit ? 4 : 0;
+      const float* src = (lane < 2 ? s.c.ks : s.c.vs) + (static_cast<size_t>(load.sq.slot) * s.c.H + load.hk) * s.c.blocks + (bytes ? key / s.c.B : 0);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n\tcp.async.mbarrier.arrive.noinc.shared::cta.b64 [%3];"
+                   ::"r"(base + V::kScales + st * 16 + lane * 4), "l"(src), "r"(bytes), "r"(bar) : "memory");
     }
+    if (lane == 0) {
+      mbar_expect_tx(bar, kStage);
+      tma_load_4d(base + st * kStage, &tmap_k, bar, 0, key0, load.hk, load.sq.slot);
+      tma_load_4d(base + st * kStage + kBox, &tmap_v, bar, 0, key0, load.hk, load.sq.slot);
+    }
+    ++load.j;
+    ++issued;
+    --left;
   };
+#pragma unroll
+  for (int st = 0; st < ST; ++st) load_next();
 
-  if (warp >= W) {
-    // ---------------- producer ----------------
-    if (NG > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp > W) return;
-    int st = 0;
-    uint32_t ph = 0;
-    walk([&](int, const SeqDesc& sq, int hk, int, int j0, int j1, int limit, bool, bool) {
-      const size_t srow = (static_cast<size_t>(sq.slot) * s.c.H + hk) * s.c.blocks;
-      for (int j = j0; j < j1; ++j) {
-        if (!mbar_wait(empty_bar(st), ph ^ 1, s.err, DEVERR_ATTN_PRODUCER)) return false;
-        const int key0 = j * kTile;
-        if (lane < 2 * kGroups) {
-          const int key = key0 + 16 * (lane & (kGroups - 1));
-          const float* src = (lane < kGroups ? s.c.ks : s.c.vs) + srow + (key < limit ? key / s.c.B : 0);
-          const uint32_t bytes = key < limit ? 4 : 0;  // (0: zero is written; blocks behind the last key may hold anything)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n\tcp.async.mbarrier.arrive.noinc.shared::cta.b64 [%3];"
-                       ::"r"(base + V::kScales + (st * 2 * kGroups + lane) * 4), "l"(src), "r"(bytes), "r"(full_bar(st)) : "memory");
-        }
-        if (lane == 0) {
-          mbar_expect_tx(full_bar(st), kStage);
-          tma_load_4d(base + st * kStage, &tmap_k, full_bar(st), 0, key0, hk, sq.slot);
-          tma_load_4d(base + st * kStage + kBox, &tmap_v, full_bar(st), 0, key0, hk, sq.slot);
-        }
-        if (++st == V::kStages) { st = 0; ph ^= 1; }
-      }
-      return true;
-    });
-    return;
-  }
-
-  // ---------------- consumers ----------------
-  if (NG > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-  const int g = lane >> 2, c = lane & 3, quarter = warp & 3, ng = warp >> 2;
-  float* sm_ml = reinterpret_cast<float*>(gen + V::kML);
   int* sm_nan = reinterpret_cast<int*>(gen + V::kNan);
-  int count = 0;  // tiles of this CTA so far
-  walk([&](int e, const SeqDesc& sq, int hk, int rg, int j0, int j1, int limit, bool whole, bool first) {
-    // ---- query terms: row tile mt by warp mt (mod W), into shared memory as A fragments ----
+  for (;;) {
+    // ---- query terms as A fragments ----
     float factor[MT];
     int rows_limit[MT];  // keys that this lane's rows see
+    uint4 q_terms[V::kSmall ? 4 : 1];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const long long r = static_cast<long long>(rg) * R + mt * 8 + g;
-      const int i = static_cast<int>(r / s.G), h = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-      const bool valid = i < sq.len;
-      rows_limit[mt] = valid ? sq.pos + i + 1 : limit;
-      if (mt % W == warp) {
-        uint32_t term[2 * TP][8];
-        const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(h) * s.c.D;
-        const float f = split_row<T, 2 * TP>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
+      const long long r = static_cast<long long>(p.rg) * R + mt * 8 + g;
+      const int i = static_cast<int>(r / s.G), h = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+      const bool valid = i < p.sq.len;
+      rows_limit[mt] = valid ? p.sq.pos + i + 1 : p.limit;
+      uint32_t term[2 * TP][8];
+      const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(h) * s.c.D;
+      factor[mt] = split_row<T, 2 * TP>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
 #pragma unroll
-        for (int tp = 0; tp < TP; ++tp)
+      for (int tp = 0; tp < TP; ++tp)
 #pragma unroll
-          for (int step = 0; step < 4; ++step)
-            reinterpret_cast<uint4*>(gen + V::kQ)[((mt * TP + tp) * 4 + step) * 32 + lane] =
-                make_uint4(term[2 * tp][2 * step], term[2 * tp + 1][2 * step], term[2 * tp][2 * step + 1], term[2 * tp + 1][2 * step + 1]);
-        if (c == 0) sm_ml[mt * 8 + g] = f;
-      }
+        for (int step = 0; step < 4; ++step) {
+          const uint4 a = make_uint4(term[2 * tp][2 * step], term[2 * tp + 1][2 * step], term[2 * tp][2 * step + 1], term[2 * tp + 1][2 * step + 1]);
+          if (V::kSmall) q_terms[step & (V::kSmall ? 3 : 0)] = a;
+          else reinterpret_cast<uint4*>(gen + V::kQ)[((mt * TP + tp) * 4 + step) * 32 + lane] = a;
+        }
     }
-    for (int d = threadIdx.x; d < 128; d += 32 * W) sm_nan[d] = 0x7fffffff;
-    named_barrier_sync(1, 32 * W);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) factor[mt] = sm_ml[mt * 8 + g];
+    if (p.sq.len > 1)
+      for (int d = lane; d < 128; d += 32) sm_nan[d] = 0x7fffffff;
+    __syncwarp();
 
     float m[MT], l[MT];
     f32x2 acc[MT][16];  // dimensions 32 c + n and 32 c + 16 + n
@@ -337,25 +358,26 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
       for (int n = 0; n < 16; ++n) acc[mt][n] = 0ull;
     }
-    bool ok = true;
-    for (int j = j0; j < j1; ++j, ++count) {
-      if (NG > 1 && count % NG != ng) continue;
-      const int st = count % V::kStages;
-      if (!mbar_wait(full_bar(st), count / V::kStages & 1, s.err, DEVERR_ATTN_SOFTMAX)) { ok = false; break; }
-      const int kb = j * kTile + 32 * quarter;
-      if (kb < limit) {
-        const uint32_t kt = base + st * kStage + (32 * quarter + g) * 128, vt = base + st * kStage + kBox + 32 * quarter * 128;
-        const uint32_t sc = base + V::kScales + st * 2 * kGroups * 4 + 2 * quarter * 4;
-        const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + kGroups * 4), vs1 = lds32(sc + kGroups * 4 + 4);
-        const bool masked = kb + 32 > sq.pos + 1;
-        // ---- scores: key 8 t + g of the warp's 32 is column g of block t; lane c reads the dimensions whose terms it holds of the query ----
+    rest -= p.end - p.j;
+    for (; p.j < p.end; ++p.j, ++count) {
+      const int st = count & (ST - 1), kb = p.j * kSlice;
+      if (!mbar_wait(base + V::kBars + 8 * st, count / ST & 1, s.err, DEVERR_ATTN_SOFTMAX)) {
+        // (nothing that this warp asked for may arrive after it has gone: the barriers are waited for once more, within their limit)
+        for (int i = count; i < issued; ++i) mbar_wait(base + V::kBars + 8 * (i & (ST - 1)), i / ST & 1, s.err, DEVERR_ATTN_SOFTMAX);
+        return;
+      }
+      if (kb < p.limit) {
+        const uint32_t kt = base + st * kStage + g * 128, vt = base + st * kStage + kBox, sc = base + V::kScales + st * 16;
+        const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + 8), vs1 = lds32(sc + 12);
+        const bool masked = kb + kSlice > p.sq.pos + 1;
+        // ---- scores: key 8 t + g of the slice is column g of block t; lane c reads the dimensions whose terms it holds of the query ----
         uint4 kw[4][2];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) kw[t][h] = lds128(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
         uint4 pf[MT][TP];
-        float alpha[MT], beta[MT];
+        float beta[MT];
         const float vmax = fmaxf(vs0, vs1);
         float r0 = 256.0f, r1 = 256.0f;
         if (vs0 != vs1) {
@@ -367,52 +389,66 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         for (int mt = 0; mt < MT; ++mt) {
           float x[4][2];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) x[t][0] = x[t][1] = 0.0f;
-#pragma unroll
           for (int tp = TP - 1; tp >= 0; --tp) {
             uint4 qa[4];
 #pragma unroll
-            for (int step = 0; step < 4; ++step) qa[step] = lds128(base + V::kQ + (((mt * TP + tp) * 4 + step) * 32 + lane) * 16);
+            for (int step = 0; step < 4; ++step)
+              qa[step] = V::kSmall ? q_terms[step & (V::kSmall ? 3 : 0)] : lds128(base + V::kQ + (((mt * TP + tp) * 4 + step) * 32 + lane) * 16);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-              float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma_e4m3_16832(d, qa[0], kw[t][0].x, kw[t][0].y);
+              float d[4];
+              mma_e4m3_16832_first(d, qa[0], kw[t][0].x, kw[t][0].y);
               mma_e4m3_16832(d, qa[1], kw[t][0].z, kw[t][0].w);
               mma_e4m3_16832(d, qa[2], kw[t][1].x, kw[t][1].y);
               mma_e4m3_16832(d, qa[3], kw[t][1].z, kw[t][1].w);
-              x[t][0] = fmaf(x[t][0], 1.0f / 256.0f, fmaf(d[2], 0.0625f, d[0]));
-              x[t][1] = fmaf(x[t][1], 1.0f / 256.0f, fmaf(d[3], 0.0625f, d[1]));
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const float both = fmaf(d[2 + z], 0.0625f, d[z]);
+                x[t][z] = tp == TP - 1 ? both : fmaf(x[t][z], 1.0f / 256.0f, both);
+              }
             }
           }
           const float f0 = factor[mt] * ks0, f1 = factor[mt] * ks1;
-          float top = -INFINITY;
 #pragma unroll
           for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              float y = x[t][z] * (t < 2 ? f0 : f1);
-              if (s.cap_l2 > 0.0f) y = softcap_log2(y, s.two_over_cap, s.cap_l2);
-              if (masked && kb + 8 * t + 2 * c + z >= rows_limit[mt]) y = -INFINITY;
-              x[t][z] = y;
-              top = fmaxf(top, y);
-            }
+            for (int z = 0; z < 2; ++z) x[t][z] *= t < 2 ? f0 : f1;
+          if (s.cap_l2 > 0.0f) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) x[t][z] = softcap_log2(x[t][z], s.two_over_cap, s.cap_l2);
+          }
+          if (masked) {
+            const int see = rows_limit[mt] - kb - 2 * c;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) x[t][z] = 8 * t + z < see ? x[t][z] : -INFINITY;
+          }
+          float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
           if (s.scores) {
-            const int r = rg * R + mt * 8 + g;  // (single tokens: a row is a query head of the group)
+            const int r = p.rg * R + mt * 8 + g;  // (single tokens: a row is a query head of the group)
             if (r < s.G) {
-              float* to = s.scores + (static_cast<size_t>(e) * s.a.Hq + hk * s.G + r) * s.c.cap + kb + 2 * c;
+              float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.c.cap + kb + 2 * c;
 #pragma unroll
               for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int z = 0; z < 2; ++z)
-                  if (!masked || kb + 8 * t + 2 * c + z < limit) to[8 * t + z] = x[t][z];
+                  if (!masked || kb + 8 * t + 2 * c + z < p.limit) to[8 * t + z] = x[t][z];
             }
           }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float from = top == -INFINITY ? 0.0f : top, m_new = fmaxf(m[mt], top), to = m_new == -INFINITY ? 0.0f : m_new;
-          alpha[mt] = ex2(m[mt] - to);
-          beta[mt] = ex2(top - to);
-          m[mt] = m_new;
+          const float from = top == -INFINITY ? 0.0f : top;
+          if (__any_sync(0xffffffffu, top > m[mt])) {  // (rare once a sequence is under way)
+            const float m_new = fmaxf(m[mt], top), alpha = ex2(m[mt] - (m_new == -INFINITY ? 0.0f : m_new));
+            m[mt] = m_new;
+            l[mt] *= alpha;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) acc[mt][n] = mul2(acc[mt][n], pack2(alpha, alpha));
+          }
+          beta[mt] = ex2(top - (m[mt] == -INFINITY ? 0.0f : m[mt]));
           float sum = 0.0f;
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -422,7 +458,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
               sum += x[t][z];
               x[t][z] *= t < 2 ? r0 : r1;
             }
-          l[mt] = fmaf(l[mt], alpha[mt], sum * beta[mt]);
+          l[mt] = fmaf(sum, beta[mt], l[mt]);
           beta[mt] *= vmax * (1.0f / 256.0f);
           // A fragments of the values' product: keys 2c, 2c + 1 of blocks 0, 1 (then 2, 3)
 #pragma unroll
@@ -450,18 +486,20 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = kb + 2 * c + (i & 1) + 8 * (i >> 1);
-            if (key >= limit) vw[i] = make_uint4(0u, 0u, 0u, 0u);  // stale rows may hold NaN, and 0 * NaN is NaN
-            if (sq.len > 1) {
+            if (key >= p.limit) vw[i] = make_uint4(0u, 0u, 0u, 0u);  // stale rows may hold NaN, and 0 * NaN is NaN
+            if (p.sq.len > 1) {
               // a NaN value counts only for the rows that see its key: noted, and put back when the rows are finished
-              uint32_t* word = &vw[i].x;
+              uint32_t word[4] = {vw[i].x, vw[i].y, vw[i].z, vw[i].w};
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 if ((((word[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u)
+#pragma unroll
                   for (int b = 0; b < 4; ++b)
                     if ((word[k] >> (8 * b) & 0x7fu) == 0x7fu) {
                       word[k] &= ~(0xffu << (8 * b));
                       atomicMin(&sm_nan[16 * g + 4 * k + b], key);
                     }
+              vw[i] = make_uint4(word[0], word[1], word[2], word[3]);
             }
           }
         }
@@ -470,9 +508,14 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           uint32_t b[2][4];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t a0 = (&vw[4 * half].x)[k], a1 = (&vw[4 * half + 1].x)[k], a2 = (&vw[4 * half + 2].x)[k], a3 = (&vw[4 * half + 3].x)[k];
-            const uint32_t l01 = __byte_perm(a0, a1, 0x5140), h01 = __byte_perm(a0, a1, 0x7362);
-            const uint32_t l23 = __byte_perm(a2, a3, 0x5140), h23 = __byte_perm(a2, a3, 0x7362);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4& v = vw[4 * half + i];
+              w[i] = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
+            }
+            const uint32_t l01 = __byte_perm(w[0], w[1], 0x5140), h01 = __byte_perm(w[0], w[1], 0x7362);
+            const uint32_t l23 = __byte_perm(w[2], w[3], 0x5140), h23 = __byte_perm(w[2], w[3], 0x7362);
             b[half][0] = __byte_perm(l01, l23, 0x5410);
             b[half][1] = __byte_perm(l01, l23, 0x7632);
             b[half][2] = __byte_perm(h01, h23, 0x5410);
@@ -480,66 +523,34 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           }
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            const f32x2 al = pack2(alpha[mt], alpha[mt]), be = pack2(beta[mt], beta[mt]), sixteenth = pack2(0.0625f, 0.0625f);
+            const f32x2 be = pack2(beta[mt], beta[mt]), sixteenth = pack2(0.0625f, 0.0625f);
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
               f32x2 o = 0ull;
 #pragma unroll
               for (int tp = TP - 1; tp >= 0; --tp) {
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma_e4m3_16832(d, pf[mt][tp], b[0][n], b[1][n]);
+                float d[4];
+                mma_e4m3_16832_first(d, pf[mt][tp], b[0][n], b[1][n]);
                 const f32x2 both = fma2(pack2(d[2], d[3]), sixteenth, pack2(d[0], d[1]));
                 o = tp == TP - 1 ? both : fma2(o, pack2(1.0f / 256.0f, 1.0f / 256.0f), both);
               }
-              acc[mt][4 * k + n] = fma2(acc[mt][4 * k + n], al, mul2(o, be));
+              acc[mt][4 * k + n] = fma2(o, be, acc[mt][4 * k + n]);
             }
           }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(empty_bar(st));
+      load_next();
     }
-    if (!ok) return false;
 
-    // ---- the warps' parts together ----
+    // ---- the rows' results, or this warp's part of them ----
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 1);
       l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 2);
-    }
-    named_barrier_sync(1, 32 * W);  // (sm_ml held the rows' factors)
-    if (c == 0)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        sm_ml[(warp * R + mt * 8 + g) * 2] = m[mt];
-        sm_ml[(warp * R + mt * 8 + g) * 2 + 1] = l[mt];
-      }
-    named_barrier_sync(1, 32 * W);
-    f32x2* merge = reinterpret_cast<f32x2*>(gen + V::kMerge);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int r8 = mt * 8 + g;
-      float mm = -INFINITY, ll = 0.0f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm_ml[(w * R + r8) * 2]);
-      const float to = mm == -INFINITY ? 0.0f : mm;
-#pragma unroll
-      for (int w = 0; w < W; ++w) ll = fmaf(sm_ml[(w * R + r8) * 2 + 1], ex2(sm_ml[(w * R + r8) * 2] - to), ll);
-      const float f = ex2(m[mt] - to);
-#pragma unroll
-      for (int n = 0; n < 16; ++n) acc[mt][n] = mul2(acc[mt][n], pack2(f, f));
-#pragma unroll
-      for (int half = W / 2; half > 0; half >>= 1) {
-        if (warp >= half && warp < 2 * half)
-#pragma unroll
-          for (int n = 0; n < 16; ++n) merge[((warp - half) * 16 + n) * 32 + lane] = acc[mt][n];
-        named_barrier_sync(1, 32 * W);
-        if (warp < half)
-#pragma unroll
-          for (int n = 0; n < 16; ++n) acc[mt][n] = fma2(merge[(warp * 16 + n) * 32 + lane], pack2(1.0f, 1.0f), acc[mt][n]);
-        if (half > 1 || MT > 1) named_barrier_sync(1, 32 * W);
-      }
-      if (warp != 0) continue;
+      const long long r = static_cast<long long>(p.rg) * R + mt * 8 + g;
+      const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+      if (i >= p.sq.len) continue;
       float o[2][16];
 #pragma unroll
       for (int n = 0; n < 16; ++n) {
@@ -547,30 +558,24 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         o[0][n] = v.x;
         o[1][n] = v.y;
       }
-      if (sq.len > 1) {
+      if (p.sq.len > 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int n = 0; n < 16; ++n)
             if (rows_limit[mt] > sm_nan[32 * c + 16 * h + n]) o[h][n] = __uint_as_float(0x7fffffffu);
       }
-      if (!whole) {
-        const size_t slot = (2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1)) * R + r8;
-        if (c == 0) {
-          s.part_ml[slot * 2] = mm;
-          s.part_ml[slot * 2 + 1] = ll;
-        }
+      if (!p.whole) {
+        const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + mt * 8 + g;
+        if (c == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(m[mt], l[mt]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) store16(s.part_o + slot * 128 + 32 * c + 16 * h, o[h], true);
         continue;
       }
-      const long long r = static_cast<long long>(rg) * R + r8;
-      const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-      if (i >= sq.len) continue;
-      const size_t row = static_cast<size_t>(sq.row0) + i;
-      if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
-      if (c == 0) note_lse(s, row, hq, mm + log2f(ll));
-      const float inv = 1.0f / ll;
+      const size_t row = static_cast<size_t>(p.sq.row0) + i;
+      if (s.a.sink) l[mt] += ex2(fmaf(s.a.sink[hq], kLog2e, -m[mt]));
+      if (c == 0) note_lse(s, row, hq, m[mt] + log2f(l[mt]));
+      const float inv = 1.0f / l[mt];
       T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -581,12 +586,13 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         store16(out + d0, o[h], s.vec_o);
       }
     }
-    named_barrier_sync(1, 32 * W);  // the next unit writes what was read here
-    return true;
-  });
+    if (rest == 0) return;
+    next_piece(s, p, R, rest);
+    __syncwarp();
+  }
 }
 
-// Adds the parts of the units that lie in several CTAs' shares: one CTA for a unit, a warp for a row (mod 8), a lane for four dimensions.
+// Adds the parts of the units that lie in several warps' shares: one CTA for a unit, a warp for a row (mod 8), a lane for four dimensions.
 template <typename T>
 __global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_constant__ Shared s, int rows, int max_groups) {
   __shared__ long long sums[8][2];
@@ -609,11 +615,12 @@ __global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_consta
   before = total = 0;
 #pragma unroll
   for (int w = 0; w < 8; ++w) { before += sums[w][0]; total += sums[w][1]; }
-  const long long u0 = before + (static_cast<long long>(hk) * es.groups + rg) * es.tiles, u1 = u0 + es.tiles;
-  auto owner = [&](long long tile) { return static_cast<int>(total <= s.parts ? tile : ((tile + 1) * s.parts - 1) / total); };
-  const int c0 = owner(u0), c1 = owner(u1 - 1);
+  const int parts = shares(s, total);
+  const long long u0 = before + (static_cast<long long>(hk) * es.groups + rg) * es.slices, u1 = u0 + es.slices;
+  // the warp whose share holds a slice: the last one that begins at or before it
+  const int c0 = static_cast<int>(((u0 + 1) * parts - 1) / total), c1 = static_cast<int>((u1 * parts - 1) / total);
   if (c0 == c1) return;
-  const int slot0 = 2 * c0 + (share_begin(total, c0, s.parts) == u0 ? 0 : 1);
+  const int slot0 = 2 * c0 + (share_begin(total, c0, parts) == u0 ? 0 : 1);
   for (int r8 = warp; r8 < rows; r8 += 8) {
     const long long r = static_cast<long long>(rg) * rows + r8;
     const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
@@ -737,7 +744,7 @@ struct Plan {
 };
 int row_tiles(int f32, int G, int max_len) {
   // as few passes over the keys as rows allow, and no more row tiles than those need
-  const int most = f32 ? 2 : 4;
+  const int most = f32 ? 1 : 4;
   const long long rows = static_cast<long long>(G) * max_len, passes = (rows + 8 * most - 1) / (8 * most);
   return static_cast<int>((rows + 8 * passes - 1) / (8 * passes));
 }
@@ -746,7 +753,7 @@ Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len
   const int G = Hq / c.H;
   p.mt = row_tiles(f32, G, max_len);
   p.groups = static_cast<int>((static_cast<long long>(G) * max_len + 8 * p.mt - 1) / (8 * p.mt));
-  p.parts = sm_count() * (!f32 && p.mt == 1 ? 2 : 1);  // (the CTAs that are resident at once)
+  p.parts = sm_count() * (!f32 && p.mt == 1 ? 3 : 2) * kWarps;  // (the warps that are resident at once)
   auto take = [&](size_t n) { const size_t at = p.bytes; p.bytes += (n + 255) / 256 * 256; return at; };
   p.part_o = take(static_cast<size_t>(2) * p.parts * 8 * p.mt * 128 * 4);
   p.part_ml = take(static_cast<size_t>(2) * p.parts * 8 * p.mt * 2 * 4);
@@ -758,13 +765,12 @@ Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len
 template <typename F>
 void for_variant(int f32, int mt, F&& f) {
   if (f32) {
-    if (mt == 1) f(cache8_attention_kernel<float, 3, 1, 2>, Variant<3, 1, 2>{});
-    else f(cache8_attention_kernel<float, 3, 2, 2>, Variant<3, 2, 2>{});
+    f(cache8_attention_kernel<float, 3, 1>, Variant<3, 1>{});
   } else {
-    if (mt == 1) f(cache8_attention_kernel<bf16, 1, 1, 1>, Variant<1, 1, 1>{});
-    else if (mt == 2) f(cache8_attention_kernel<bf16, 1, 2, 2>, Variant<1, 2, 2>{});
-    else if (mt == 3) f(cache8_attention_kernel<bf16, 1, 3, 2>, Variant<1, 3, 2>{});
-    else f(cache8_attention_kernel<bf16, 1, 4, 2>, Variant<1, 4, 2>{});
+    if (mt == 1) f(cache8_attention_kernel<bf16, 1, 1>, Variant<1, 1>{});
+    else if (mt == 2) f(cache8_attention_kernel<bf16, 1, 2>, Variant<1, 2>{});
+    else if (mt == 3) f(cache8_attention_kernel<bf16, 1, 3>, Variant<1, 3>{});
+    else f(cache8_attention_kernel<bf16, 1, 4>, Variant<1, 4>{});
   }
 }
 int prepare() {
@@ -774,7 +780,7 @@ int prepare() {
   if (dev < 64 && (done.load(std::memory_order_acquire) >> dev) & 1ull) return 0;
   cudaError_t e = cudaSuccess;
   for (int f32 = 0; f32 < 2; ++f32)
-    for (int mt = 1; mt <= (f32 ? 2 : 4); ++mt)
+    for (int mt = 1; mt <= (f32 ? 1 : 4); ++mt)
       for_variant(f32, mt, [&](auto kernel, auto v) {
         const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(v)::kBytes);
         if (e == cudaSuccess) e = rc;
@@ -786,7 +792,7 @@ int prepare() {
 int encode_codes(CUtensorMap* map, const uint8_t* base, int d, const Cache8& c) {
   const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(c.cap), static_cast<uint64_t>(c.H), static_cast<uint64_t>(c.slots)};
   const uint64_t strides[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(d) * c.cap, static_cast<uint64_t>(d) * c.cap * c.H};
-  const uint32_t box[4] = {kCache8Head, kTile, 1, 1};
+  const uint32_t box[4] = {kCache8Head, kSlice, 1, 1};
   return encode_tensor_map_u8(map, base, 4, dims, strides, box);
 }
 struct PdlScope {  // kernels of a call behind its first one start their set-up while it ends
@@ -832,7 +838,7 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   if (!s.err) return TEENY_ERR_DRIVER;
   for_variant(a.f32, p.mt, [&](auto kernel, auto v) {
     using V = decltype(v);
-    launch_kernel(kernel, dim3(p.parts), dim3(V::kThreads), V::kBytes, st, 1, mk, mv, s);
+    launch_kernel(kernel, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
   });
   const PdlScope behind;
   const dim3 units(static_cast<unsigned>(n_seqs) * c.H * p.groups);
