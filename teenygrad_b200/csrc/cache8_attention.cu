@@ -1,13 +1,13 @@
 // Causal attention over the 8-bit key/value cache (layout in teeny_cache8.h) for any number of query rows, and the weights that the cached tokens
 // receive.
 //
-// Both products run on E4M3 operands as they lie in the cache (mma.sync m16n8k32, f32 sums), which needs no conversion of keys and values: of
-// a 16-row tile, rows 0-7 hold the first E4M3 term of eight query rows and rows 8-15 the second, x = t0 + t1 / 16, which is a bf16
-// number exactly (each term has four of its eight bits; a row is scaled so that its largest number is in [128, 256), below 2^-20 of that a
-// rest is cut).  f32 rows take three such tiles, six terms.  The two halves of a sum lie in the same thread's registers.  Probabilities are split
-// the same way, relative to the largest one of the 32 keys that a warp takes at a time, so that no product depends on how far a
-// key is below the row's maximum.  Scales of key blocks multiply the scores; those of value blocks, relative to the larger one of the 32
-// keys, the probabilities.
+// Both products run on f16 operands with f32 sums (mma.sync m16n8k16): an E4M3 number is an f16 number exactly, and one conversion makes two of
+// them.  (mma.sync on E4M3 operands is made of the same f16 products here, with additions of its own behind each: 0.19 m16n8k32 a clock
+// and SM, where the f16 pairs run at 0.42 / 2.)  A query row is scaled by a power of two so that its largest number is in [2^14, 2^15): a bf16
+// number below 2^-28 of that loses bits, no other.  f32 rows are two f16 terms, 22 bits, in rows 0-7 and 8-15 of a tile: the halves
+// of a sum lie in the same thread's registers.  Probabilities are f16 numbers times 2^14 (f32: two terms as well), so that a key is lost
+// only 2^-38 below the row's maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to
+// the largest so far, the probabilities.
 //
 // The call is bound by reading the cache.  Every warp works alone: it takes slices of 32 keys of one sequence and head, and keeps the next ones in
 // flight itself (keys and values by TMA, their scales by 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry
@@ -15,6 +15,8 @@
 // the lengths.  A sequence that lies in several warps' shares leaves partial results in scratch, at most two for each warp, which a
 // second kernel adds.  No warp waits for another.
 #include <atomic>
+#include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -30,31 +32,44 @@ constexpr int kBox = kSlice * kCache8Head;     // 4 KB: their keys, or their val
 constexpr int kStage = 2 * kBox;
 constexpr int kWarps = 4;                      // of a CTA
 
-// Variant of the kernel: TP tiles of two terms each (1: bf16, 3: f32), MT x 8 query rows.  Eight bf16 rows fit 168 registers, which twelve warps
-// of an SM can have; with more rows it is eight warps.
-template <int TP, int MT>
+// Variant of the kernel: tiles of the query's rows, which are eight bf16 rows (kEight), 16 (kSixteen), 2 x 16 (kPair), or eight f32 rows in two terms
+// (kF32).  Eight bf16 rows fit 168 registers, with which an SM has twelve warps; the others take eight.
+enum : int { kEight = 0, kSixteen, kPair, kF32 };
+template <int KIND>
 struct Variant {
-  static constexpr int kRows = 8 * MT, kSmall = TP * MT == 1, kCtas = kSmall ? 3 : 2, kStages = 2;
-  // a warp's part of shared memory: stages, scales f32 [stages][4], query terms uint4 [MT][TP][4 steps][32 lanes] (in registers when there is one tile
-  // of them), int [128] first NaN value of each dimension, barriers
+  static constexpr int kTiles = KIND == kPair ? 2 : 1, kRows = KIND == kEight || KIND == kF32 ? 8 : 16 * kTiles;
+  static constexpr int kHalves = KIND == kEight ? 1 : 2;  // halves of a tile whose sums are used
+  static constexpr int kCtas = KIND == kEight ? 3 : 2, kStages = 2;
+  static constexpr bool kTerms = KIND == kF32, kQRegs = KIND != kPair;
+  using T = typename std::conditional<KIND == kF32, float, bf16>::type;
+  // a warp's part of shared memory: stages, scales f32 [stages][4], queries uint4 [tiles][8 steps][32 lanes] (in registers but for kPair), int [128] first NaN
+  // value of each dimension, barriers
   static constexpr int kScales = kStages * kStage;
   static constexpr int kQ = kScales + kStages * 16;
-  static constexpr int kNan = kQ + (kSmall ? 0 : MT * TP * 4 * 32 * 16);
+  static constexpr int kNan = kQ + (kQRegs ? 0 : kTiles * 8 * 32 * 16);
   static constexpr int kBars = kNan + 128 * 4;
   static constexpr int kWarpBytes = (kBars + kStages * 8 + 1023) / 1024 * 1024;
   static constexpr int kBytes = kWarps * kWarpBytes + 1024;
   static_assert((kBytes + 1024) * kCtas <= 233472, "shared memory");
 };
 
-__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_e4m3_16832_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {  // the sum starts here
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+// Four E4M3 numbers as two f16 pairs
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// what the f16 numbers `two` leave of x and y, times 2^11
+__device__ __forceinline__ uint32_t rest_f16x2(uint32_t two, float x, float y) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+  return pack_f16x2((x - f.x) * 2048.0f, (y - f.y) * 2048.0f);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
@@ -65,18 +80,6 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
-}
-__device__ __forceinline__ float2 halves(unsigned short two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-// The first E4M3 term of two numbers; x, y become what is left of them, times 16.
-__device__ __forceinline__ unsigned short take_term(float& x, float& y) {
-  const unsigned short t = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-  const float2 f = halves(t);
-  x = (x - f.x) * 16.0f;
-  y = (y - f.y) * 16.0f;
-  return t;
 }
 __device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -154,10 +157,10 @@ __device__ __forceinline__ void store16(float* p, const float (&x)[16], bool vec
   }
 }
 
-// Terms of one query row, of which this lane (c = lane % 4) has the dimensions 32 c .. 32 c + 31, as the words of a lane's A fragments: word w of the
-// steps' eight is dimensions 32 c + 4 w ..; term[t][w].  Returns the factor that takes a sum of terms back (base-2 scores).
+// A query row, of which this lane (c = lane % 4) has the dimensions 32 c .. 32 c + 31, scaled, as f16 pairs: word w is dimensions 32 c + 2 w, + 1.
+// term[1]: the rest.  Returns the factor that takes scores back (base 2).
 template <typename T, int TERMS>
-__device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool vec, int c, float scale_log2, uint32_t (&term)[TERMS][8]) {
+__device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool vec, int c, float scale_log2, uint32_t (&term)[TERMS][16]) {
   float x[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) x[i] = 0.0f;
@@ -174,6 +177,12 @@ __device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool
 #pragma unroll
           for (int e = 0; e < 4; ++e) { x[16 * h + 8 * i + 2 * e] = bf16_lo(r[e]); x[16 * h + 8 * i + 2 * e + 1] = bf16_hi(r[e]); }
         }
+      } else if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + d0 + 4 * i);
+          x[16 * h + 4 * i] = w.x; x[16 * h + 4 * i + 1] = w.y; x[16 * h + 4 * i + 2] = w.z; x[16 * h + 4 * i + 3] = w.w;
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[16 * h + i] = load_one(q + d0 + i);
@@ -185,21 +194,16 @@ __device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool
   for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  const int p = split_scale_exponent(amax);
-  const float up = exp2f(static_cast<float>(p));
+  int p = 0;
+  if (amax > 0.0f && amax < INFINITY) p = min(100, max(-100, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23)));
+  const float up = __uint_as_float(static_cast<unsigned>(127 + p) << 23), down = __uint_as_float(static_cast<unsigned>(127 - p) << 23);
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    // (an infinity would saturate: it has to stay what it is, not a number of E4M3's range)
-    float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = fabsf(x[4 * w + e]) < INFINITY ? x[4 * w + e] * up : __uint_as_float(0x7fffffffu);
-#pragma unroll
-    for (int t = 0; t < TERMS; ++t) {
-      const uint32_t lo = take_term(y[0], y[1]), hi = take_term(y[2], y[3]);
-      term[t][w] = lo | hi << 16;
-    }
+  for (int w = 0; w < 16; ++w) {
+    const float a = x[2 * w] * up, b = x[2 * w + 1] * up;
+    term[0][w] = pack_f16x2(a, b);
+    if (TERMS > 1) term[TERMS - 1][w] = rest_f16x2(term[0][w], a, b);
   }
-  return exp2f(static_cast<float>(-p)) * scale_log2;
+  return down * scale_log2;
 }
 
 // One (entry, head, row group) as far as it lies in a warp's share.
@@ -235,11 +239,14 @@ __device__ __forceinline__ void next_piece(const Shared& s, Piece& p, int rows, 
   piece_range(s, p, rows, 0, left);
 }
 
-template <typename T, int TP, int MT>
-__global__ void __launch_bounds__(32 * kWarps, Variant<TP, MT>::kCtas)
+template <int KIND>
+__global__ void __launch_bounds__(32 * kWarps, Variant<KIND>::kCtas)
 cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Shared s) {
-  using V = Variant<TP, MT>;
-  constexpr int R = V::kRows, ST = V::kStages;
+  using V = Variant<KIND>;
+  using T = typename V::T;
+  constexpr int R = V::kRows, ST = V::kStages, MT = V::kTiles, HV = V::kHalves;
+  // a lane's rows: those of its accumulators' halves (f32: the second half is the first one's second term)
+  constexpr int RH = V::kTerms ? 1 : HV, ROWS = MT * RH;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const uint32_t offset = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw) + warp * V::kWarpBytes;
@@ -323,41 +330,51 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
   int* sm_nan = reinterpret_cast<int*>(gen + V::kNan);
   for (;;) {
-    // ---- query terms as A fragments ----
-    float factor[MT];
-    int rows_limit[MT];  // keys that this lane's rows see
-    uint4 q_terms[V::kSmall ? 4 : 1];
+    // ---- queries as A fragments; row tile mt's row g + 8 h is this lane's row n = RH mt + h ----
+    float factor[ROWS];
+    int rows_limit[ROWS];  // keys that the rows see
+    uint4 q_regs[V::kQRegs ? 8 : 1];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const long long r = static_cast<long long>(p.rg) * R + mt * 8 + g;
-      const int i = static_cast<int>(r / s.G), h = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-      const bool valid = i < p.sq.len;
-      rows_limit[mt] = valid ? p.sq.pos + i + 1 : p.limit;
-      uint32_t term[2 * TP][8];
-      const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(h) * s.c.D;
-      factor[mt] = split_row<T, 2 * TP>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
+      uint32_t term[2][16];
 #pragma unroll
-      for (int tp = 0; tp < TP; ++tp)
+      for (int h = 0; h < RH; ++h) {
+        const int n = RH * mt + h;
+        const long long r = static_cast<long long>(p.rg) * R + mt * 16 + 8 * h + g;
+        const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+        const bool valid = i < p.sq.len;
+        rows_limit[n] = valid ? p.sq.pos + i + 1 : p.limit;
+        const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
+        if constexpr (V::kTerms) factor[n] = split_row<T, 2>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
+        else {
+          uint32_t one[1][16];
+          factor[n] = split_row<T, 1>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, one);
 #pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const uint4 a = make_uint4(term[2 * tp][2 * step], term[2 * tp + 1][2 * step], term[2 * tp][2 * step + 1], term[2 * tp + 1][2 * step + 1]);
-          if (V::kSmall) q_terms[step & (V::kSmall ? 3 : 0)] = a;
-          else reinterpret_cast<uint4*>(gen + V::kQ)[((mt * TP + tp) * 4 + step) * 32 + lane] = a;
+          for (int w = 0; w < 16; ++w) term[h][w] = one[0][w];
         }
+      }
+#pragma unroll
+      for (int step = 0; step < 8; ++step) {
+        const uint4 a = make_uint4(term[0][2 * step], HV > 1 ? term[1][2 * step] : 0u, term[0][2 * step + 1], HV > 1 ? term[1][2 * step + 1] : 0u);
+        if (V::kQRegs) q_regs[V::kQRegs ? step : 0] = a;
+        else reinterpret_cast<uint4*>(gen + V::kQ)[(mt * 8 + step) * 32 + lane] = a;
+      }
     }
     if (p.sq.len > 1)
       for (int d = lane; d < 128; d += 32) sm_nan[d] = 0x7fffffff;
     __syncwarp();
 
-    float m[MT], l[MT];
-    f32x2 acc[MT][16];  // dimensions 32 c + n and 32 c + 16 + n
+    float m[ROWS], l[ROWS], acc[MT][16][4];  // dimensions 32 c + n and 32 c + 16 + n, in units of vref * 2^-14
+    float vref = 0.0f;                       // largest scale of the values so far
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      m[mt] = -INFINITY;
-      l[mt] = 0.0f;
-#pragma unroll
-      for (int n = 0; n < 16; ++n) acc[mt][n] = 0ull;
+    for (int n = 0; n < ROWS; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < 16; ++n) acc[mt][n][0] = acc[mt][n][1] = acc[mt][n][2] = acc[mt][n][3] = 0.0f;
     rest -= p.end - p.j;
     for (; p.j < p.end; ++p.j, ++count) {
       const int st = count & (ST - 1), kb = p.j * kSlice;
@@ -370,112 +387,126 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         const uint32_t kt = base + st * kStage + g * 128, vt = base + st * kStage + kBox, sc = base + V::kScales + st * 16;
         const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + 8), vs1 = lds32(sc + 12);
         const bool masked = kb + kSlice > p.sq.pos + 1;
-        // ---- scores: key 8 t + g of the slice is column g of block t; lane c reads the dimensions whose terms it holds of the query ----
-        uint4 kw[4][2];
+        // ---- scores: key 8 t + g of the slice is column g of block t; lane c reads the dimensions that it holds of the query ----
+        float x[MT][4][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) kw[t][h] = lds128(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
-        uint4 pf[MT][TP];
-        float beta[MT];
-        const float vmax = fmaxf(vs0, vs1);
-        float r0 = 256.0f, r1 = 256.0f;
-        if (vs0 != vs1) {
-          const float inv = vmax > 0.0f ? 256.0f / vmax : 0.0f;
-          r0 = vs0 * inv;
-          r1 = vs1 * inv;
-        }
+          for (int t = 0; t < 4; ++t) x[mt][t][0] = x[mt][t][1] = x[mt][t][2] = x[mt][t][3] = 0.0f;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float x[4][2];
+        for (int h = 0; h < 2; ++h) {
+          uint4 kw[4];
 #pragma unroll
-          for (int tp = TP - 1; tp >= 0; --tp) {
-            uint4 qa[4];
+          for (int t = 0; t < 4; ++t) kw[t] = lds128(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
 #pragma unroll
-            for (int step = 0; step < 4; ++step)
-              qa[step] = V::kSmall ? q_terms[step & (V::kSmall ? 3 : 0)] : lds128(base + V::kQ + (((mt * TP + tp) * 4 + step) * 32 + lane) * 16);
+          for (int i = 0; i < 4; ++i) {
+            uint4 qa[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              qa[mt] = V::kQRegs ? q_regs[V::kQRegs ? 4 * h + i : 0] : lds128(base + V::kQ + ((mt * 8 + 4 * h + i) * 32 + lane) * 16);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-              float d[4];
-              mma_e4m3_16832_first(d, qa[0], kw[t][0].x, kw[t][0].y);
-              mma_e4m3_16832(d, qa[1], kw[t][0].z, kw[t][0].w);
-              mma_e4m3_16832(d, qa[2], kw[t][1].x, kw[t][1].y);
-              mma_e4m3_16832(d, qa[3], kw[t][1].z, kw[t][1].w);
+              uint32_t b0, b1;
+              widen(i == 0 ? kw[t].x : i == 1 ? kw[t].y : i == 2 ? kw[t].z : kw[t].w, b0, b1);
 #pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const float both = fmaf(d[2 + z], 0.0625f, d[z]);
-                x[t][z] = tp == TP - 1 ? both : fmaf(x[t][z], 1.0f / 256.0f, both);
-              }
+              for (int mt = 0; mt < MT; ++mt) mma_f16_16816(x[mt][t], qa[mt], b0, b1);
             }
           }
-          const float f0 = factor[mt] * ks0, f1 = factor[mt] * ks1;
+        }
+        if (V::kTerms) {
 #pragma unroll
           for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int z = 0; z < 2; ++z) x[t][z] *= t < 2 ? f0 : f1;
-          if (s.cap_l2 > 0.0f) {
+            for (int z = 0; z < 2; ++z) x[0][t][z] = fmaf(x[0][t][2 + z], 1.0f / 2048.0f, x[0][t][z]);
+        }
+        // ---- a new reference for the values' scales (rare) ----
+        const float vmax = fmaxf(vs0, vs1);
+        if (vmax > vref) {
+          const float down = vref / vmax;
+          vref = vmax;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+#pragma unroll
+              for (int z = 0; z < 2 * HV; ++z) acc[mt][n][z] *= down;
+        }
+        const float inv = vref > 0.0f ? 16384.0f / vref : 0.0f, r0 = vs0 * inv, r1 = vs1 * inv;
+        uint4 pf[MT][2];  // A fragments of the values' product, for the first and the last 16 keys
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t pw[4][2];
+#pragma unroll
+          for (int h = 0; h < RH; ++h) {
+            const int n = RH * mt + h;
+            float y[4][2];
+            const float f0 = factor[n] * ks0, f1 = factor[n] * ks1;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) x[t][z] = softcap_log2(x[t][z], s.two_over_cap, s.cap_l2);
-          }
-          if (masked) {
-            const int see = rows_limit[mt] - kb - 2 * c;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-              for (int z = 0; z < 2; ++z) x[t][z] = 8 * t + z < see ? x[t][z] : -INFINITY;
-          }
-          float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
-          if (s.scores) {
-            const int r = p.rg * R + mt * 8 + g;  // (single tokens: a row is a query head of the group)
-            if (r < s.G) {
-              float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.c.cap + kb + 2 * c;
+              for (int z = 0; z < 2; ++z) y[t][z] = x[mt][t][2 * h + z] * (t < 2 ? f0 : f1);
+            if (s.cap_l2 > 0.0f) {
 #pragma unroll
               for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int z = 0; z < 2; ++z)
-                  if (!masked || kb + 8 * t + 2 * c + z < p.limit) to[8 * t + z] = x[t][z];
+                for (int z = 0; z < 2; ++z) y[t][z] = softcap_log2(y[t][z], s.two_over_cap, s.cap_l2);
             }
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float from = top == -INFINITY ? 0.0f : top;
-          if (__any_sync(0xffffffffu, top > m[mt])) {  // (rare once a sequence is under way)
-            const float m_new = fmaxf(m[mt], top), alpha = ex2(m[mt] - (m_new == -INFINITY ? 0.0f : m_new));
-            m[mt] = m_new;
-            l[mt] *= alpha;
+            if (masked) {
+              const int see = rows_limit[n] - kb - 2 * c;
 #pragma unroll
-            for (int n = 0; n < 16; ++n) acc[mt][n] = mul2(acc[mt][n], pack2(alpha, alpha));
-          }
-          beta[mt] = ex2(top - (m[mt] == -INFINITY ? 0.0f : m[mt]));
-          float sum = 0.0f;
+              for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              x[t][z] = ex2(x[t][z] - from);
-              sum += x[t][z];
-              x[t][z] *= t < 2 ? r0 : r1;
+                for (int z = 0; z < 2; ++z) y[t][z] = 8 * t + z < see ? y[t][z] : -INFINITY;
             }
-          l[mt] = fmaf(sum, beta[mt], l[mt]);
-          beta[mt] *= vmax * (1.0f / 256.0f);
-          // A fragments of the values' product: keys 2c, 2c + 1 of blocks 0, 1 (then 2, 3)
+            if (s.scores) {
+              const int r = p.rg * R + mt * 16 + 8 * h + g;  // (single tokens: a row is a query head of the group)
+              if (r < s.G) {
+                float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.c.cap + kb + 2 * c;
 #pragma unroll
-          for (int tp = 0; tp < TP; ++tp) {
-            uint32_t w[2][2];
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int z = 0; z < 2; ++z)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const uint32_t lo = take_term(x[2 * half][0], x[2 * half][1]), hi = take_term(x[2 * half + 1][0], x[2 * half + 1][1]);
-                w[z][half] = lo | hi << 16;
+                  for (int z = 0; z < 2; ++z)
+                    if (!masked || kb + 8 * t + 2 * c + z < p.limit) to[8 * t + z] = y[t][z];
               }
-            pf[mt][tp] = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
+            }
+            float top = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1])), fmaxf(fmaxf(y[2][0], y[2][1]), fmaxf(y[3][0], y[3][1])));
+            if (__any_sync(0xffffffffu, top > m[n])) {  // (rare once a sequence is under way)
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+              const float m_new = fmaxf(m[n], top), alpha = ex2(m[n] - (m_new == -INFINITY ? 0.0f : m_new));
+              m[n] = m_new;
+              l[n] *= alpha;
+#pragma unroll
+              for (int d = 0; d < 16; ++d) {
+                acc[mt][d][2 * h] *= alpha;
+                acc[mt][d][2 * h + 1] *= alpha;
+                if (V::kTerms) {
+                  acc[mt][d][2] *= alpha;
+                  acc[mt][d][3] *= alpha;
+                }
+              }
+            }
+            const float from = m[n] == -INFINITY ? 0.0f : m[n];
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                y[t][z] = ex2(y[t][z] - from);
+                sum += y[t][z];
+                y[t][z] *= t < 2 ? r0 : r1;
+              }
+              pw[t][h] = pack_f16x2(y[t][0], y[t][1]);
+              if (V::kTerms) pw[t][1] = rest_f16x2(pw[t][0], y[t][0], y[t][1]);
+            }
+            l[n] += sum;
           }
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+            pf[mt][kk] = make_uint4(pw[2 * kk][0], HV > 1 ? pw[2 * kk][1] : 0u, pw[2 * kk + 1][0], HV > 1 ? pw[2 * kk + 1][1] : 0u);
         }
-        // ---- values: lane (g, c) reads the dimensions 16 g .. 16 g + 15 of the keys whose probabilities it holds; transposed by bytes they are the
-        // B fragments of 16 blocks of eight dimensions {16 g + n} ----
+        // ---- values: lane (g, c) reads the dimensions 16 g .. 16 g + 15 of the keys whose probabilities it holds; pairs of keys by bytes, then
+        // widened, they are the B fragments of 16 blocks of eight dimensions {16 g + n} ----
         uint4 vw[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -504,40 +535,25 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t b[2][4];
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t w[4];
+          for (int kk = 0; kk < 2; ++kk) {
+            uint32_t w[4], b[2][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint4& v = vw[4 * half + i];
+              const uint4& v = vw[4 * kk + i];
               w[i] = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
             }
-            const uint32_t l01 = __byte_perm(w[0], w[1], 0x5140), h01 = __byte_perm(w[0], w[1], 0x7362);
-            const uint32_t l23 = __byte_perm(w[2], w[3], 0x5140), h23 = __byte_perm(w[2], w[3], 0x7362);
-            b[half][0] = __byte_perm(l01, l23, 0x5410);
-            b[half][1] = __byte_perm(l01, l23, 0x7632);
-            b[half][2] = __byte_perm(h01, h23, 0x5410);
-            b[half][3] = __byte_perm(h01, h23, 0x7632);
-          }
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const f32x2 be = pack2(beta[mt], beta[mt]), sixteenth = pack2(0.0625f, 0.0625f);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              f32x2 o = 0ull;
-#pragma unroll
-              for (int tp = TP - 1; tp >= 0; --tp) {
-                float d[4];
-                mma_e4m3_16832_first(d, pf[mt][tp], b[0][n], b[1][n]);
-                const f32x2 both = fma2(pack2(d[2], d[3]), sixteenth, pack2(d[0], d[1]));
-                o = tp == TP - 1 ? both : fma2(o, pack2(1.0f / 256.0f, 1.0f / 256.0f), both);
-              }
-              acc[mt][4 * k + n] = fma2(o, be, acc[mt][4 * k + n]);
+            for (int i = 0; i < 2; ++i) {
+              widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), b[i][0], b[i][1]);
+              widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), b[i][2], b[i][3]);
             }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) mma_f16_16816(acc[mt][4 * k + n], pf[mt][kk], b[0][n], b[1][n]);
           }
-        }
       }
       __syncwarp();
       load_next();
@@ -545,47 +561,50 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
     // ---- the rows' results, or this warp's part of them ----
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 1);
-      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 2);
-      const long long r = static_cast<long long>(p.rg) * R + mt * 8 + g;
-      const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-      if (i >= p.sq.len) continue;
-      float o[2][16];
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        const float2 v = unpack2(acc[mt][n]);
-        o[0][n] = v.x;
-        o[1][n] = v.y;
+      for (int h = 0; h < RH; ++h) {
+        const int n = RH * mt + h, r_in = mt * 16 + 8 * h + g;
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+        const long long r = static_cast<long long>(p.rg) * R + r_in;
+        const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+        if (i >= p.sq.len) continue;
+        float o[2][16];
+        const float unit = vref * (1.0f / 16384.0f);
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+            o[z][d] = (V::kTerms ? fmaf(acc[mt][d][2 + z], 1.0f / 2048.0f, acc[mt][d][z]) : acc[mt][d][2 * h + z]) * unit;
+        if (p.sq.len > 1) {
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int d = 0; d < 16; ++d)
+              if (rows_limit[n] > sm_nan[32 * c + 16 * z + d]) o[z][d] = __uint_as_float(0x7fffffffu);
+        }
+        if (!p.whole) {
+          const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + r_in;
+          if (c == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(m[n], l[n]);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) store16(s.part_o + slot * 128 + 32 * c + 16 * z, o[z], true);
+          continue;
+        }
+        const size_t row = static_cast<size_t>(p.sq.row0) + i;
+        if (s.a.sink) l[n] += ex2(fmaf(s.a.sink[hq], kLog2e, -m[n]));
+        if (c == 0) note_lse(s, row, hq, m[n] + log2f(l[n]));
+        const float inv = 1.0f / l[n];
+        T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int d0 = 32 * c + 16 * z;
+          if (d0 >= s.c.V) continue;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) o[z][d] = finished<T>(s, row, hq, d0 + d, o[z][d], inv);
+          store16(out + d0, o[z], s.vec_o);
+        }
       }
-      if (p.sq.len > 1) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-            if (rows_limit[mt] > sm_nan[32 * c + 16 * h + n]) o[h][n] = __uint_as_float(0x7fffffffu);
-      }
-      if (!p.whole) {
-        const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + mt * 8 + g;
-        if (c == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(m[mt], l[mt]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) store16(s.part_o + slot * 128 + 32 * c + 16 * h, o[h], true);
-        continue;
-      }
-      const size_t row = static_cast<size_t>(p.sq.row0) + i;
-      if (s.a.sink) l[mt] += ex2(fmaf(s.a.sink[hq], kLog2e, -m[mt]));
-      if (c == 0) note_lse(s, row, hq, m[mt] + log2f(l[mt]));
-      const float inv = 1.0f / l[mt];
-      T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int d0 = 32 * c + 16 * h;
-        if (d0 >= s.c.V) continue;
-#pragma unroll
-        for (int n = 0; n < 16; ++n) o[h][n] = finished<T>(s, row, hq, d0 + n, o[h][n], inv);
-        store16(out + d0, o[h], s.vec_o);
-      }
-    }
     if (rest == 0) return;
     next_piece(s, p, R, rest);
     __syncwarp();
@@ -668,9 +687,11 @@ __global__ void __launch_bounds__(256) cache8_weights_kernel(const __grid_consta
 }
 
 // Weights of calls with several tokens: the scores once more, from the rows' lse.  A warp takes 32 keys of a (kv head, entry) and goes through the
-// rows eight at a time.
-template <typename T, int TP>
+// rows, 16 at a time (f32: eight, in two terms).
+template <typename T>
 __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_constant__ Shared s) {
+  constexpr bool kTerms = sizeof(T) == 4;
+  constexpr int RH = kTerms ? 1 : 2, R = 8 * RH;
   pdl_wait();
   const int e = blockIdx.z, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const SeqDesc sq = s.seqs[e];
@@ -693,35 +714,44 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
     ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + (kb + 16) / s.c.B] : 0.0f;
     float sum[4][2] = {};
     const long long rows = static_cast<long long>(sq.len) * s.G;
-    for (long long r0 = static_cast<long long>(max(0, kb - sq.pos)) * s.G / 8 * 8; r0 < rows; r0 += 8) {
-      const long long r = r0 + g;
-      const int i = static_cast<int>(min(r, rows - 1) / s.G), hq = hk * s.G + static_cast<int>(min(r, rows - 1) - static_cast<long long>(i) * s.G);
-      const size_t row = static_cast<size_t>(sq.row0) + i;
-      uint32_t term[2 * TP][8];
-      const float f = split_row<T, 2 * TP>(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c,
-                                           s.scale_log2, term);
-      const float z = s.lse2[row * s.a.Hq + hq];
+    for (long long r0 = static_cast<long long>(max(0, kb - sq.pos)) * s.G / R * R; r0 < rows; r0 += R) {
+      uint32_t term[2][16];
+      float f[RH], z[RH];
+      int sees[RH];
+#pragma unroll
+      for (int h = 0; h < RH; ++h) {
+        const long long r = r0 + 8 * h + g, at = min(r, rows - 1);
+        const int i = static_cast<int>(at / s.G), hq = hk * s.G + static_cast<int>(at - static_cast<long long>(i) * s.G);
+        const size_t row = static_cast<size_t>(sq.row0) + i;
+        const T* q = static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
+        if constexpr (kTerms) f[h] = split_row<T, 2>(q, s.c.D, r < rows, s.vec_q, c, s.scale_log2, term);
+        else {
+          uint32_t one[1][16];
+          f[h] = split_row<T, 1>(q, s.c.D, r < rows, s.vec_q, c, s.scale_log2, one);
+#pragma unroll
+          for (int w = 0; w < 16; ++w) term[h][w] = one[0][w];
+        }
+        z[h] = s.lse2[row * s.a.Hq + hq];
+        sees[h] = r < rows ? sq.pos + i + 1 - kb - 2 * c : -64;
+      }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        float x[2] = {0.0f, 0.0f};
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int tp = TP - 1; tp >= 0; --tp) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int step = 0; step < 8; ++step) {
+          const uint4& k = kw[t][step >> 2];
+          uint32_t b0, b1;
+          widen((step & 3) == 0 ? k.x : (step & 3) == 1 ? k.y : (step & 3) == 2 ? k.z : k.w, b0, b1);
+          mma_f16_16816(d, make_uint4(term[0][2 * step], term[1][2 * step], term[0][2 * step + 1], term[1][2 * step + 1]), b0, b1);
+        }
 #pragma unroll
-          for (int step = 0; step < 4; ++step) {
-            const uint4 a = make_uint4(term[2 * tp][2 * step], term[2 * tp + 1][2 * step], term[2 * tp][2 * step + 1], term[2 * tp + 1][2 * step + 1]);
-            const uint4& k = kw[t][step >> 1];
-            mma_e4m3_16832(d, a, step & 1 ? k.z : k.x, step & 1 ? k.w : k.y);
+        for (int h = 0; h < RH; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float v = (kTerms ? fmaf(d[2 + y], 1.0f / 2048.0f, d[y]) : d[2 * h + y]) * (f[h] * ks[t >> 1]);
+            if (s.cap_l2 > 0.0f) v = softcap_log2(v, s.two_over_cap, s.cap_l2);
+            if (8 * t + y < sees[h]) sum[t][y] += ex2(v - z[h]);
           }
-          x[0] = fmaf(x[0], 1.0f / 256.0f, fmaf(d[2], 0.0625f, d[0]));
-          x[1] = fmaf(x[1], 1.0f / 256.0f, fmaf(d[3], 0.0625f, d[1]));
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float v = x[y] * (f * ks[t >> 1]);
-          if (s.cap_l2 > 0.0f) v = softcap_log2(v, s.two_over_cap, s.cap_l2);
-          if (r < rows && kb + 8 * t + 2 * c + y <= sq.pos + i) sum[t][y] += ex2(v - z);
-        }
       }
     }
 #pragma unroll
@@ -739,39 +769,32 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
 
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
-  int mt, parts, groups;
+  int kind, rows, parts, groups;
   size_t part_o, part_ml, lse2, scores, bytes;
 };
-int row_tiles(int f32, int G, int max_len) {
-  // as few passes over the keys as rows allow, and no more row tiles than those need
-  const int most = f32 ? 1 : 4;
-  const long long rows = static_cast<long long>(G) * max_len, passes = (rows + 8 * most - 1) / (8 * most);
-  return static_cast<int>((rows + 8 * passes - 1) / (8 * passes));
+template <typename F>
+void for_variant(int kind, F&& f) {
+  if (kind == kEight) f(cache8_attention_kernel<kEight>, Variant<kEight>{});
+  else if (kind == kSixteen) f(cache8_attention_kernel<kSixteen>, Variant<kSixteen>{});
+  else if (kind == kPair) f(cache8_attention_kernel<kPair>, Variant<kPair>{});
+  else f(cache8_attention_kernel<kF32>, Variant<kF32>{});
 }
 Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights) {
   Plan p{};
-  const int G = Hq / c.H;
-  p.mt = row_tiles(f32, G, max_len);
-  p.groups = static_cast<int>((static_cast<long long>(G) * max_len + 8 * p.mt - 1) / (8 * p.mt));
-  p.parts = sm_count() * (!f32 && p.mt == 1 ? 3 : 2) * kWarps;  // (the warps that are resident at once)
+  const long long unit = static_cast<long long>(Hq / c.H) * max_len;  // rows of the longest entry and a kv head
+  p.kind = f32 ? kF32 : unit <= 8 ? kEight : unit <= 16 ? kSixteen : kPair;
+  for_variant(p.kind, [&](auto, auto v) {
+    using V = decltype(v);
+    p.rows = V::kRows;
+    p.parts = sm_count() * V::kCtas * kWarps;  // the warps that are resident at once
+  });
+  p.groups = static_cast<int>((unit + p.rows - 1) / p.rows);
   auto take = [&](size_t n) { const size_t at = p.bytes; p.bytes += (n + 255) / 256 * 256; return at; };
-  p.part_o = take(static_cast<size_t>(2) * p.parts * 8 * p.mt * 128 * 4);
-  p.part_ml = take(static_cast<size_t>(2) * p.parts * 8 * p.mt * 2 * 4);
+  p.part_o = take(static_cast<size_t>(2) * p.parts * p.rows * 128 * 4);
+  p.part_ml = take(static_cast<size_t>(2) * p.parts * p.rows * 2 * 4);
   p.lse2 = weights ? take(static_cast<size_t>(rows) * Hq * 4) : 0;
   p.scores = weights && max_len == 1 ? take(static_cast<size_t>(n_seqs) * Hq * c.cap * 4) : 0;
   return p;
-}
-
-template <typename F>
-void for_variant(int f32, int mt, F&& f) {
-  if (f32) {
-    f(cache8_attention_kernel<float, 3, 1>, Variant<3, 1>{});
-  } else {
-    if (mt == 1) f(cache8_attention_kernel<bf16, 1, 1>, Variant<1, 1>{});
-    else if (mt == 2) f(cache8_attention_kernel<bf16, 1, 2>, Variant<1, 2>{});
-    else if (mt == 3) f(cache8_attention_kernel<bf16, 1, 3>, Variant<1, 3>{});
-    else f(cache8_attention_kernel<bf16, 1, 4>, Variant<1, 4>{});
-  }
 }
 int prepare() {
   static std::atomic<unsigned long long> done{0};  // one bit per device; threads may race to set it
@@ -779,12 +802,11 @@ int prepare() {
   cudaGetDevice(&dev);
   if (dev < 64 && (done.load(std::memory_order_acquire) >> dev) & 1ull) return 0;
   cudaError_t e = cudaSuccess;
-  for (int f32 = 0; f32 < 2; ++f32)
-    for (int mt = 1; mt <= (f32 ? 1 : 4); ++mt)
-      for_variant(f32, mt, [&](auto kernel, auto v) {
-        const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(v)::kBytes);
-        if (e == cudaSuccess) e = rc;
-      });
+  for (int kind : {kEight, kSixteen, kPair, kF32})
+    for_variant(kind, [&](auto kernel, auto v) {
+      const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(v)::kBytes);
+      if (e == cudaSuccess) e = rc;
+    });
   if (e != cudaSuccess) return static_cast<int>(e);
   if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   return 0;
@@ -836,20 +858,20 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   s.vec_o = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) & 15) == 0;
   s.err = device_error_word();
   if (!s.err) return TEENY_ERR_DRIVER;
-  for_variant(a.f32, p.mt, [&](auto kernel, auto v) {
+  for_variant(p.kind, [&](auto kernel, auto v) {
     using V = decltype(v);
     launch_kernel(kernel, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
   });
   const PdlScope behind;
   const dim3 units(static_cast<unsigned>(n_seqs) * c.H * p.groups);
-  if (a.f32) launch_kernel(cache8_combine_kernel<float>, units, dim3(256), 0, st, 1, s, 8 * p.mt, p.groups);
-  else launch_kernel(cache8_combine_kernel<bf16>, units, dim3(256), 0, st, 1, s, 8 * p.mt, p.groups);
+  if (a.f32) launch_kernel(cache8_combine_kernel<float>, units, dim3(256), 0, st, 1, s, p.rows, p.groups);
+  else launch_kernel(cache8_combine_kernel<bf16>, units, dim3(256), 0, st, 1, s, p.rows, p.groups);
   if (a.weights) {
     const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
     if (max_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);
-    else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float, 3>, grid, dim3(128), 0, st, 1, s);
-    else launch_kernel(cache8_rows_weights_kernel<bf16, 1>, grid, dim3(128), 0, st, 1, s);
+    else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float>, grid, dim3(128), 0, st, 1, s);
+    else launch_kernel(cache8_rows_weights_kernel<bf16>, grid, dim3(128), 0, st, 1, s);
   }
   return static_cast<int>(cudaGetLastError());
 }
