@@ -3,11 +3,11 @@
 //
 // Both products run on f16 operands with f32 sums (mma.sync m16n8k16): an E4M3 number is an f16 number exactly, and one conversion makes two of
 // them.  (mma.sync on E4M3 operands is made of the same f16 products here, with additions of its own behind each: 0.19 m16n8k32 a clock
-// and SM, where the f16 pairs run at 0.42 / 2.)  A query row is scaled by a power of two so that its largest number is in [2^14, 2^15): a bf16
-// number below 2^-28 of that loses bits, no other.  f32 rows are two f16 terms, 22 bits, in rows 0-7 and 8-15 of a tile: the halves
-// of a sum lie in the same thread's registers.  Probabilities are f16 numbers times 2^14 (f32: two terms as well), so that a key is lost
-// only 2^-38 below the row's maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to
-// the largest so far, the probabilities.
+// and SM, where the f16 pairs run at 0.42 / 2.)  The 16 rows of a product are keys, then dimensions of the values; its eight columns are query rows,
+// so that few query heads waste nothing.  A query row is scaled by a power of two so that its largest number is in [2^14, 2^15): a bf16
+// number below 2^-28 of that loses bits, no other.  f32 rows are two f16 terms, 22 bits, in two columns tiles whose sums lie in the same thread's
+// registers.  Probabilities are f16 numbers times 2^14 (f32: two terms as well), so that a key is lost only 2^-38 below the row's
+// maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to the largest so far, the probabilities.
 //
 // The call is bound by reading the cache.  Every warp works alone: it takes slices of 32 keys of one sequence and head, and keeps the next ones in
 // flight itself (keys and values by TMA, their scales by 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry
@@ -15,7 +15,6 @@
 // the lengths.  A sequence that lies in several warps' shares leaves partial results in scratch, at most two for each warp, which a
 // second kernel adds.  No warp waits for another.
 #include <atomic>
-#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -32,31 +31,35 @@ constexpr int kBox = kSlice * kCache8Head;     // 4 KB: their keys, or their val
 constexpr int kStage = 2 * kBox;
 constexpr int kWarps = 4;                      // of a CTA
 
-// Variant of the kernel: tiles of the query's rows, which are eight bf16 rows (kEight), 16 (kSixteen), 2 x 16 (kPair), or eight f32 rows in two terms
-// (kF32).  Eight bf16 rows fit 168 registers, with which an SM has twelve warps; the others take eight.
-enum : int { kEight = 0, kSixteen, kPair, kF32 };
-template <int KIND>
+// Variant of the kernel: RT tiles of eight query rows in TERMS f16 terms (bf16: 1, f32: 2).  Up to two column tiles fit 168 registers, with which an SM
+// has twelve warps; more take eight.
+template <int RT_, int TERMS_>
 struct Variant {
-  static constexpr int kTiles = KIND == kPair ? 2 : 1, kRows = KIND == kEight || KIND == kF32 ? 8 : 16 * kTiles;
-  static constexpr int kHalves = KIND == kEight ? 1 : 2;  // halves of a tile whose sums are used
-  static constexpr int kCtas = KIND == kEight ? 3 : 2, kStages = 2;
-  static constexpr bool kTerms = KIND == kF32, kQRegs = KIND != kPair;
-  using T = typename std::conditional<KIND == kF32, float, bf16>::type;
-  // a warp's part of shared memory: stages, scales f32 [stages][4], queries uint4 [tiles][8 steps][32 lanes] (in registers but for kPair), int [128] first NaN
-  // value of each dimension, barriers
+  static constexpr int RT = RT_, TERMS = TERMS_, NT = RT * TERMS, kRows = 8 * RT, kCtas = NT <= 2 ? 3 : 2, kStages = 2;
+  static constexpr bool kQRegs = NT <= 2;
+  using T = typename std::conditional<TERMS == 2, float, bf16>::type;
+  // a warp's part of shared memory: stages, scales f32 [stages][4], queries uint2 [column tiles][8 steps][32 lanes] (up to two tiles: in registers), int [128]
+  // first NaN value of each dimension, barriers
   static constexpr int kScales = kStages * kStage;
-  static constexpr int kQ = kScales + kStages * 16;
-  static constexpr int kNan = kQ + (kQRegs ? 0 : kTiles * 8 * 32 * 16);
+  static constexpr int kNan = kScales + kStages * 16;
   static constexpr int kBars = kNan + 128 * 4;
-  static constexpr int kWarpBytes = (kBars + kStages * 8 + 1023) / 1024 * 1024;
+  static constexpr int kQ = kBars + kStages * 8;
+  static constexpr int kWarpBytes = (kQ + (kQRegs ? 0 : NT * 8 * 32 * 8) + 1023) / 1024 * 1024;
   static constexpr int kBytes = kWarps * kWarpBytes + 1024;
   static_assert((kBytes + 1024) * kCtas <= 233472, "shared memory");
 };
 
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+// D (16 x 8) += A (16 x 16) B
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 x 8 16-bit numbers: lane (g, c) gives (row g, columns 2c, 2c + 1) and gets (rows 2c, 2c + 1 of column g)
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 // Four E4M3 numbers as two f16 pairs
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -239,14 +242,11 @@ __device__ __forceinline__ void next_piece(const Shared& s, Piece& p, int rows, 
   piece_range(s, p, rows, 0, left);
 }
 
-template <int KIND>
-__global__ void __launch_bounds__(32 * kWarps, Variant<KIND>::kCtas)
+template <typename V>
+__global__ void __launch_bounds__(32 * kWarps, V::kCtas)
 cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Shared s) {
-  using V = Variant<KIND>;
   using T = typename V::T;
-  constexpr int R = V::kRows, ST = V::kStages, MT = V::kTiles, HV = V::kHalves;
-  // a lane's rows: those of its accumulators' halves (f32: the second half is the first one's second term)
-  constexpr int RH = V::kTerms ? 1 : HV, ROWS = MT * RH;
+  constexpr int R = V::kRows, ST = V::kStages, RT = V::RT, TERMS = V::TERMS, NT = V::NT;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const uint32_t offset = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw) + warp * V::kWarpBytes;
@@ -301,6 +301,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     load.first = true;
     piece_range(s, load, R, static_cast<int>(at - unit * es.slices), left);
   }
+  pdl_trigger();
   Piece p = load;
   long long rest = left;  // slices of the share that are still to be computed
   int issued = 0, count = 0;
@@ -330,51 +331,51 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
   int* sm_nan = reinterpret_cast<int*>(gen + V::kNan);
   for (;;) {
-    // ---- queries as A fragments; row tile mt's row g + 8 h is this lane's row n = RH mt + h ----
-    float factor[ROWS];
-    int rows_limit[ROWS];  // keys that the rows see
-    uint4 q_regs[V::kQRegs ? 8 : 1];
+    // ---- queries as B fragments: row g of tile rt is column g ----
+    float factor[RT][2];      // of the rows 2c, 2c + 1, whose scores this lane gets
+    int rows_limit[RT][2];    // keys that they see
+    uint2 q_regs[V::kQRegs ? NT * 8 : 1];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      uint32_t term[2][16];
+    for (int rt = 0; rt < RT; ++rt) {
+      const long long r = static_cast<long long>(p.rg) * R + rt * 8 + g;
+      const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+      const bool valid = i < p.sq.len;
+      const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
+      uint32_t term[TERMS][16];
+      const float f = split_row<T, TERMS>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
+      const int see = valid ? p.sq.pos + i + 1 : p.limit;
 #pragma unroll
-      for (int h = 0; h < RH; ++h) {
-        const int n = RH * mt + h;
-        const long long r = static_cast<long long>(p.rg) * R + mt * 16 + 8 * h + g;
-        const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-        const bool valid = i < p.sq.len;
-        rows_limit[n] = valid ? p.sq.pos + i + 1 : p.limit;
-        const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
-        if constexpr (V::kTerms) factor[n] = split_row<T, 2>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
-        else {
-          uint32_t one[1][16];
-          factor[n] = split_row<T, 1>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, one);
+      for (int z = 0; z < 2; ++z) {
+        factor[rt][z] = __shfl_sync(0xffffffffu, f, (2 * c + z) * 4);
+        rows_limit[rt][z] = __shfl_sync(0xffffffffu, see, (2 * c + z) * 4);
+      }
 #pragma unroll
-          for (int w = 0; w < 16; ++w) term[h][w] = one[0][w];
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int step = 0; step < 8; ++step) {
+          const uint2 b = make_uint2(term[t][2 * step], term[t][2 * step + 1]);
+          if (V::kQRegs) q_regs[V::kQRegs ? (rt * TERMS + t) * 8 + step : 0] = b;
+          else reinterpret_cast<uint2*>(gen + V::kQ)[((rt * TERMS + t) * 8 + step) * 32 + lane] = b;
         }
-      }
-#pragma unroll
-      for (int step = 0; step < 8; ++step) {
-        const uint4 a = make_uint4(term[0][2 * step], HV > 1 ? term[1][2 * step] : 0u, term[0][2 * step + 1], HV > 1 ? term[1][2 * step + 1] : 0u);
-        if (V::kQRegs) q_regs[V::kQRegs ? step : 0] = a;
-        else reinterpret_cast<uint4*>(gen + V::kQ)[(mt * 8 + step) * 32 + lane] = a;
-      }
     }
     if (p.sq.len > 1)
       for (int d = lane; d < 128; d += 32) sm_nan[d] = 0x7fffffff;
     __syncwarp();
 
-    float m[ROWS], l[ROWS], acc[MT][16][4];  // dimensions 32 c + n and 32 c + 16 + n, in units of vref * 2^-14
-    float vref = 0.0f;                       // largest scale of the values so far
+    // acc[tile][j]: dimensions 16 g + 2j (rows 2c, 2c + 1), 16 g + 2j + 1 (the same), in units of vref * 2^-14
+    float m[RT][2], l[RT][2], acc[NT][8][4];
+    float vref = 0.0f;  // largest scale of the values so far
 #pragma unroll
-    for (int n = 0; n < ROWS; ++n) {
-      m[n] = -INFINITY;
-      l[n] = 0.0f;
-    }
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int z = 0; z < 2; ++z) {
+        m[rt][z] = -INFINITY;
+        l[rt][z] = 0.0f;
+      }
 #pragma unroll
-      for (int n = 0; n < 16; ++n) acc[mt][n][0] = acc[mt][n][1] = acc[mt][n][2] = acc[mt][n][3] = 0.0f;
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.0f;
     rest -= p.end - p.j;
     for (; p.j < p.end; ++p.j, ++count) {
       const int st = count & (ST - 1), kb = p.j * kSlice;
@@ -387,12 +388,12 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         const uint32_t kt = base + st * kStage + g * 128, vt = base + st * kStage + kBox, sc = base + V::kScales + st * 16;
         const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + 8), vs1 = lds32(sc + 12);
         const bool masked = kb + kSlice > p.sq.pos + 1;
-        // ---- scores: key 8 t + g of the slice is column g of block t; lane c reads the dimensions that it holds of the query ----
-        float x[MT][4][4];
+        // ---- scores: keys 16 u + g and 16 u + 8 + g of the slice are rows g and g + 8 of tile u; lane c reads the dimensions that it holds of the query ----
+        float x[NT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) x[mt][t][0] = x[mt][t][1] = x[mt][t][2] = x[mt][t][3] = 0.0f;
+          for (int u = 0; u < 2; ++u) x[nt][u][0] = x[nt][u][1] = x[nt][u][2] = x[nt][u][3] = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4 kw[4];
@@ -400,24 +401,20 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           for (int t = 0; t < 4; ++t) kw[t] = lds128(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint4 qa[MT];
+            uint2 qb[NT];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-              qa[mt] = V::kQRegs ? q_regs[V::kQRegs ? 4 * h + i : 0] : lds128(base + V::kQ + ((mt * 8 + 4 * h + i) * 32 + lane) * 16);
+            for (int nt = 0; nt < NT; ++nt)
+              qb[nt] = V::kQRegs ? q_regs[V::kQRegs ? nt * 8 + 4 * h + i : 0] : reinterpret_cast<const uint2*>(gen + V::kQ)[(nt * 8 + 4 * h + i) * 32 + lane];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              uint32_t b0, b1;
-              widen(i == 0 ? kw[t].x : i == 1 ? kw[t].y : i == 2 ? kw[t].z : kw[t].w, b0, b1);
+            for (int u = 0; u < 2; ++u) {
+              uint32_t a[4];
+              const uint4 &k0 = kw[2 * u], &k1 = kw[2 * u + 1];
+              widen(i == 0 ? k0.x : i == 1 ? k0.y : i == 2 ? k0.z : k0.w, a[0], a[2]);
+              widen(i == 0 ? k1.x : i == 1 ? k1.y : i == 2 ? k1.z : k1.w, a[1], a[3]);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) mma_f16_16816(x[mt][t], qa[mt], b0, b1);
+              for (int nt = 0; nt < NT; ++nt) mma_f16_16816(x[nt][u], a[0], a[1], a[2], a[3], qb[nt].x, qb[nt].y);
             }
           }
-        }
-        if (V::kTerms) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int z = 0; z < 2; ++z) x[0][t][z] = fmaf(x[0][t][2 + z], 1.0f / 2048.0f, x[0][t][z]);
         }
         // ---- a new reference for the values' scales (rare) ----
         const float vmax = fmaxf(vs0, vs1);
@@ -425,88 +422,86 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
           const float down = vref / vmax;
           vref = vmax;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int n = 0; n < 16; ++n)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-              for (int z = 0; z < 2 * HV; ++z) acc[mt][n][z] *= down;
+              for (int z = 0; z < 4; ++z) acc[nt][j][z] *= down;
         }
         const float inv = vref > 0.0f ? 16384.0f / vref : 0.0f, r0 = vs0 * inv, r1 = vs1 * inv;
-        uint4 pf[MT][2];  // A fragments of the values' product, for the first and the last 16 keys
+        uint32_t pb[NT][4];  // B fragments of the values' product, by blocks of eight keys
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t pw[4][2];
+        for (int rt = 0; rt < RT; ++rt) {
+          float y[4][2];  // [keys 8 t + g][rows 2c, 2c + 1]
 #pragma unroll
-          for (int h = 0; h < RH; ++h) {
-            const int n = RH * mt + h;
-            float y[4][2];
-            const float f0 = factor[n] * ks0, f1 = factor[n] * ks1;
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              float v = x[rt * TERMS][t >> 1][2 * (t & 1) + z];
+              if (TERMS == 2) v = fmaf(x[rt * TERMS + TERMS - 1][t >> 1][2 * (t & 1) + z], 1.0f / 2048.0f, v);
+              y[t][z] = v * (factor[rt][z] * (t < 2 ? ks0 : ks1));
+            }
+          if (s.cap_l2 > 0.0f) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) y[t][z] = x[mt][t][2 * h + z] * (t < 2 ? f0 : f1);
-            if (s.cap_l2 > 0.0f) {
+              for (int z = 0; z < 2; ++z) y[t][z] = softcap_log2(y[t][z], s.two_over_cap, s.cap_l2);
+          }
+          if (masked) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) y[t][z] = kb + 8 * t + g < rows_limit[rt][z] ? y[t][z] : -INFINITY;
+          }
+          if (s.scores) {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int r = p.rg * R + rt * 8 + 2 * c + z;  // (single tokens: a row is a query head of the group)
+              float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.c.cap + kb + g;
 #pragma unroll
               for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int z = 0; z < 2; ++z) y[t][z] = softcap_log2(y[t][z], s.two_over_cap, s.cap_l2);
+                if (r < s.G && kb + 8 * t + g < p.limit) to[8 * t] = y[t][z];
             }
-            if (masked) {
-              const int see = rows_limit[n] - kb - 2 * c;
+          }
+          float top[2];
 #pragma unroll
-              for (int t = 0; t < 4; ++t)
+          for (int z = 0; z < 2; ++z) top[z] = fmaxf(fmaxf(y[0][z], y[1][z]), fmaxf(y[2][z], y[3][z]));
+          if (__any_sync(0xffffffffu, top[0] > m[rt][0] || top[1] > m[rt][1])) {  // (rare once a sequence is under way)
 #pragma unroll
-                for (int z = 0; z < 2; ++z) y[t][z] = 8 * t + z < see ? y[t][z] : -INFINITY;
-            }
-            if (s.scores) {
-              const int r = p.rg * R + mt * 16 + 8 * h + g;  // (single tokens: a row is a query head of the group)
-              if (r < s.G) {
-                float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.c.cap + kb + 2 * c;
+            for (int z = 0; z < 2; ++z) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
+              for (int o = 4; o < 32; o <<= 1) top[z] = fmaxf(top[z], __shfl_xor_sync(0xffffffffu, top[z], o));
+              const float m_new = fmaxf(m[rt][z], top[z]), alpha = ex2(m[rt][z] - (m_new == -INFINITY ? 0.0f : m_new));
+              m[rt][z] = m_new;
+              l[rt][z] *= alpha;
 #pragma unroll
-                  for (int z = 0; z < 2; ++z)
-                    if (!masked || kb + 8 * t + 2 * c + z < p.limit) to[8 * t + z] = y[t][z];
-              }
-            }
-            float top = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1])), fmaxf(fmaxf(y[2][0], y[2][1]), fmaxf(y[3][0], y[3][1])));
-            if (__any_sync(0xffffffffu, top > m[n])) {  // (rare once a sequence is under way)
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-              const float m_new = fmaxf(m[n], top), alpha = ex2(m[n] - (m_new == -INFINITY ? 0.0f : m_new));
-              m[n] = m_new;
-              l[n] *= alpha;
+              for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-              for (int d = 0; d < 16; ++d) {
-                acc[mt][d][2 * h] *= alpha;
-                acc[mt][d][2 * h + 1] *= alpha;
-                if (V::kTerms) {
-                  acc[mt][d][2] *= alpha;
-                  acc[mt][d][3] *= alpha;
+                for (int j = 0; j < 8; ++j) {
+                  acc[rt * TERMS + t][j][z] *= alpha;
+                  acc[rt * TERMS + t][j][2 + z] *= alpha;
                 }
-              }
             }
-            const float from = m[n] == -INFINITY ? 0.0f : m[n];
-            float sum = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                y[t][z] = ex2(y[t][z] - from);
-                sum += y[t][z];
-                y[t][z] *= t < 2 ? r0 : r1;
-              }
-              pw[t][h] = pack_f16x2(y[t][0], y[t][1]);
-              if (V::kTerms) pw[t][1] = rest_f16x2(pw[t][0], y[t][0], y[t][1]);
-            }
-            l[n] += sum;
           }
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk)
-            pf[mt][kk] = make_uint4(pw[2 * kk][0], HV > 1 ? pw[2 * kk][1] : 0u, pw[2 * kk + 1][0], HV > 1 ? pw[2 * kk + 1][1] : 0u);
+          for (int z = 0; z < 2; ++z) {
+            const float from = m[rt][z] == -INFINITY ? 0.0f : m[rt][z];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              y[t][z] = ex2(y[t][z] - from);
+              l[rt][z] += y[t][z];
+              y[t][z] *= t < 2 ? r0 : r1;
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t two = pack_f16x2(y[t][0], y[t][1]);
+            pb[rt * TERMS][t] = transposed(two);
+            if (TERMS == 2) pb[rt * TERMS + TERMS - 1][t] = transposed(rest_f16x2(two, y[t][0], y[t][1]));
+          }
         }
-        // ---- values: lane (g, c) reads the dimensions 16 g .. 16 g + 15 of the keys whose probabilities it holds; pairs of keys by bytes, then
-        // widened, they are the B fragments of 16 blocks of eight dimensions {16 g + n} ----
+        // ---- values: lane (g, c) reads the dimensions 16 g .. 16 g + 15 of the keys 2c, 2c + 1 of the four blocks; pairs of keys by bytes, then
+        // widened, they are the A fragments of eight tiles: dimension 16 g + 2j is row g of tile j, 16 g + 2j + 1 its row g + 8 ----
         uint4 vw[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -538,21 +533,21 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
-            uint32_t w[4], b[2][4];
+            uint32_t w[4], a[2][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint4& v = vw[4 * kk + i];
               w[i] = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
             }
+            widen(__byte_perm(w[0], w[1], 0x5140), a[0][0], a[0][1]);
+            widen(__byte_perm(w[2], w[3], 0x5140), a[0][2], a[0][3]);
+            widen(__byte_perm(w[0], w[1], 0x7362), a[1][0], a[1][1]);
+            widen(__byte_perm(w[2], w[3], 0x7362), a[1][2], a[1][3]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x5140), b[i][0], b[i][1]);
-              widen(__byte_perm(w[2 * i], w[2 * i + 1], 0x7362), b[i][2], b[i][3]);
-            }
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int n = 0; n < 4; ++n) mma_f16_16816(acc[mt][4 * k + n], pf[mt][kk], b[0][n], b[1][n]);
+              for (int j = 0; j < 2; ++j)
+                mma_f16_16816(acc[nt][2 * k + j], a[j][0], a[j][1], a[j][2], a[j][3], pb[nt][2 * kk], pb[nt][2 * kk + 1]);
           }
       }
       __syncwarp();
@@ -561,49 +556,44 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
     // ---- the rows' results, or this warp's part of them ----
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int h = 0; h < RH; ++h) {
-        const int n = RH * mt + h, r_in = mt * 16 + 8 * h + g;
-        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
-        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+      for (int z = 0; z < 2; ++z) {
+        float ll = l[rt][z];
+        const float mm = m[rt][z];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+        const int r_in = rt * 8 + 2 * c + z;
         const long long r = static_cast<long long>(p.rg) * R + r_in;
         const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
         if (i >= p.sq.len) continue;
-        float o[2][16];
+        float o[16];
         const float unit = vref * (1.0f / 16384.0f);
 #pragma unroll
-        for (int d = 0; d < 16; ++d)
-#pragma unroll
-          for (int z = 0; z < 2; ++z)
-            o[z][d] = (V::kTerms ? fmaf(acc[mt][d][2 + z], 1.0f / 2048.0f, acc[mt][d][z]) : acc[mt][d][2 * h + z]) * unit;
+        for (int d = 0; d < 16; ++d) {
+          o[d] = acc[rt * TERMS][d >> 1][2 * (d & 1) + z];
+          if (TERMS == 2) o[d] = fmaf(acc[rt * TERMS + TERMS - 1][d >> 1][2 * (d & 1) + z], 1.0f / 2048.0f, o[d]);
+          o[d] *= unit;
+        }
         if (p.sq.len > 1) {
 #pragma unroll
-          for (int z = 0; z < 2; ++z)
-#pragma unroll
-            for (int d = 0; d < 16; ++d)
-              if (rows_limit[n] > sm_nan[32 * c + 16 * z + d]) o[z][d] = __uint_as_float(0x7fffffffu);
+          for (int d = 0; d < 16; ++d)
+            if (rows_limit[rt][z] > sm_nan[16 * g + d]) o[d] = __uint_as_float(0x7fffffffu);
         }
         if (!p.whole) {
           const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + r_in;
-          if (c == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(m[n], l[n]);
-#pragma unroll
-          for (int z = 0; z < 2; ++z) store16(s.part_o + slot * 128 + 32 * c + 16 * z, o[z], true);
+          if (g == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(mm, ll);
+          store16(s.part_o + slot * 128 + 16 * g, o, true);
           continue;
         }
         const size_t row = static_cast<size_t>(p.sq.row0) + i;
-        if (s.a.sink) l[n] += ex2(fmaf(s.a.sink[hq], kLog2e, -m[n]));
-        if (c == 0) note_lse(s, row, hq, m[n] + log2f(l[n]));
-        const float inv = 1.0f / l[n];
-        T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V;
+        if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
+        if (g == 0) note_lse(s, row, hq, mm + log2f(ll));
+        if (16 * g >= s.c.V) continue;
+        const float inv = 1.0f / ll;
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int d0 = 32 * c + 16 * z;
-          if (d0 >= s.c.V) continue;
-#pragma unroll
-          for (int d = 0; d < 16; ++d) o[z][d] = finished<T>(s, row, hq, d0 + d, o[z][d], inv);
-          store16(out + d0, o[z], s.vec_o);
-        }
+        for (int d = 0; d < 16; ++d) o[d] = finished<T>(s, row, hq, 16 * g + d, o[d], inv);
+        store16(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 16 * g, o, s.vec_o);
       }
     if (rest == 0) return;
     next_piece(s, p, R, rest);
@@ -611,21 +601,27 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   }
 }
 
-// Adds the parts of the units that lie in several warps' shares: one CTA for a unit, a warp for a row (mod 8), a lane for four dimensions.
+// Adds the parts of a row whose unit lies in several warps' shares: one CTA for a row, warp w takes the parts w, w + 8, .., a lane four dimensions.
+// (One warp for a row, part after part, was a chain of loads: 31 us for 20 rows of 128 units in ten parts.)
 template <typename T>
-__global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_constant__ Shared s, int rows, int max_groups) {
+__global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_constant__ Shared s, int rows, int max_groups, int max_rows) {
   __shared__ long long sums[8][2];
+  __shared__ float sm_ml[8][2];
+  __shared__ float4 sm_o[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int e = blockIdx.x / (s.c.H * max_groups), unit = blockIdx.x % (s.c.H * max_groups), hk = unit / max_groups, rg = unit % max_groups;
+  const int r_in = blockIdx.x % max_rows, u = blockIdx.x / max_rows, e = u / (s.c.H * max_groups), unit = u % (s.c.H * max_groups),
+            hk = unit / max_groups, rg = unit % max_groups;
   pdl_wait();
   const SeqDesc sq = s.seqs[e];
   const EntryShape es = entry_shape(s, sq, rows);
-  if (rg >= es.groups) return;
+  const long long r = static_cast<long long>(rg) * rows + r_in;
+  const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+  if (es.all == 0 || i >= sq.len) return;
   long long before = 0, total = 0;
-  for (int i = threadIdx.x; i < s.n_seqs; i += 256) {
-    const long long t = entry_shape(s, s.seqs[i], rows).all;
+  for (int k = threadIdx.x; k < s.n_seqs; k += 256) {
+    const long long t = entry_shape(s, s.seqs[k], rows).all;
     total += t;
-    if (i < e) before += t;
+    if (k < e) before += t;
   }
   before = warp_sum_ll(before);
   total = warp_sum_ll(total);
@@ -640,34 +636,51 @@ __global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_consta
   const int c0 = static_cast<int>(((u0 + 1) * parts - 1) / total), c1 = static_cast<int>((u1 * parts - 1) / total);
   if (c0 == c1) return;
   const int slot0 = 2 * c0 + (share_begin(total, c0, parts) == u0 ? 0 : 1);
-  for (int r8 = warp; r8 < rows; r8 += 8) {
-    const long long r = static_cast<long long>(rg) * rows + r8;
-    const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-    if (i >= sq.len) break;
-    auto place = [&](int part) { return static_cast<size_t>(part == c0 ? slot0 : 2 * part) * rows + r8; };
-    float mm = -INFINITY, ll = 0.0f;
-    for (int p = c0 + lane; p <= c1; p += 32) mm = fmaxf(mm, s.part_ml[place(p) * 2]);
-    mm = warp_max(mm);
-    const float to = mm == -INFINITY ? 0.0f : mm;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p = c0; p <= c1; ++p) {
-      const float pm = s.part_ml[place(p) * 2];
-      if (pm == -INFINITY && s.part_ml[place(p) * 2 + 1] == 0.0f) continue;  // no key of this row: nothing was written but that
-      const float f = ex2(pm - to);
-      const float4 x = *reinterpret_cast<const float4*>(s.part_o + place(p) * 128 + 4 * lane);
-      ll = fmaf(s.part_ml[place(p) * 2 + 1], f, ll);
-      o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
-    }
-    const size_t row = static_cast<size_t>(sq.row0) + i;
-    if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
-    if (lane == 0) note_lse(s, row, hq, mm + log2f(ll));
-    const float inv = 1.0f / ll;
-    T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 4 * lane;
-    if (4 * lane >= s.c.V) continue;
-    const float y[4] = {o.x, o.y, o.z, o.w};
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int p0 = c0 + warp; p0 <= c1; p0 += 32) {  // four parts at a time
+    float2 ml[4];
+    float4 x[4];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) store_one(out + d, finished<T>(s, row, hq, 4 * lane + d, y[d], inv));
+    for (int k = 0; k < 4; ++k) {
+      const int p = p0 + 8 * k;
+      ml[k] = make_float2(-INFINITY, 0.0f);
+      x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p > c1) continue;
+      const size_t slot = static_cast<size_t>(p == c0 ? slot0 : 2 * p) * rows + r_in;
+      ml[k] = *reinterpret_cast<const float2*>(s.part_ml + slot * 2);
+      x[k] = *reinterpret_cast<const float4*>(s.part_o + slot * 128 + 4 * lane);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float top = fmaxf(m, ml[k].x), to = top == -INFINITY ? 0.0f : top, a = ex2(m - to), f = ex2(ml[k].x - to);
+      m = top;
+      l = fmaf(ml[k].y, f, l * a);
+      o.x = fmaf(x[k].x, f, o.x * a); o.y = fmaf(x[k].y, f, o.y * a); o.z = fmaf(x[k].z, f, o.z * a); o.w = fmaf(x[k].w, f, o.w * a);
+    }
   }
+  if (lane == 0) { sm_ml[warp][0] = m; sm_ml[warp][1] = l; }
+  sm_o[warp][lane] = o;
+  __syncthreads();
+  if (threadIdx.x >= 128) return;
+  const int d = threadIdx.x;
+  m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, sm_ml[w][0]);
+  const float to = m == -INFINITY ? 0.0f : m;
+  float y = 0.0f;
+  l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float f = ex2(sm_ml[w][0] - to);
+    l = fmaf(sm_ml[w][1], f, l);
+    y = fmaf(reinterpret_cast<const float*>(&sm_o[w][0])[d], f, y);
+  }
+  const size_t row = static_cast<size_t>(sq.row0) + i;
+  if (s.a.sink) l += ex2(fmaf(s.a.sink[hq], kLog2e, -m));
+  if (d == 0) note_lse(s, row, hq, m + log2f(l));
+  if (d < s.c.V)
+    store_one(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + d, finished<T>(s, row, hq, d, y, 1.0f / l));
 }
 
 // Weights of single tokens' calls, from the scores that the attention kernel left: blockIdx = (share of the keys, kv head, entry).
@@ -687,11 +700,10 @@ __global__ void __launch_bounds__(256) cache8_weights_kernel(const __grid_consta
 }
 
 // Weights of calls with several tokens: the scores once more, from the rows' lse.  A warp takes 32 keys of a (kv head, entry) and goes through the
-// rows, 16 at a time (f32: eight, in two terms).
+// rows, eight at a time.
 template <typename T>
 __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_constant__ Shared s) {
-  constexpr bool kTerms = sizeof(T) == 4;
-  constexpr int RH = kTerms ? 1 : 2, R = 8 * RH;
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   pdl_wait();
   const int e = blockIdx.z, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const SeqDesc sq = s.seqs[e];
@@ -699,71 +711,72 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
   const int live = sq.pos + sq.len;
   const size_t head = static_cast<size_t>(sq.slot) * s.c.H + hk;
   for (int kb = (blockIdx.x * 4 + warp) * 32; kb < live; kb += gridDim.x * 128) {
-    uint4 kw[4][2];
+    uint32_t ka[2][8][4];  // the keys' A fragments
     float ks[2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int key = kb + 8 * t + g;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int d0 = 16 * (2 * c + h);
-        kw[t][h] = key < live && d0 < s.c.D ? *reinterpret_cast<const uint4*>(s.c.k + (head * s.c.cap + key) * s.c.D + d0) : make_uint4(0u, 0u, 0u, 0u);
+      for (int half = 0; half < 2; ++half) {
+        const int key = kb + 16 * u + 8 * half + g;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d0 = 16 * (2 * c + h);
+          const uint4 w = key < live && d0 < s.c.D ? *reinterpret_cast<const uint4*>(s.c.k + (head * s.c.cap + key) * s.c.D + d0) : make_uint4(0u, 0u, 0u, 0u);
+          widen(w.x, ka[u][4 * h][half], ka[u][4 * h][2 + half]);
+          widen(w.y, ka[u][4 * h + 1][half], ka[u][4 * h + 1][2 + half]);
+          widen(w.z, ka[u][4 * h + 2][half], ka[u][4 * h + 2][2 + half]);
+          widen(w.w, ka[u][4 * h + 3][half], ka[u][4 * h + 3][2 + half]);
+        }
       }
-    }
     ks[0] = s.c.ks[head * s.c.blocks + kb / s.c.B];
     ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + (kb + 16) / s.c.B] : 0.0f;
-    float sum[4][2] = {};
+    float sum[4] = {};
     const long long rows = static_cast<long long>(sq.len) * s.G;
-    for (long long r0 = static_cast<long long>(max(0, kb - sq.pos)) * s.G / R * R; r0 < rows; r0 += R) {
-      uint32_t term[2][16];
-      float f[RH], z[RH];
-      int sees[RH];
+    for (long long r0 = static_cast<long long>(max(0, kb - sq.pos)) * s.G / 8 * 8; r0 < rows; r0 += 8) {
+      const long long r = r0 + g, at = min(r, rows - 1);
+      const int i = static_cast<int>(at / s.G), hq = hk * s.G + static_cast<int>(at - static_cast<long long>(i) * s.G);
+      const size_t row = static_cast<size_t>(sq.row0) + i;
+      uint32_t term[TERMS][16];
+      const float f = split_row<T, TERMS>(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c,
+                                          s.scale_log2, term);
+      const float lse = s.lse2[row * s.a.Hq + hq];
+      const int see = r < rows ? sq.pos + i + 1 - kb : 0;
+      float factor[2], z2[2];
+      int sees[2];
 #pragma unroll
-      for (int h = 0; h < RH; ++h) {
-        const long long r = r0 + 8 * h + g, at = min(r, rows - 1);
-        const int i = static_cast<int>(at / s.G), hq = hk * s.G + static_cast<int>(at - static_cast<long long>(i) * s.G);
-        const size_t row = static_cast<size_t>(sq.row0) + i;
-        const T* q = static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
-        if constexpr (kTerms) f[h] = split_row<T, 2>(q, s.c.D, r < rows, s.vec_q, c, s.scale_log2, term);
-        else {
-          uint32_t one[1][16];
-          f[h] = split_row<T, 1>(q, s.c.D, r < rows, s.vec_q, c, s.scale_log2, one);
-#pragma unroll
-          for (int w = 0; w < 16; ++w) term[h][w] = one[0][w];
-        }
-        z[h] = s.lse2[row * s.a.Hq + hq];
-        sees[h] = r < rows ? sq.pos + i + 1 - kb - 2 * c : -64;
+      for (int z = 0; z < 2; ++z) {
+        factor[z] = __shfl_sync(0xffffffffu, f, (2 * c + z) * 4);
+        z2[z] = __shfl_sync(0xffffffffu, lse, (2 * c + z) * 4);
+        sees[z] = __shfl_sync(0xffffffffu, see, (2 * c + z) * 4);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < 2; ++u) {
+        float d[TERMS][4] = {};
 #pragma unroll
-        for (int step = 0; step < 8; ++step) {
-          const uint4& k = kw[t][step >> 2];
-          uint32_t b0, b1;
-          widen((step & 3) == 0 ? k.x : (step & 3) == 1 ? k.y : (step & 3) == 2 ? k.z : k.w, b0, b1);
-          mma_f16_16816(d, make_uint4(term[0][2 * step], term[1][2 * step], term[0][2 * step + 1], term[1][2 * step + 1]), b0, b1);
-        }
+        for (int step = 0; step < 8; ++step)
 #pragma unroll
-        for (int h = 0; h < RH; ++h)
+          for (int t = 0; t < TERMS; ++t)
+            mma_f16_16816(d[t], ka[u][step][0], ka[u][step][1], ka[u][step][2], ka[u][step][3], term[t][2 * step], term[t][2 * step + 1]);
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            float v = (kTerms ? fmaf(d[2 + y], 1.0f / 2048.0f, d[y]) : d[2 * h + y]) * (f[h] * ks[t >> 1]);
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            float v = d[0][2 * half + z];
+            if (TERMS == 2) v = fmaf(d[TERMS - 1][2 * half + z], 1.0f / 2048.0f, v);
+            v *= factor[z] * ks[u];
             if (s.cap_l2 > 0.0f) v = softcap_log2(v, s.two_over_cap, s.cap_l2);
-            if (8 * t + y < sees[h]) sum[t][y] += ex2(v - z[h]);
+            if (16 * u + 8 * half + g < sees[z]) sum[2 * u + half] += ex2(v - z2[z]);
           }
       }
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum[t][y] += __shfl_xor_sync(0xffffffffu, sum[t][y], o);
-        const int key = kb + 8 * t + 2 * c + y;
-        float* w = s.c.w + head * s.c.cap + key;
-        if (g == 0 && key < live) *w = s.a.decay == 0.0f ? sum[t][y] : fmaf(s.a.decay, *w, sum[t][y]);
-      }
+    for (int t = 0; t < 4; ++t) {
+      sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 1);
+      sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 2);
+      const int key = kb + 8 * t + g;
+      float* w = s.c.w + head * s.c.cap + key;
+      if (c == 0 && key < live) *w = s.a.decay == 0.0f ? sum[t] : fmaf(s.a.decay, *w, sum[t]);
+    }
   }
 }
 
@@ -773,17 +786,20 @@ struct Plan {
   size_t part_o, part_ml, lse2, scores, bytes;
 };
 template <typename F>
-void for_variant(int kind, F&& f) {
-  if (kind == kEight) f(cache8_attention_kernel<kEight>, Variant<kEight>{});
-  else if (kind == kSixteen) f(cache8_attention_kernel<kSixteen>, Variant<kSixteen>{});
-  else if (kind == kPair) f(cache8_attention_kernel<kPair>, Variant<kPair>{});
-  else f(cache8_attention_kernel<kF32>, Variant<kF32>{});
+void for_variant(int kind, F&& f) {  // rows in tiles of eight, or 0 for f32
+  if (kind == 0) f(Variant<1, 2>{});
+  else if (kind == 1) f(Variant<1, 1>{});
+  else if (kind == 2) f(Variant<2, 1>{});
+  else if (kind == 3) f(Variant<3, 1>{});
+  else f(Variant<4, 1>{});
 }
 Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights) {
   Plan p{};
   const long long unit = static_cast<long long>(Hq / c.H) * max_len;  // rows of the longest entry and a kv head
-  p.kind = f32 ? kF32 : unit <= 8 ? kEight : unit <= 16 ? kSixteen : kPair;
-  for_variant(p.kind, [&](auto, auto v) {
+  // as few passes over the keys as there can be, and no more row tiles than they need
+  const long long passes = (unit + 31) / 32;
+  p.kind = f32 ? 0 : static_cast<int>((unit + 8 * passes - 1) / (8 * passes));
+  for_variant(p.kind, [&](auto v) {
     using V = decltype(v);
     p.rows = V::kRows;
     p.parts = sm_count() * V::kCtas * kWarps;  // the warps that are resident at once
@@ -802,9 +818,10 @@ int prepare() {
   cudaGetDevice(&dev);
   if (dev < 64 && (done.load(std::memory_order_acquire) >> dev) & 1ull) return 0;
   cudaError_t e = cudaSuccess;
-  for (int kind : {kEight, kSixteen, kPair, kF32})
-    for_variant(kind, [&](auto kernel, auto v) {
-      const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(v)::kBytes);
+  for (int kind = 0; kind <= 4; ++kind)
+    for_variant(kind, [&](auto v) {
+      using V = decltype(v);
+      const cudaError_t rc = cudaFuncSetAttribute(cache8_attention_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, V::kBytes);
       if (e == cudaSuccess) e = rc;
     });
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -858,14 +875,16 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   s.vec_o = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) & 15) == 0;
   s.err = device_error_word();
   if (!s.err) return TEENY_ERR_DRIVER;
-  for_variant(p.kind, [&](auto kernel, auto v) {
+  for_variant(p.kind, [&](auto v) {
     using V = decltype(v);
-    launch_kernel(kernel, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
+    launch_kernel(cache8_attention_kernel<V>, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
   });
   const PdlScope behind;
-  const dim3 units(static_cast<unsigned>(n_seqs) * c.H * p.groups);
-  if (a.f32) launch_kernel(cache8_combine_kernel<float>, units, dim3(256), 0, st, 1, s, p.rows, p.groups);
-  else launch_kernel(cache8_combine_kernel<bf16>, units, dim3(256), 0, st, 1, s, p.rows, p.groups);
+  const long long unit_rows = static_cast<long long>(s.G) * max_len;
+  const int max_rows = static_cast<int>(unit_rows < p.rows ? unit_rows : p.rows);
+  const dim3 rows(static_cast<unsigned>(n_seqs) * c.H * p.groups * max_rows);
+  if (a.f32) launch_kernel(cache8_combine_kernel<float>, rows, dim3(256), 0, st, 1, s, p.rows, p.groups, max_rows);
+  else launch_kernel(cache8_combine_kernel<bf16>, rows, dim3(256), 0, st, 1, s, p.rows, p.groups, max_rows);
   if (a.weights) {
     const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
