@@ -18,7 +18,7 @@
  * f32: element type of k, v, q, out and gate (0 bf16, 1 f32).  Row strides are in elements, heads lie side by side within a row.
  * dim and vdim are multiples of 16 up to 128, block is 16, 32, 64 or 128, the caches' bases are 16-byte aligned.
  * All pointers are device pointers owned by the caller unless stated; nothing here allocates device memory, and scratch holds
- * nothing from one call to the next.  Status codes are those of teeny_b200.h.
+ * no results from one call to the next.  Status codes are those of teeny_b200.h.
  */
 #ifndef TEENY_CACHE8_H_
 #define TEENY_CACHE8_H_
@@ -46,9 +46,11 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
  * null: logarithm of the denominator, the sink's part included.  weights (or null): for every live token of the entries' slots
  * weights <- weight_decay * weights + the probabilities that the entry's tokens and query heads gave it; with weight_decay 0 what
  * was there is not read.  The gate does not count there.  Rows of out that belong to no entry stay as they are.  Sums are made in
- * a fixed order: the same call gives the same bits. */
+ * a fixed order: the same call gives the same bits.
+ * scratch: its first teeny_cache8_attention_zeroed_bytes bytes (counters) are zero before the first call, and every call leaves them zero. */
 size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int f32, int heads, int rows, int n_seqs, int max_len,
                                             int with_weights);
+size_t teeny_cache8_attention_zeroed_bytes(const teeny_cache8_shape* shape, int f32, int heads, int n_seqs, int max_len);
 int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void* k, const void* v, const float* k_scale,
                            const float* v_scale, float* weights, float weight_decay, const void* q, long long ldq, void* out,
                            long long ldo, int rows, int heads, float score_scale, float softcap, const float* sink, const void* gate,

@@ -354,6 +354,12 @@ size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int
   return cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, with_weights != 0);
 }
 
+size_t teeny_cache8_attention_zeroed_bytes(const teeny_cache8_shape* shape, int f32, int heads, int n_seqs, int max_len) {
+  Cache8 c;
+  if (!cache_of(shape, &c) || heads <= 0 || heads % c.H || !step_sizes(1, n_seqs, max_len)) return 0;
+  return cache8_attention_zeroed_bytes(c, f32 != 0, heads, n_seqs, max_len);
+}
+
 int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void* k, const void* v, const float* k_scale,
                            const float* v_scale, float* weights, float weight_decay, const void* q, long long ldq, void* out,
                            long long ldo, int rows, int heads, float score_scale, float softcap, const float* sink, const void* gate,

@@ -12,8 +12,8 @@
 // The call is bound by reading the cache.  Every warp works alone: it takes slices of 32 keys of one sequence and head, and keeps the next ones in
 // flight itself (keys and values by TMA, their scales by 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry
 // after entry, head after head, row group after row group, each warp takes the same number of consecutive slices of all of them, whatever
-// the lengths.  A sequence that lies in several warps' shares leaves partial results in scratch, at most two for each warp, which a
-// second kernel adds.  No warp waits for another.
+// the lengths.  A sequence that lies in several warps' shares leaves partial results in scratch, at most two for each warp; the last CTA to have
+// stored its part of a sequence adds them (a second kernel for it cost 4 to 10 us a call).  No warp waits for another CTA's.
 #include <atomic>
 #include <type_traits>
 
@@ -97,6 +97,8 @@ struct Shared {  // what a call's kernels share
   float scale_log2, two_over_cap, cap_l2;
   float* part_o;   // [2 * warps][rows of a unit][128]
   float* part_ml;  // [2 * warps][rows of a unit][2]
+  unsigned* arrivals;  // [entries][kv heads][max_groups]: CTAs that have stored their parts, zero between calls
+  int max_groups;
   float* lse2;     // [rows][Hq], base 2, or null
   float* scores;   // [entries][Hq][cap] base 2, or null
   int parts;       // warps of the main kernel
@@ -104,28 +106,35 @@ struct Shared {  // what a call's kernels share
   int* err;
 };
 
-// Slices of an entry: its units are (head, row group), each over all its slices.
-struct EntryShape { int slices, groups; long long all; };
+// Slices of an entry: its units are (head, row group), each over all its slices.  (All counts of a call fit 31 bits, the host sees to that: divisions
+// of 64-bit numbers, a hundred instructions each, made up most of a short call.)
+struct EntryShape { int slices, groups, all; };
 __device__ __forceinline__ EntryShape entry_shape(const Shared& s, const SeqDesc& sq, int rows) {
   EntryShape e{0, 0, 0};
   if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return e;
   e.slices = (sq.pos + sq.len + kSlice - 1) / kSlice;
-  e.groups = static_cast<int>((static_cast<long long>(sq.len) * s.G + rows - 1) / rows);
-  e.all = static_cast<long long>(e.slices) * e.groups * s.c.H;
+  e.groups = (sq.len * s.G + rows - 1) / rows;
+  e.all = e.slices * e.groups * s.c.H;
   return e;
 }
-// Where warp w's share begins; no share takes less than kLeast slices, and none between two others is empty.
-constexpr int kLeast = 2;
-__device__ __forceinline__ int shares(const Shared& s, long long total) {
-  return static_cast<int>(min(static_cast<long long>(s.parts), (total + kLeast - 1) / kLeast));
-}
-__device__ __forceinline__ long long share_begin(long long total, int part, int parts) { return total * part / parts; }
+// How the slices are shared: none of `parts` warps takes less than two, nor are there many more than 256 to a unit, whose parts have to be added
+// again.  The first `more` warps take one slice more than the others' `each`.
+struct Shares {
+  int parts, each, more;
+  __device__ __forceinline__ Shares(int most, int total, int units) {
+    const int least = max(2, total / 256 / units), all = (total + least - 1) / least;
+    parts = min(most, all);
+    each = total / parts;
+    more = total - parts * each;
+  }
+  __device__ __forceinline__ int begin(int part) const { return part * each + min(part, more); }
+  __device__ __forceinline__ int owner(int slice) const {
+    const int big = more * (each + 1);
+    return slice < big ? slice / (each + 1) : more + (slice - big) / each;
+  }
+};
 
-__device__ __forceinline__ long long warp_sum_ll(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+__device__ __forceinline__ int warp_sum_int(int v) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(v))); }
 
 // Output element of query head h in row `row`: o unnormalised, l the row sum (with the sink's part).
 template <typename T>
@@ -215,16 +224,14 @@ struct Piece {
   int e, slices, groups, hk, rg, j, end, limit;  // slices j .. end - 1; limit: keys that the group's last row sees
   bool whole, first;
 };
-__device__ __forceinline__ void piece_range(const Shared& s, Piece& p, int rows, int j0, long long left) {
+__device__ __forceinline__ void piece_range(const Shared& s, Piece& p, int rows, int j0, int left) {
   p.j = j0;
-  const int stop = static_cast<int>(min(static_cast<long long>(p.slices), j0 + left));
-  p.whole = j0 == 0 && stop == p.slices;
-  const int last = static_cast<int>(min(static_cast<long long>(p.sq.len) * s.G, (static_cast<long long>(p.rg) + 1) * rows) - 1) / s.G;
-  p.limit = p.sq.pos + last + 1;
-  p.end = stop;
+  p.end = min(p.slices, j0 + left);
+  p.whole = j0 == 0 && p.end == p.slices;
+  p.limit = p.sq.pos + (min(p.sq.len * s.G, (p.rg + 1) * rows) - 1) / s.G + 1;
 }
 // to the next unit, of which `left` slices may be taken
-__device__ __forceinline__ void next_piece(const Shared& s, Piece& p, int rows, long long left) {
+__device__ __forceinline__ void next_piece(const Shared& s, Piece& p, int rows, int left) {
   if (++p.rg == p.groups) {
     p.rg = 0;
     if (++p.hk == s.c.H) {
@@ -252,37 +259,46 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   const uint32_t offset = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw) + warp * V::kWarpBytes;
   const uint32_t base = smem_u32(smem_raw) + offset;
   uint8_t* gen = smem_raw + offset;
+  // parts that this CTA's warps have left: of their first and of their last unit (entry, head, row group, slices, first slice of all)
+  __shared__ struct Left { int begin, e, hk, rg, slices; } sm_left[2 * kWarps];
+  __shared__ int sm_c0[2 * kWarps], sm_c1[2 * kWarps];  // warps whose parts are to be added here (none: c1 < c0)
   if (lane == 0) {
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
     for (int st = 0; st < ST; ++st) mbar_init(base + V::kBars + 8 * st, 1 + 4);
     mbar_fence_init();
+    sm_left[2 * warp].slices = sm_left[2 * warp + 1].slices = 0;
   }
   __syncwarp();
   pdl_wait();
   // ---- this warp's share ----
   const int part = blockIdx.x * kWarps + warp;
   Piece load;
-  long long left;  // slices of the share that are still to be loaded
-  {
-    long long total = 0;
-    for (int e = lane; e < s.n_seqs; e += 32) total += entry_shape(s, s.seqs[e], R).all;
-    total = warp_sum_ll(total);
-    const int parts = shares(s, total);
-    if (part >= parts) return;
-    const long long t0 = share_begin(total, part, parts);
-    left = share_begin(total, part + 1, parts) - t0;
-    long long before = 0, at = 0;
-    int found = -1;
+  int left = 0;  // slices of the share that are still to be loaded
+  int total = 0, units = 0, unit_begin = 0;
+  for (int e = lane; e < s.n_seqs; e += 32) {
+    const EntryShape es = entry_shape(s, s.seqs[e], R);
+    total += es.all;
+    units += es.groups * s.c.H;
+  }
+  total = warp_sum_int(total);
+  units = warp_sum_int(units);
+  if (total == 0) return;
+  const Shares shares(s.parts, total, units);
+  if (static_cast<int>(blockIdx.x) * kWarps >= shares.parts) return;
+  if (part < shares.parts) {
+    const int t0 = shares.begin(part);
+    left = shares.begin(part + 1) - t0;
+    int before = 0, at = 0, found = -1;
     for (int e0 = 0; found < 0; e0 += 32) {
-      const long long mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
-      long long run = mine;
+      const int mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
+      int run = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, run, o);
+        const int up = __shfl_up_sync(0xffffffffu, run, o);
         if (lane >= o) run += up;
       }
-      const long long end = before + run;
+      const int end = before + run;
       const unsigned who = __ballot_sync(0xffffffffu, mine > 0 && t0 >= end - mine && t0 < end);
       before = __shfl_sync(0xffffffffu, end, 31);
       if (!who) continue;
@@ -295,15 +311,16 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     const EntryShape es = entry_shape(s, load.sq, R);
     load.slices = es.slices;
     load.groups = es.groups;
-    const long long unit = at / es.slices;
-    load.hk = static_cast<int>(unit / es.groups);
-    load.rg = static_cast<int>(unit - static_cast<long long>(load.hk) * es.groups);
+    const int unit = at / es.slices;
+    load.hk = unit / es.groups;
+    load.rg = unit - load.hk * es.groups;
     load.first = true;
-    piece_range(s, load, R, static_cast<int>(at - unit * es.slices), left);
+    piece_range(s, load, R, at - unit * es.slices, left);
+    unit_begin = t0 - load.j;
   }
   pdl_trigger();
   Piece p = load;
-  long long rest = left;  // slices of the share that are still to be computed
+  int rest = left;  // slices of the share that are still to be computed
   int issued = 0, count = 0;
   auto load_next = [&]() {
     if (left == 0) return;
@@ -330,15 +347,15 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   for (int st = 0; st < ST; ++st) load_next();
 
   int* sm_nan = reinterpret_cast<int*>(gen + V::kNan);
-  for (;;) {
+  bool ok = true;
+  while (rest > 0) {
     // ---- queries as B fragments: row g of tile rt is column g ----
     float factor[RT][2];      // of the rows 2c, 2c + 1, whose scores this lane gets
     int rows_limit[RT][2];    // keys that they see
     uint2 q_regs[V::kQRegs ? NT * 8 : 1];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const long long r = static_cast<long long>(p.rg) * R + rt * 8 + g;
-      const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+      const int r = p.rg * R + rt * 8 + g, i = r / s.G, hq = p.hk * s.G + r - i * s.G;
       const bool valid = i < p.sq.len;
       const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
       uint32_t term[TERMS][16];
@@ -382,7 +399,8 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       if (!mbar_wait(base + V::kBars + 8 * st, count / ST & 1, s.err, DEVERR_ATTN_SOFTMAX)) {
         // (nothing that this warp asked for may arrive after it has gone: the barriers are waited for once more, within their limit)
         for (int i = count; i < issued; ++i) mbar_wait(base + V::kBars + 8 * (i & (ST - 1)), i / ST & 1, s.err, DEVERR_ATTN_SOFTMAX);
-        return;
+        ok = false;
+        break;
       }
       if (kb < p.limit) {
         const uint32_t kt = base + st * kStage + g * 128, vt = base + st * kStage + kBox, sc = base + V::kScales + st * 16;
@@ -554,7 +572,17 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       load_next();
     }
 
+    if (!ok) break;
+
     // ---- the rows' results, or this warp's part of them ----
+    if (!p.whole && lane == 0) {
+      Left& of = sm_left[2 * warp + (p.first ? 0 : 1)];
+      of.begin = unit_begin;
+      of.e = p.e;
+      of.hk = p.hk;
+      of.rg = p.rg;
+      of.slices = p.slices;
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -564,8 +592,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
         const int r_in = rt * 8 + 2 * c + z;
-        const long long r = static_cast<long long>(p.rg) * R + r_in;
-        const int i = static_cast<int>(r / s.G), hq = p.hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
+        const int r = p.rg * R + r_in, i = r / s.G, hq = p.hk * s.G + r - i * s.G;
         if (i >= p.sq.len) continue;
         float o[16];
         const float unit = vref * (1.0f / 16384.0f);
@@ -595,92 +622,93 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         for (int d = 0; d < 16; ++d) o[d] = finished<T>(s, row, hq, 16 * g + d, o[d], inv);
         store16(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 16 * g, o, s.vec_o);
       }
-    if (rest == 0) return;
+    if (rest == 0) break;
+    unit_begin += p.slices;
     next_piece(s, p, R, rest);
     __syncwarp();
   }
-}
+  (void)ok;  // (the error word is set: what the call leaves is not a result)
 
-// Adds the parts of a row whose unit lies in several warps' shares: one CTA for a row, warp w takes the parts w, w + 8, .., a lane four dimensions.
-// (One warp for a row, part after part, was a chain of loads: 31 us for 20 rows of 128 units in ten parts.)
-template <typename T>
-__global__ void __launch_bounds__(256) cache8_combine_kernel(const __grid_constant__ Shared s, int rows, int max_groups, int max_rows) {
-  __shared__ long long sums[8][2];
-  __shared__ float sm_ml[8][2];
-  __shared__ float4 sm_o[8][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r_in = blockIdx.x % max_rows, u = blockIdx.x / max_rows, e = u / (s.c.H * max_groups), unit = u % (s.c.H * max_groups),
-            hk = unit / max_groups, rg = unit % max_groups;
-  pdl_wait();
-  const SeqDesc sq = s.seqs[e];
-  const EntryShape es = entry_shape(s, sq, rows);
-  const long long r = static_cast<long long>(rg) * rows + r_in;
-  const int i = static_cast<int>(r / s.G), hq = hk * s.G + static_cast<int>(r - static_cast<long long>(i) * s.G);
-  if (es.all == 0 || i >= sq.len) return;
-  long long before = 0, total = 0;
-  for (int k = threadIdx.x; k < s.n_seqs; k += 256) {
-    const long long t = entry_shape(s, s.seqs[k], rows).all;
-    total += t;
-    if (k < e) before += t;
-  }
-  before = warp_sum_ll(before);
-  total = warp_sum_ll(total);
-  if (lane == 0) { sums[warp][0] = before; sums[warp][1] = total; }
+  // ---- units whose parts this CTA completes ----
   __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) { before += sums[w][0]; total += sums[w][1]; }
-  const int parts = shares(s, total);
-  const long long u0 = before + (static_cast<long long>(hk) * es.groups + rg) * es.slices, u1 = u0 + es.slices;
-  // the warp whose share holds a slice: the last one that begins at or before it
-  const int c0 = static_cast<int>(((u0 + 1) * parts - 1) / total), c1 = static_cast<int>((u1 * parts - 1) / total);
-  if (c0 == c1) return;
-  const int slot0 = 2 * c0 + (share_begin(total, c0, parts) == u0 ? 0 : 1);
-  float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int p0 = c0 + warp; p0 <= c1; p0 += 32) {  // four parts at a time
-    float2 ml[4];
-    float4 x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int p = p0 + 8 * k;
-      ml[k] = make_float2(-INFINITY, 0.0f);
-      x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (p > c1) continue;
-      const size_t slot = static_cast<size_t>(p == c0 ? slot0 : 2 * p) * rows + r_in;
-      ml[k] = *reinterpret_cast<const float2*>(s.part_ml + slot * 2);
-      x[k] = *reinterpret_cast<const float4*>(s.part_o + slot * 128 + 4 * lane);
+  if (threadIdx.x < 2 * kWarps) {
+    const Left u = sm_left[threadIdx.x];
+    bool mine = u.slices > 0;
+    for (int k = 0; k < static_cast<int>(threadIdx.x); ++k) mine = mine && !(sm_left[k].slices > 0 && sm_left[k].begin == u.begin);  // (said before)
+    int c0 = 0, c1 = -1;
+    if (mine) {
+      c0 = shares.owner(u.begin);
+      c1 = shares.owner(u.begin + u.slices - 1);
+      const int ctas = c1 / kWarps - c0 / kWarps + 1;
+      if (ctas > 1) {  // (the counter goes back to zero with the last arrival)
+        __threadfence();
+        mine = atomicInc(s.arrivals + (static_cast<size_t>(u.e) * s.c.H + u.hk) * s.max_groups + u.rg, ctas - 1) == static_cast<unsigned>(ctas - 1);
+        __threadfence();
+      }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float top = fmaxf(m, ml[k].x), to = top == -INFINITY ? 0.0f : top, a = ex2(m - to), f = ex2(ml[k].x - to);
-      m = top;
-      l = fmaf(ml[k].y, f, l * a);
-      o.x = fmaf(x[k].x, f, o.x * a); o.y = fmaf(x[k].y, f, o.y * a); o.z = fmaf(x[k].z, f, o.z * a); o.w = fmaf(x[k].w, f, o.w * a);
-    }
+    sm_c0[threadIdx.x] = c0;
+    sm_c1[threadIdx.x] = mine ? c1 : -1;
   }
-  if (lane == 0) { sm_ml[warp][0] = m; sm_ml[warp][1] = l; }
-  sm_o[warp][lane] = o;
   __syncthreads();
-  if (threadIdx.x >= 128) return;
-  const int d = threadIdx.x;
-  m = -INFINITY;
+  for (int k = 0; k < 2 * kWarps; ++k) {
+    const int c0 = sm_c0[k], c1 = sm_c1[k];
+    if (c1 < c0) continue;
+    const Left u = sm_left[k];
+    const SeqDesc sq = s.seqs[u.e];
+    const int slot0 = 2 * c0 + (shares.begin(c0) == u.begin ? 0 : 1);
+    const int rows = min(R, sq.len * s.G - u.rg * R);
+    const int wpr = rows >= 4 ? 1 : rows >= 2 ? 2 : 4;  // warps for a row
+    float4* sm_o = reinterpret_cast<float4*>(smem_raw + ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));  // [warps][32]: the stages are done with
+    float* sm_ml = reinterpret_cast<float*>(sm_o + kWarps * 32);
+    for (int r0 = 0; r0 < rows; r0 += kWarps / wpr) {
+      const int r_in = r0 + warp / wpr;
+      float m = -INFINITY, l = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      auto join = [&](float pm, float pl, const float4& x) {
+        const float top = fmaxf(m, pm), to = top == -INFINITY ? 0.0f : top, a = ex2(m - to), f = ex2(pm - to);
+        m = top;
+        l = fmaf(pl, f, l * a);
+        o.x = fmaf(x.x, f, o.x * a); o.y = fmaf(x.y, f, o.y * a); o.z = fmaf(x.z, f, o.z * a); o.w = fmaf(x.w, f, o.w * a);
+      };
+      if (r_in < rows)
+        for (int q0 = c0 + warp % wpr; q0 <= c1; q0 += 8 * wpr) {
+          float2 ml[8];
+          float4 x[8];
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, sm_ml[w][0]);
-  const float to = m == -INFINITY ? 0.0f : m;
-  float y = 0.0f;
-  l = 0.0f;
+          for (int i = 0; i < 8; ++i) {
+            const int q = q0 + wpr * i;
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (q > c1) continue;
+            const size_t slot = static_cast<size_t>(q == c0 ? slot0 : 2 * q) * R + r_in;
+            ml[i] = __ldcg(reinterpret_cast<const float2*>(s.part_ml + slot * 2));
+            x[i] = __ldcg(reinterpret_cast<const float4*>(s.part_o + slot * 128 + 4 * lane));
+          }
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float f = ex2(sm_ml[w][0] - to);
-    l = fmaf(sm_ml[w][1], f, l);
-    y = fmaf(reinterpret_cast<const float*>(&sm_o[w][0])[d], f, y);
+          for (int i = 0; i < 8; ++i) join(ml[i].x, ml[i].y, x[i]);
+        }
+      if (wpr > 1) {
+        sm_o[warp * 32 + lane] = o;
+        if (lane == 0) { sm_ml[2 * warp] = m; sm_ml[2 * warp + 1] = l; }
+        __syncthreads();
+        if (warp % wpr == 0)
+          for (int w = warp + 1; w < warp + wpr; ++w) join(sm_ml[2 * w], sm_ml[2 * w + 1], sm_o[w * 32 + lane]);
+        __syncthreads();
+        if (warp % wpr) continue;
+      }
+      if (r_in >= rows) continue;
+      const int r = u.rg * R + r_in, i = r / s.G, hq = u.hk * s.G + r - i * s.G;
+      const size_t row = static_cast<size_t>(sq.row0) + i;
+      if (s.a.sink) l += ex2(fmaf(s.a.sink[hq], kLog2e, -m));
+      if (lane == 0) note_lse(s, row, hq, m + log2f(l));
+      if (4 * lane >= s.c.V) continue;
+      const float inv = 1.0f / l;
+      T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 4 * lane;
+      const float y[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int d = 0; d < 4; ++d) store_one(out + d, finished<T>(s, row, hq, 4 * lane + d, y[d], inv));
+    }
   }
-  const size_t row = static_cast<size_t>(sq.row0) + i;
-  if (s.a.sink) l += ex2(fmaf(s.a.sink[hq], kLog2e, -m));
-  if (d == 0) note_lse(s, row, hq, m + log2f(l));
-  if (d < s.c.V)
-    store_one(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + d, finished<T>(s, row, hq, d, y, 1.0f / l));
 }
 
 // Weights of single tokens' calls, from the scores that the attention kernel left: blockIdx = (share of the keys, kv head, entry).
@@ -731,10 +759,9 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
     ks[0] = s.c.ks[head * s.c.blocks + kb / s.c.B];
     ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + (kb + 16) / s.c.B] : 0.0f;
     float sum[4] = {};
-    const long long rows = static_cast<long long>(sq.len) * s.G;
-    for (long long r0 = static_cast<long long>(max(0, kb - sq.pos)) * s.G / 8 * 8; r0 < rows; r0 += 8) {
-      const long long r = r0 + g, at = min(r, rows - 1);
-      const int i = static_cast<int>(at / s.G), hq = hk * s.G + static_cast<int>(at - static_cast<long long>(i) * s.G);
+    const int rows = sq.len * s.G;
+    for (int r0 = max(0, kb - sq.pos) * s.G / 8 * 8; r0 < rows; r0 += 8) {
+      const int r = r0 + g, at = min(r, rows - 1), i = at / s.G, hq = hk * s.G + at - i * s.G;
       const size_t row = static_cast<size_t>(sq.row0) + i;
       uint32_t term[TERMS][16];
       const float f = split_row<T, TERMS>(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c,
@@ -783,7 +810,7 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   int kind, rows, parts, groups;
-  size_t part_o, part_ml, lse2, scores, bytes;
+  size_t arrivals, part_o, part_ml, lse2, scores, bytes;
 };
 template <typename F>
 void for_variant(int kind, F&& f) {  // rows in tiles of eight, or 0 for f32
@@ -806,6 +833,7 @@ Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len
   });
   p.groups = static_cast<int>((unit + p.rows - 1) / p.rows);
   auto take = [&](size_t n) { const size_t at = p.bytes; p.bytes += (n + 255) / 256 * 256; return at; };
+  p.arrivals = take(static_cast<size_t>(n_seqs) * c.H * p.groups * 4);
   p.part_o = take(static_cast<size_t>(2) * p.parts * p.rows * 128 * 4);
   p.part_ml = take(static_cast<size_t>(2) * p.parts * p.rows * 2 * 4);
   p.lse2 = weights ? take(static_cast<size_t>(rows) * Hq * 4) : 0;
@@ -846,9 +874,16 @@ size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows
   return plan_of(c, f32, Hq, rows, n_seqs, max_len, weights).bytes;
 }
 
+size_t cache8_attention_zeroed_bytes(const Cache8& c, int f32, int Hq, int n_seqs, int max_len) {
+  return plan_of(c, f32, Hq, 1, n_seqs, max_len, false).part_o;
+}
+
 int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc*, int n_seqs, int max_len, cudaStream_t st) {
   if (const int rc = prepare()) return rc;
   const Plan p = plan_of(c, a.f32, a.Hq, a.rows, n_seqs, max_len, a.weights != 0);
+  // the kernels count slices in 32 bits
+  if (static_cast<double>(max_len) * (a.Hq / c.H) > 2e9 || static_cast<double>(n_seqs) * c.H * p.groups * ((c.cap + kSlice - 1) / kSlice) > 2e9)
+    return TEENY_ERR_BAD_ARG;
   CUtensorMap mk, mv;
   if (const int rc = encode_codes(&mk, c.k, c.D, c)) return rc;
   if (const int rc = encode_codes(&mv, c.v, c.V, c)) return rc;
@@ -865,6 +900,8 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
     s.cap_l2 = a.softcap * kLog2e;
   }
   uint8_t* scratch = static_cast<uint8_t*>(a.scratch);
+  s.arrivals = reinterpret_cast<unsigned*>(scratch + p.arrivals);
+  s.max_groups = p.groups;
   s.part_o = reinterpret_cast<float*>(scratch + p.part_o);
   s.part_ml = reinterpret_cast<float*>(scratch + p.part_ml);
   if (a.weights) s.lse2 = reinterpret_cast<float*>(scratch + p.lse2);
@@ -880,11 +917,6 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
     launch_kernel(cache8_attention_kernel<V>, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
   });
   const PdlScope behind;
-  const long long unit_rows = static_cast<long long>(s.G) * max_len;
-  const int max_rows = static_cast<int>(unit_rows < p.rows ? unit_rows : p.rows);
-  const dim3 rows(static_cast<unsigned>(n_seqs) * c.H * p.groups * max_rows);
-  if (a.f32) launch_kernel(cache8_combine_kernel<float>, rows, dim3(256), 0, st, 1, s, p.rows, p.groups, max_rows);
-  else launch_kernel(cache8_combine_kernel<bf16>, rows, dim3(256), 0, st, 1, s, p.rows, p.groups, max_rows);
   if (a.weights) {
     const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);

@@ -544,6 +544,7 @@ struct Cache8Attn {
   size_t scratch_bytes;
 };
 size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights);
+size_t cache8_attention_zeroed_bytes(const Cache8& c, int f32, int Hq, int n_seqs, int max_len);
 int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int max_len, cudaStream_t st);
 size_t cache8_evict_scratch_bytes(const Cache8& c, int n_seqs, int keep);
 int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, int n_seqs, cudaStream_t st);

@@ -622,9 +622,12 @@ def cache8_append(cache, k, v, table):
 
 
 def cache8_attention_scratch(cache, table, q, weights=False):
-    """Scratch for calls with this many entries and rows (None: they need none).  Calls in one stream may share it."""
-    n = lib.teeny_cache8_attention_scratch_bytes(cache.shape, _f32_flag(q), q.shape[1], q.shape[0], table.n, table.longest, int(weights))
-    return torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+    """Scratch for calls with this many entries and rows.  Calls that follow one another in a stream may share it."""
+    f32, heads = _f32_flag(q), q.shape[1]
+    out = torch.empty(lib.teeny_cache8_attention_scratch_bytes(cache.shape, f32, heads, q.shape[0], table.n, table.longest, int(weights)),
+                      dtype=torch.uint8, device=cache.device)
+    out[:lib.teeny_cache8_attention_zeroed_bytes(cache.shape, f32, heads, table.n, table.longest)].zero_()
+    return out
 
 
 def cache8_attention(q, cache, score_scale, table, softcap=0.0, sink=None, gate=None, weight_decay=None, lse=None, out=None, scratch=None):
