@@ -54,8 +54,11 @@
 //   OPT 2  soft-capped scores as well: cap tanh(s / cap) by an odd polynomial while a warp's scores are all within half the cap
 //          (the multiply pipes have room beside the exponentials; two more special-function operations per score have not), by
 //          exponential and reciprocal otherwise.  In tiles without a mask the polynomial runs inside the exponential's loop.
+//   RAGGED entries of unequal lengths and positions in one launch, by a step table on the device: an item is a query tile of one entry, whose keys begin at
+//          a row of their own in k and v.  Output boxes that reach behind an entry's last row are written row by row.
 // Tensor memory columns per CTA: S0 0-127, S1 128-255 (f32 scores), O 256-383 (f32), Q 384-447, P 448-511 (bf16 pairs).
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -102,6 +105,13 @@ struct PrefillArgs {  // (Q, K, V and O travel as tensor maps)
   int gate;             // the gate's tensor map is valid
   const float* sink;    // [Hq] or null: exp(sink) joins the row sum
   int two_out_boxes;    // values are wider than one 64-column box
+  // RAGGED (Sq and Skv are the entry's, k and v have one batch)
+  const SeqDesc* seqs;
+  Cache8 cache;
+  int n_seqs, min_len, max_len, rows, key_rows;  // entries of at least min_len tokens; entry e's keys begin at row e * key_rows
+  float* lse2;       // base 2, like lse [rows, Hq]
+  bf16* out;
+  long long ldo;
   int n_pair_tiles;  // 256-row query tiles per (batch, head)
   int n_items;       // n_pair_tiles * Hq * B work items; CTA pair p takes items p, p + pairs, ...
   int* err;
@@ -238,7 +248,11 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
       : "memory");
 }
 
-template <int OPT, bool WIDE>
+constexpr int kRagged = 128;  // entries of a RAGGED launch at most
+struct PlainItem { int pt, h, b, hk, t0, n_tiles; };  // t0: first key tile
+struct RaggedItem : PlainItem { int Sq, Skv, row0, key0; };
+
+template <int OPT, bool WIDE, bool RAGGED = false>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                          const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_o,
@@ -273,11 +287,38 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   // item into the next: the loads of the next item's keys and values, and its first products, overlap the current
   // item's last softmax steps and output.
   const int pair_id = static_cast<int>(blockIdx.x >> 1), n_pairs = static_cast<int>(gridDim.x >> 1);
-  const int off = args.Skv - args.Sq;                           // causal: query i sees keys <= i + off
   const int heads_x_batch = args.Hq * args.B;
-  struct Item { int pt, h, b, hk, t0, n_tiles; };  // t0: first key tile
+  using Item = typename std::conditional<RAGGED, RaggedItem, PlainItem>::type;
+  __shared__ int rag_first[RAGGED ? kRagged + 1 : 1];  // items before an entry's
+  const int plain_off = args.Skv - args.Sq;  // causal: query i sees keys <= i + off
+  auto rows_of = [&](const Item& it) { if constexpr (RAGGED) return it.Sq; else return args.Sq; };
+  auto keys_of = [&](const Item& it) { if constexpr (RAGGED) return it.Skv; else return args.Skv; };
+  auto off_of = [&](const Item& it) { if constexpr (RAGGED) return it.Skv - it.Sq; else return plain_off; };
+  auto row0_of = [&](const Item& it) { if constexpr (RAGGED) return it.row0; else return 0; };
+  auto n_items = [&]() { if constexpr (RAGGED) return rag_first[args.n_seqs]; else return args.n_items; };
+  auto key0_of = [&](const Item& it) { if constexpr (RAGGED) return it.key0; else return 0; };
   auto item_at = [&](int item) {
     Item it;
+    if constexpr (RAGGED) {
+      int e = 0;  // the last entry that begins at or before the item
+#pragma unroll
+      for (int step = kRagged / 2; step > 0; step >>= 1)
+        if (e + step < args.n_seqs && rag_first[e + step] <= item) e += step;
+      const SeqDesc sq = args.seqs[e];
+      const int rest = item - rag_first[e], tiles = (sq.len + 2 * kQT - 1) / (2 * kQT);
+      it.pt = tiles - 1 - rest / args.Hq;
+      it.h = rest % args.Hq;
+      it.hk = it.h / (args.Hq / args.Hkv);
+      it.b = 0;
+      it.t0 = 0;
+      it.Sq = sq.len;
+      it.Skv = sq.pos + sq.len;
+      it.row0 = sq.row0;
+      it.key0 = e * args.key_rows;
+      it.n_tiles = (min(it.Skv, it.pt * 2 * kQT + 2 * kQT + sq.pos) + kKT - 1) / kKT;
+      return it;
+    }
+    const int off = plain_off;
     it.pt = args.n_pair_tiles - 1 - item / heads_x_batch;
     const int rest = item % heads_x_batch;
     it.b = rest / args.Hq;
@@ -310,6 +351,28 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  if constexpr (RAGGED) {
+    pdl_wait();
+    if (warp == 1) {
+      int run = 0;
+      for (int e0 = 0; e0 < args.n_seqs; e0 += 32) {
+        int mine = 0;
+        if (e0 + lane < args.n_seqs) {
+          const SeqDesc sq = args.seqs[e0 + lane];
+          if (sq.len >= args.min_len && cache8_fits(sq, args.cache, args.rows, args.max_len)) mine = (sq.len + 2 * kQT - 1) / (2 * kQT) * args.Hq;
+        }
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += up;
+        }
+        if (e0 + lane < args.n_seqs) rag_first[e0 + lane] = run + sum - mine;
+        run += __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == 0) rag_first[args.n_seqs] = run;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   pair_sync();  // both CTAs' barriers exist before either CTA can signal the other
@@ -325,7 +388,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   if (warp == 0) {
     if (lane == 0) {  // this CTA's 64 keys of every K tile
       bool ok = true;
-      for (int item = pair_id, g = 0; ok && item < args.n_items; item += n_pairs) {
+      for (int item = pair_id, g = 0; ok && item < n_items(); item += n_pairs) {
         const Item it = item_at(item);
         for (int j = 0; j < it.n_tiles; ++j, ++g) {
           const int st = g % kKV;
@@ -333,7 +396,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           if (!mbar_wait(bar(K_EMPTY + st), ph ^ 1, err, DEVERR_ATTN_PRODUCER)) { ok = false; break; }
           if (leader) mbar_expect_tx(bar(K_FULL + st), 2 * L::kStageK);  // both CTAs' halves
           const uint32_t dst = base + kSmemK + st * L::kStageK;
-          const int key0 = (it.t0 + j) * kKT + static_cast<int>(rank) * 64;
+          const int key0 = key0_of(it) + (it.t0 + j) * kKT + static_cast<int>(rank) * 64;
           tma_load_4d_pair(dst, &tmap_k, bar(K_FULL + st), 0, key0, it.hk, it.b);
           tma_load_4d_pair(dst + kKBoxBytes, &tmap_k, bar(K_FULL + st), 64, key0, it.hk, it.b);
           if (WIDE) tma_load_4d_pair(dst + 2 * kKBoxBytes, &tmap_k, bar(K_FULL + st), 128, key0, it.hk, it.b);
@@ -343,14 +406,14 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   } else if (warp == 3) {
     if (lane == 0) {  // this CTA's 64 d columns of every V tile
       bool ok = true;
-      for (int item = pair_id, g = 0; ok && item < args.n_items; item += n_pairs) {
+      for (int item = pair_id, g = 0; ok && item < n_items(); item += n_pairs) {
         const Item it = item_at(item);
         for (int j = 0; j < it.n_tiles; ++j, ++g) {
           const int st = g % kKV;
           const uint32_t ph = (g / kKV) & 1;
           if (!mbar_wait(bar(V_EMPTY + st), ph ^ 1, err, DEVERR_ATTN_PRODUCER)) { ok = false; break; }
           if (leader) mbar_expect_tx(bar(V_FULL + st), 2 * kHalfBytes);
-          tma_load_4d_pair(base + kSmemV + st * kHalfBytes, &tmap_v, bar(V_FULL + st), static_cast<int>(rank) * 64, (it.t0 + j) * kKT,
+          tma_load_4d_pair(base + kSmemV + st * kHalfBytes, &tmap_v, bar(V_FULL + st), static_cast<int>(rank) * 64, key0_of(it) + (it.t0 + j) * kKT,
                            it.hk, it.b);
         }
       }
@@ -367,7 +430,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       TRACE_ONLY(long long w_k = 0, w_se = 0, c0; const long long c_begin = clock64();)
       bool ok = true;
       int g = 0;
-      for (int item = pair_id, seq = 0; ok && item < args.n_items; item += n_pairs, ++seq) {
+      for (int item = pair_id, seq = 0; ok && item < n_items(); item += n_pairs, ++seq) {
         const Item it = item_at(item);
         if (!mbar_wait(bar(Q_READY), seq & 1, err, DEVERR_ATTN_MMA)) break;  // this item's Q is in tensor memory
         for (int j = 0; j < it.n_tiles; ++j, ++g) {
@@ -408,7 +471,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       TRACE_ONLY(long long w_v = 0, w_p = 0, c0; const long long c_begin = clock64();)
       bool ok = true;
       int g = 0;
-      for (int item = pair_id, seq = 0; ok && item < args.n_items; item += n_pairs, ++seq) {
+      for (int item = pair_id, seq = 0; ok && item < n_items(); item += n_pairs, ++seq) {
         const Item it = item_at(item);
         // the output accumulator is free once the softmax threads have read the previous item's out of it
         if (seq > 0 && !mbar_wait(bar(O_FREE), (seq - 1) & 1, err, DEVERR_ATTN_MMA)) break;
@@ -450,7 +513,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     // All 128 d columns of this thread's Q row of an item, global -> tensor memory (by the ONE group that opens the item)
     // An item's Q rows of this CTA, global -> the staging boxes in shared memory (one thread; an item ahead of their use)
     auto fetch_q = [&](const Item& it, int n) {  // n-th item of this pair
-      const int y = it.pt * 2 * kQT + static_cast<int>(rank) * kQT;
+      const int y = row0_of(it) + it.pt * 2 * kQT + static_cast<int>(rank) * kQT;
       mbar_expect_tx(bar(QS_FULL), (WIDE ? 3 : 2) * kQT * 128);
       if (WIDE) tma_load_4d(base + L::kSmemQX + (n & 1) * (kQT * 128), &tmap_q, bar(QS_FULL), 128, y, it.h, it.b);
       tma_load_4d(base + kSmemQ, &tmap_q, bar(QS_FULL), 0, y, it.h, it.b);
@@ -484,13 +547,13 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       if (gated_items > 0 && ok) ok = mbar_wait(bar(O_BOX + quarter), (gated_items - 1) & 1, err, DEVERR_ATTN_SOFTMAX);
       if (!ok) return;
       const uint32_t box = base + kSmemO + quarter * (32 * 256), full = bar(G_FULL + quarter);
-      const int y = q0 + quarter * 32;
+      const int y = row0_of(it) + q0 + quarter * 32;
       mbar_expect_tx(full, args.two_out_boxes ? 32 * 256 : 32 * 128);
       tma_load_4d(box, &tmap_g, full, 0, y, it.h, it.b);
       if (args.two_out_boxes) tma_load_4d(box + 32 * 128, &tmap_g, full, 64, y, it.h, it.b);
     };
     // The first item: group 1 brings Q in while group 0, which takes tile 0, has nothing else to do either.
-    if (wg == 1 && pair_id < args.n_items) {
+    if (wg == 1 && pair_id < n_items()) {
       if (r == 0) fetch_q(item_at(pair_id), 0);
       put_q(0);
     }
@@ -499,11 +562,11 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
     TRACE_ONLY(long long w_s = 0, w_s0 = 0, t_ld = 0, t_max = 0, w_pv = 0, t_exp = 0, t_end = 0, t_close = 0, c0; const long long c_begin = clock64();)
     int g0 = 0;  // key tiles of the items before this one: tile j of the item is tile g0 + j of the pair
     uint32_t m_seen0 = 0, m_seen1 = 0;
-    Item next_it = item_at(pair_id < args.n_items ? pair_id : 0);
+    Item next_it = item_at(pair_id < n_items() ? pair_id : 0);
 #pragma unroll 1
-    for (int item = pair_id, seq = 0; item < args.n_items; item += n_pairs, ++seq) {
+    for (int item = pair_id, seq = 0; item < n_items(); item += n_pairs, ++seq) {
       const Item it = next_it;  // worked out during the previous item's last waits: the divisions are off this group's path
-      const int n_tiles = it.n_tiles;
+      const int n_tiles = it.n_tiles, off = off_of(it);
       const int q0 = it.pt * 2 * kQT + static_cast<int>(rank) * kQT;   // this CTA's first query row
       const int qi = q0 + r;
       float* m_sh = xch + (seq & 1) * 384;  // running maximum of the item's rows, log2 domain
@@ -520,8 +583,8 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
       const int m_ready = M_READY + (seq & 1) * 2;
       const int j_other = (wg ^ 1) ^ (g0 & 1);
       const uint32_t m_seen = (seq & 1) ? m_seen1 : m_seen0;
-      const bool more = item + n_pairs < args.n_items;
-      const bool has_rows = q0 + quarter * 32 < args.Sq;  // this warp's rows of the item
+      const bool more = item + n_pairs < n_items();
+      const bool has_rows = q0 + quarter * 32 < rows_of(it);  // this warp's rows of the item
       if (!closer && more && r == 0) {
         // this group brings the next item's Q in, an item from now: fetch it as soon as this item's has left the boxes
         if (ok) ok = mbar_wait(bar(QS_FREE), seq & 1, err, DEVERR_ATTN_SOFTMAX);
@@ -568,7 +631,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         mbar_arrive_cluster(s_empty_leader);  // the buffer can take QK^T of tile g + 2 (once the peer's group is here too)
         const int k0 = (it.t0 + j) * kKT;
         const int first = args.window > 0 ? qi + off - args.window + 1 : 0;  // first visible key
-        const bool need_mask = (k0 + kKT > args.Skv) || (args.causal && (k0 + kKT - 1 > q0 + off)) ||
+        const bool need_mask = (k0 + kKT > keys_of(it)) || (args.causal && (k0 + kKT - 1 > q0 + off)) ||
                                (args.window > 0 && k0 < q0 + kQT + off - args.window);
         bool raw = false;  // the scores go uncapped into the exponential's loop
         float tmax = 0.0f;
@@ -589,7 +652,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           }
         }
         if (need_mask) {
-          const int limit = args.causal ? min(args.Skv - 1, qi + off) : args.Skv - 1;  // last visible key
+          const int limit = args.causal ? min(keys_of(it) - 1, qi + off) : keys_of(it) - 1;  // last visible key
 #pragma unroll
           for (int e = 0; e < 128; ++e)
             if (k0 + e > limit || k0 + e < first) s[e] = -INFINITY;
@@ -734,7 +797,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(l));  // l >= 1 (the row's maximum contributes 2^0); 1 ulp
           inv *= args.out_scale;
           const float2 inv2 = {inv, inv};
-          const bool valid = qi < args.Sq;
+          const bool valid = qi < rows_of(it);
           uint32_t t[4][32];  // the whole row in flight, so that the accumulator is free for the next item at once
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_32x32(tmem_o + lane_addr + c * 32, t[c]);
@@ -770,13 +833,28 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && y < args.Sq) {  // rows past the end are clipped by the copy
-            tma_store_4d(&tmap_o, o_box, 0, y, it.h, it.b);
-            if (args.two_out_boxes) tma_store_4d(&tmap_o, o_box + 32 * 128, 64, y, it.h, it.b);
+          if (RAGGED && y < rows_of(it) && y + 32 > rows_of(it)) {  // the rows behind are another entry's
+            if (valid) {
+              bf16* to = args.out + (static_cast<size_t>(row0_of(it)) + qi) * args.ldo + static_cast<size_t>(it.h) * args.cache.V;
+#pragma unroll
+              for (int ch = 0; ch < 16; ++ch)
+                if (ch * 8 < args.cache.V)
+                  *reinterpret_cast<uint4*>(to + ch * 8) = *reinterpret_cast<const uint4*>(orow + (ch >> 3) * (32 * 128) + (((ch & 7) ^ (lane & 7)) << 4));
+            }
+            __syncwarp();
+            leaving = lane == 0;  // (the boxes are free for a gate's rows, once lane 0 says so)
+          } else if (lane == 0 && y < rows_of(it)) {  // rows past the end are clipped by the copy
+            tma_store_4d(&tmap_o, o_box, 0, row0_of(it) + y, it.h, it.b);
+            if (args.two_out_boxes) tma_store_4d(&tmap_o, o_box + 32 * 128, 64, row0_of(it) + y, it.h, it.b);
             bulk_commit();
             leaving = true;
           }
-          if (valid && args.lse)
+          if constexpr (RAGGED) {
+            const size_t at = (static_cast<size_t>(row0_of(it)) + qi) * args.Hq + it.h;
+            const float lse2 = m_fin + log2f(l);
+            if (valid && args.lse2) args.lse2[at] = lse2;
+            if (valid && args.lse) args.lse[at] = 0.6931471805599453f * lse2;
+          } else if (valid && args.lse)
             args.lse[(static_cast<long long>(it.b) * args.Hq + it.h) * args.Sq + qi] = 0.6931471805599453f * (m_fin + log2f(l));
         } else {
           mbar_arrive_cluster(map_to_leader(bar(O_FREE)));  // after a failed wait: let the issuer run into its own limit, not hang on this
@@ -814,6 +892,18 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
   }
 }
 
+void set_softcap(PrefillArgs* a, float softcap, float scale) {
+  a->cap_l2 = softcap * 1.4426950408889634f;
+  a->two_y = 2.0f * a->scale_log2 / softcap;
+  a->scale_log2 = 1.0f;
+  // tanh(x) = x P(x^2) on [-1/2, 1/2]: minimax fit of the relative error (6e-7 in f32)
+  static const float kTanh[4] = {0.99999946f, -0.33326319f, 0.13190296f, -0.044402227f};
+  const float x = scale / softcap;
+  float power = x * a->cap_l2;
+  for (int i = 0; i < 4; ++i, power *= x * x) a->cap_c[i] = kTanh[i] * power;
+  a->small = a->cap_c[3] < -1e-30f ? 0.5f / x : -1.0f;  // (coefficients near the end of f32's range: exponential and reciprocal only)
+}
+
 // `d` < 128: the copies fill the columns beyond with zeros (loads) or leave them out (stores)
 int make_map(CUtensorMap* m, const bf16* p, int d, int S, int H, int B, long long ss, long long sh, long long sb, int box_rows) {
   const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(S), static_cast<uint64_t>(H), static_cast<uint64_t>(B)};
@@ -840,6 +930,9 @@ int attention_prefill_prepare() {
   raise(attention_prefill_kernel<2, false>, Smem<false>::kSmemTotal);
   raise(attention_prefill_kernel<0, true>, Smem<true>::kSmemTotal);
   raise(attention_prefill_kernel<2, true>, Smem<true>::kSmemTotal);
+  raise(attention_prefill_kernel<0, false, true>, Smem<false>::kSmemTotal);
+  raise(attention_prefill_kernel<1, false, true>, Smem<false>::kSmemTotal);
+  raise(attention_prefill_kernel<2, false, true>, Smem<false>::kSmemTotal);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   return 0;
@@ -877,17 +970,7 @@ int attention_prefill_bf16(const bf16* q, const bf16* k, const bf16* v, bf16* o,
   a.causal = s.causal;
   a.window = s.window;
   a.out_scale = s.out_scale;
-  if (s.softcap > 0.0f) {
-    a.cap_l2 = s.softcap * 1.4426950408889634f;
-    a.two_y = 2.0f * a.scale_log2 / s.softcap;
-    a.scale_log2 = 1.0f;
-    // tanh(x) = x P(x^2) on [-1/2, 1/2]: minimax fit of the relative error (6e-7 in f32)
-    static const float kTanh[4] = {0.99999946f, -0.33326319f, 0.13190296f, -0.044402227f};
-    const float x = s.scale / s.softcap;
-    float power = x * a.cap_l2;
-    for (int i = 0; i < 4; ++i, power *= x * x) a.cap_c[i] = kTanh[i] * power;
-    a.small = a.cap_c[3] < -1e-30f ? 0.5f / x : -1.0f;  // (coefficients near the end of f32's range: exponential and reciprocal only)
-  }
+  if (s.softcap > 0.0f) set_softcap(&a, s.softcap, s.scale);
   a.sink = s.sink;
   a.two_out_boxes = DV > 64;
   a.err = device_error_word();
@@ -915,6 +998,50 @@ int attention_prefill_bf16(const bf16* q, const bf16* k, const bf16* v, bf16* o,
                 : s.gate || s.sink ? (wide ? attention_prefill_kernel<1, true> : attention_prefill_kernel<1, false>)
                                    : (wide ? attention_prefill_kernel<0, true> : attention_prefill_kernel<0, false>);
   launch_kernel(kernel, grid, dim3(kThreads), wide ? Smem<true>::kSmemTotal : Smem<false>::kSmemTotal, stream, 2, mk, mv, mq, mo, mg, a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int attention_prefill_ragged(const Cache8& c, const Cache8Attn& t, const bf16* k, const bf16* v, int key_rows, float* lse2, const SeqDesc* seqs,
+                             int n_seqs, int min_len, int max_len, cudaStream_t stream) {
+  if (n_seqs <= 0 || n_seqs > kRagged) return TEENY_ERR_BAD_ARG;
+  if (const int rc = attention_prefill_prepare()) return rc;
+  CUtensorMap mk, mv, mq, mo, mg;
+  const long long keys = static_cast<long long>(n_seqs) * key_rows;
+  if (keys > 0x7fffffffLL) return TEENY_ERR_BAD_ARG;
+  int rc;
+  if ((rc = make_map(&mk, k, c.D, static_cast<int>(keys), c.H, 1, c.D, keys * c.D, keys * c.D * c.H, 64))) return rc;
+  if ((rc = make_map(&mv, v, c.V, static_cast<int>(keys), c.H, 1, c.V, keys * c.V, keys * c.V * c.H, 128))) return rc;
+  if ((rc = make_map(&mq, static_cast<const bf16*>(t.q), c.D, t.rows, t.Hq, 1, t.ldq, c.D, t.ldq, kQT))) return rc;
+  if ((rc = make_map(&mo, static_cast<bf16*>(t.out), c.V, t.rows, t.Hq, 1, t.ldo, c.V, t.ldo, 32))) return rc;
+  if (!t.gate) mg = mo;
+  else if ((rc = make_map(&mg, static_cast<const bf16*>(t.gate), c.V, t.rows, t.Hq, 1, t.ldg, c.V, t.ldg, 32))) return rc;
+  PrefillArgs a{};
+  a.gate = t.gate != nullptr;
+  a.lse = t.lse;
+  a.lse2 = lse2;
+  a.B = 1;
+  a.Hq = t.Hq;
+  a.Hkv = c.H;
+  a.scale_log2 = t.scale * 1.4426950408889634f;
+  a.causal = 1;
+  a.out_scale = 1.0f;
+  if (t.softcap > 0.0f) set_softcap(&a, t.softcap, t.scale);
+  a.sink = t.sink;
+  a.two_out_boxes = c.V > 64;
+  a.seqs = seqs;
+  a.cache = c;
+  a.n_seqs = n_seqs;
+  a.min_len = min_len;
+  a.max_len = max_len;
+  a.rows = t.rows;
+  a.key_rows = key_rows;
+  a.out = static_cast<bf16*>(t.out);
+  a.ldo = t.ldo;
+  a.err = device_error_word();
+  if (!a.err) return TEENY_ERR_DRIVER;
+  auto kernel = t.softcap > 0.0f ? attention_prefill_kernel<2, false, true>
+                : t.gate || t.sink ? attention_prefill_kernel<1, false, true> : attention_prefill_kernel<0, false, true>;
+  launch_kernel(kernel, dim3(static_cast<unsigned>(sm_count() / 2 * 2)), dim3(kThreads), Smem<false>::kSmemTotal, stream, 2, mk, mv, mq, mo, mg, a);
   return static_cast<int>(cudaGetLastError());
 }
 

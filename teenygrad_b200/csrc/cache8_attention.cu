@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   int kind, rows, parts, groups;
-  size_t arrivals, part_o, part_ml, lse2, scores, bytes;
+  size_t arrivals, part_o, part_ml, lse2, scores, widened, bytes;
 };
 template <typename F>
 void for_variant(int kind, F&& f) {  // rows in tiles of eight, or 0 for f32
@@ -820,24 +820,37 @@ void for_variant(int kind, F&& f) {  // rows in tiles of eight, or 0 for f32
   else if (kind == 3) f(Variant<3, 1>{});
   else f(Variant<4, 1>{});
 }
-Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights) {
+// max_len: of the entries that the main kernel takes.  Scratch has room for either way of dividing a call (see cache8_attention), wherever it lies.
+Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, int call_len, bool weights) {
   Plan p{};
-  const long long unit = static_cast<long long>(Hq / c.H) * max_len;  // rows of the longest entry and a kv head
-  // as few passes over the keys as there can be, and no more row tiles than they need
-  const long long passes = (unit + 31) / 32;
-  p.kind = f32 ? 0 : static_cast<int>((unit + 8 * passes - 1) / (8 * passes));
-  for_variant(p.kind, [&](auto v) {
-    using V = decltype(v);
-    p.rows = V::kRows;
-    p.parts = sm_count() * V::kCtas * kWarps;  // the warps that are resident at once
-  });
-  p.groups = static_cast<int>((unit + p.rows - 1) / p.rows);
+  auto divide = [&](int len) {
+    const long long unit = static_cast<long long>(Hq / c.H) * len;  // rows of the longest entry and a kv head
+    // as few passes over the keys as there can be, and no more row tiles than they need
+    const long long passes = (unit + 31) / 32;
+    p.kind = f32 ? 0 : static_cast<int>((unit + 8 * passes - 1) / (8 * passes));
+    for_variant(p.kind, [&](auto v) {
+      using V = decltype(v);
+      p.rows = V::kRows;
+      p.parts = sm_count() * V::kCtas * kWarps;  // the warps that are resident at once
+    });
+    p.groups = static_cast<int>((unit + p.rows - 1) / p.rows);
+    return static_cast<size_t>(2) * p.parts * p.rows;
+  };
+  const bool prompts = !f32 && call_len >= cache8_prefill_min_len(c, Hq);
+  size_t part_rows = divide(call_len);
+  const size_t groups = p.groups;
+  if (prompts) {
+    const size_t n = divide(cache8_prefill_min_len(c, Hq) - 1);
+    part_rows = part_rows > n ? part_rows : n;
+  }
+  divide(max_len);
   auto take = [&](size_t n) { const size_t at = p.bytes; p.bytes += (n + 255) / 256 * 256; return at; };
-  p.arrivals = take(static_cast<size_t>(n_seqs) * c.H * p.groups * 4);
-  p.part_o = take(static_cast<size_t>(2) * p.parts * p.rows * 128 * 4);
-  p.part_ml = take(static_cast<size_t>(2) * p.parts * p.rows * 2 * 4);
+  p.arrivals = take(static_cast<size_t>(n_seqs) * c.H * groups * 4);
+  p.part_o = take(part_rows * 128 * 4);
+  p.part_ml = take(part_rows * 2 * 4);
   p.lse2 = weights ? take(static_cast<size_t>(rows) * Hq * 4) : 0;
-  p.scores = weights && max_len == 1 ? take(static_cast<size_t>(n_seqs) * Hq * c.cap * 4) : 0;
+  p.scores = weights && call_len == 1 ? take(static_cast<size_t>(n_seqs) * Hq * c.cap * 4) : 0;
+  p.widened = prompts ? take(cache8_prefill_scratch_bytes(c, n_seqs)) : 0;
   return p;
 }
 int prepare() {
@@ -871,18 +884,28 @@ struct PdlScope {  // kernels of a call behind its first one start their set-up 
 }  // namespace
 
 size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights) {
-  return plan_of(c, f32, Hq, rows, n_seqs, max_len, weights).bytes;
+  return plan_of(c, f32, Hq, rows, n_seqs, max_len, max_len, weights).bytes;
 }
 
 size_t cache8_attention_zeroed_bytes(const Cache8& c, int f32, int Hq, int n_seqs, int max_len) {
-  return plan_of(c, f32, Hq, 1, n_seqs, max_len, false).part_o;
+  return plan_of(c, f32, Hq, 1, n_seqs, max_len, max_len, false).part_o;
 }
 
-int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc*, int n_seqs, int max_len, cudaStream_t st) {
+int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int call_len, cudaStream_t st) {
   if (const int rc = prepare()) return rc;
-  const Plan p = plan_of(c, a.f32, a.Hq, a.rows, n_seqs, max_len, a.weights != 0);
+  // Entries of many tokens go to the kernels of cache8_prefill.cu, the others to this file's: by their lengths on the device, the host only
+  // leaves out a launch that has nothing to do.
+  const int min_len = cache8_prefill_min_len(c, a.Hq);
+  const bool prompts = cache8_prefill_takes(c, a, call_len);
+  const int max_len = prompts && min_len - 1 < call_len ? min_len - 1 : call_len;
+  bool any_long = prompts, any_short = true;
+  if (host && prompts) {
+    any_long = any_short = false;
+    for (int i = 0; i < n_seqs; ++i) (host[i].len >= min_len ? any_long : any_short) |= host[i].len > 0;
+  }
+  const Plan p = plan_of(c, a.f32, a.Hq, a.rows, n_seqs, max_len, call_len, a.weights != 0);
   // the kernels count slices in 32 bits
-  if (static_cast<double>(max_len) * (a.Hq / c.H) > 2e9 || static_cast<double>(n_seqs) * c.H * p.groups * ((c.cap + kSlice - 1) / kSlice) > 2e9)
+  if (static_cast<double>(call_len) * (a.Hq / c.H) > 2e9 || static_cast<double>(n_seqs) * c.H * p.groups * ((c.cap + kSlice - 1) / kSlice) > 2e9)
     return TEENY_ERR_BAD_ARG;
   CUtensorMap mk, mv;
   if (const int rc = encode_codes(&mk, c.k, c.D, c)) return rc;
@@ -905,22 +928,27 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   s.part_o = reinterpret_cast<float*>(scratch + p.part_o);
   s.part_ml = reinterpret_cast<float*>(scratch + p.part_ml);
   if (a.weights) s.lse2 = reinterpret_cast<float*>(scratch + p.lse2);
-  if (a.weights && max_len == 1) s.scores = reinterpret_cast<float*>(scratch + p.scores);
+  if (a.weights && call_len == 1) s.scores = reinterpret_cast<float*>(scratch + p.scores);
   s.parts = p.parts;
   const int size = a.f32 ? 4 : 2;
   s.vec_q = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.ldq * size)) & 15) == 0;
   s.vec_o = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) & 15) == 0;
   s.err = device_error_word();
   if (!s.err) return TEENY_ERR_DRIVER;
-  for_variant(p.kind, [&](auto v) {
-    using V = decltype(v);
-    launch_kernel(cache8_attention_kernel<V>, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
-  });
-  const PdlScope behind;
+  if (any_long) {
+    if (const int rc = cache8_prefill(c, a, s.lse2, scratch + p.widened, seqs, n_seqs, call_len, st)) return rc;
+  }
+  if (any_short)
+    for_variant(p.kind, [&](auto v) {
+      using V = decltype(v);
+      launch_kernel(cache8_attention_kernel<V>, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
+    });
   if (a.weights) {
+    const PdlScope behind;
+    s.max_len = call_len;
     const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
-    if (max_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);
+    if (call_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);
     else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float>, grid, dim3(128), 0, st, 1, s);
     else launch_kernel(cache8_rows_weights_kernel<bf16>, grid, dim3(128), 0, st, 1, s);
   }
