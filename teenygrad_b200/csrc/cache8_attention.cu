@@ -943,9 +943,8 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
       using V = decltype(v);
       launch_kernel(cache8_attention_kernel<V>, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
     });
-  if (a.weights) {
+  if (a.weights && any_short) {
     const PdlScope behind;
-    s.max_len = call_len;
     const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
     if (call_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);

@@ -1,8 +1,11 @@
 // Prompts and long portions over the 8-bit cache: their work is the products, not the cache's bytes, so an entry's live tokens are widened to bf16 in
 // scratch once (exact: an E4M3 number times a power of two) and the tcgen05 kernel of attention_prefill.cu runs on those.  Widening
 // reads one byte and writes two for each number, 0.8 KB a token and kv head at head size 128, against len * group * 512 multiply-adds.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
+#include "mma.cuh"
 
 namespace teeny {
 
@@ -101,6 +104,246 @@ __global__ void __launch_bounds__(128) cache8_nan_kernel(const Cache8 c, const C
       static_cast<bf16*>(a.out)[(static_cast<size_t>(sq.row0) + i) * a.ldo + static_cast<size_t>(head * G + g) * c.V + d] = __ushort_as_bfloat16(0x7fff);
 }
 
+// ---- weights that the cached tokens receive from a prompt's rows ----
+// w_j = sum over rows i and the group's query heads of exp2(score_ij - lse2_i): the scores once more, transposed, with keys as the 128 rows of a tcgen05
+// product and query rows as its columns, so that a thread has one key and adds along its own registers; no sum crosses threads, and a key
+// tile's sums are one CTA's: no atomics.  Bound by the exponentials (128 x 128 of a tile take the special-function units 1024 clocks,
+// its product 512).  Two warpgroups take the tiles alternately, over four score buffers in tensor memory.
+constexpr int kWThreads = 384, kWQ = 3, kWLse = 4, kWS = 4;
+struct WSmem {
+  static constexpr int kK = 0;                                // two key tiles, two boxes of [128][64] each
+  static constexpr int kQ = kK + 2 * 32768;                   // ring of query tiles
+  static constexpr int kLse = kQ + kWQ * 32768;               // f32 [kWLse][128]
+  static constexpr int kSum = kLse + kWLse * 512;             // f32 [2][128]: what the second warpgroup hands over, by item
+  static constexpr int kBar = kSum + 2 * 512;
+  static constexpr int kTotal = kBar + 256 + 1024;
+};
+struct WeightsArgs {
+  Cache8 c;
+  const SeqDesc* seqs;
+  const float* lse2;  // [rows][Hq]
+  int n_seqs, key_rows, tiles, min_len, max_len, rows, Hq;
+  float scale_log2, two_over_cap, cap_l2, decay;
+  int* err;
+};
+
+__global__ void __launch_bounds__(kWThreads, 1)
+cache8_prompt_weights_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ WeightsArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int K_FULL = 0, K_EMPTY = 2, Q_FULL = 4, Q_EMPTY = Q_FULL + kWQ, S_FULL = Q_EMPTY + kWQ, S_EMPTY = S_FULL + kWS, L_FULL = S_EMPTY + kWS,
+                L_EMPTY = L_FULL + kWLse, X_FULL = L_EMPTY + kWLse, X_EMPTY = X_FULL + 2, kBars = X_EMPTY + 2;
+  static_assert(8 * kBars + 4 <= 256, "barrier block");
+  auto bar = [&](int i) { return base + WSmem::kBar + 8u * i; };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + WSmem::kBar + 8 * kBars);
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_q);
+    for (int i = 0; i < kBars; ++i)
+      mbar_init(bar(i), (i >= S_EMPTY && i < L_FULL) || i >= L_EMPTY ? 128 : i >= L_FULL ? 32 : 1);
+    mbar_fence_init();
+  }
+  if (warp == 3) {
+    tmem_alloc(base + WSmem::kBar + 8 * kBars, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  const int G = a.Hq / a.c.H, per_tile = a.n_seqs * a.c.H;
+  // item(n, entry, sq, kv head, first key, first query tile, query tiles) for every key tile of this CTA; key tiles with most rows come first
+  auto walk = [&](auto&& item) {
+    int n = 0;
+    for (int i = blockIdx.x; i < per_tile * a.tiles; i += gridDim.x) {
+      const int kt = i / per_tile, e = i % per_tile / a.c.H, hk = i % a.c.H;
+      const SeqDesc sq = a.seqs[e];
+      if (sq.len < a.min_len || !cache8_fits(sq, a.c, a.rows, a.max_len) || kt * 128 >= sq.pos + sq.len) continue;
+      if (!item(n++, e, sq, hk, kt * 128, max(0, kt * 128 - sq.pos) / 128, (sq.len + 127) / 128)) return;
+    }
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      int t = 0;
+      walk([&](int n, int e, const SeqDesc& sq, int hk, int key0, int q0, int q1) {
+        const int kb = n & 1;
+        if (!mbar_wait(bar(K_EMPTY + kb), (n >> 1 & 1) ^ 1, a.err, DEVERR_ATTN_PRODUCER)) return false;
+        mbar_expect_tx(bar(K_FULL + kb), 32768);
+        for (int x = 0; x < 2; ++x) tma_load_3d(base + WSmem::kK + kb * 32768 + x * 16384, &tmap_k, bar(K_FULL + kb), 64 * x, e * a.key_rows + key0, hk);
+        for (int g = 0; g < G; ++g)
+          for (int q = q0; q < q1; ++q, ++t) {
+            const int st = t % kWQ;
+            if (!mbar_wait(bar(Q_EMPTY + st), (t / kWQ & 1) ^ 1, a.err, DEVERR_ATTN_PRODUCER)) return false;
+            mbar_expect_tx(bar(Q_FULL + st), 32768);
+            for (int x = 0; x < 2; ++x)
+              tma_load_3d(base + WSmem::kQ + st * 32768 + x * 16384, &tmap_q, bar(Q_FULL + st), 64 * x, sq.row0 + q * 128, hk * G + g);
+          }
+        return true;
+      });
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_bf16(128, 128, false, false);
+      const uint64_t kd = make_smem_desc_sw128(base + WSmem::kK, 16, 1024), qd = make_smem_desc_sw128(base + WSmem::kQ, 16, 1024);
+      int t = 0;
+      walk([&](int n, int, const SeqDesc&, int, int, int q0, int q1) {
+        const int kb = n & 1, tiles = G * (q1 - q0);
+        if (!mbar_wait(bar(K_FULL + kb), n >> 1 & 1, a.err, DEVERR_ATTN_MMA)) return false;
+        for (int i = 0; i < tiles; ++i, ++t) {
+          const int st = t % kWQ, sb = t % kWS;
+          if (!mbar_wait(bar(Q_FULL + st), t / kWQ & 1, a.err, DEVERR_ATTN_MMA)) return false;
+          if (!mbar_wait(bar(S_EMPTY + sb), (t / kWS & 1) ^ 1, a.err, DEVERR_ATTN_MMA)) return false;
+          tc_fence_after();
+          const uint64_t ka = kd + static_cast<uint64_t>(kb * (32768 >> 4)), qb = qd + static_cast<uint64_t>(st * (32768 >> 4));
+          umma_bf16_ss_x4<2, 2>(tmem + sb * 128, ka, qb, idesc, 0u);
+          umma_bf16_ss_x4<2, 2>(tmem + sb * 128, ka + (16384 >> 4), qb + (16384 >> 4), idesc, 1u);
+          umma_commit(bar(Q_EMPTY + st));
+          umma_commit(bar(S_FULL + sb));
+        }
+        umma_commit(bar(K_EMPTY + kb));
+        return true;
+      });
+    }
+  } else if (warp == 2) {
+    int t = 0;
+    walk([&](int, int, const SeqDesc& sq, int hk, int, int q0, int q1) {
+      for (int g = 0; g < G; ++g)
+        for (int q = q0; q < q1; ++q, ++t) {
+          const int sl = t % kWLse;
+          if (!mbar_wait(bar(L_EMPTY + sl), (t / kWLse & 1) ^ 1, a.err, DEVERR_ATTN_PRODUCER)) return false;
+          float* to = reinterpret_cast<float*>(gen + WSmem::kLse) + sl * 128;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int i = q * 128 + x * 32 + lane;
+            to[x * 32 + lane] = i < sq.len ? a.lse2[(static_cast<size_t>(sq.row0) + i) * a.Hq + hk * G + g] : 0.0f;
+          }
+          mbar_arrive(bar(L_FULL + sl));
+        }
+      return true;
+    });
+  } else if (warp >= 4) {
+    const int wg = (warp - 4) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+    int t = 0;
+    walk([&](int n, int, const SeqDesc& sq, int hk, int key0, int q0, int q1) {
+      const bool mine = key0 + key < sq.pos + sq.len;
+      float* w = a.c.w + (static_cast<size_t>(sq.slot) * a.c.H + hk) * a.c.cap + key0 + key;
+      const float old = wg == 0 && mine && a.decay != 0.0f ? *w : 0.0f;
+      float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+      for (int g = 0; g < G; ++g)
+        for (int q = q0; q < q1; ++q, ++t) {
+          if ((t & 1) != wg) continue;
+          const int sb = t % kWS, sl = t % kWLse;
+          if (!mbar_wait(bar(L_FULL + sl), t / kWLse & 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
+          if (!mbar_wait(bar(S_FULL + sb), t / kWS & 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
+          tc_fence_after();
+          const int hidden = key0 + key - sq.pos - q * 128;  // columns before this one do not see the key
+          const int rows = sq.len - q * 128;  // columns from this one on are not the entry's
+          const bool masked = key0 + 127 > sq.pos + q * 128 || rows < 128;
+          const float4* lse = reinterpret_cast<const float4*>(gen + WSmem::kLse + sl * 512);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t r[32];
+            tmem_ld_32x32(tmem + lane_addr + sb * 128 + x * 32, r);
+            tmem_wait_ld();
+            if (a.cap_l2 > 0.0f) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(softcap_log2(__uint_as_float(r[i]) * a.scale_log2, a.two_over_cap, a.cap_l2));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 z = lse[x * 8 + i];
+              float2 s0 = make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), s1 = make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+              const float2 z0 = make_float2(-z.x, -z.y), z1 = make_float2(-z.z, -z.w);
+              s0 = a.cap_l2 > 0.0f ? __fadd2_rn(s0, z0) : __ffma2_rn(s0, sc2, z0);
+              s1 = a.cap_l2 > 0.0f ? __fadd2_rn(s1, z1) : __ffma2_rn(s1, sc2, z1);
+              if (masked) {
+                const int col = x * 32 + 4 * i;
+                if (col < hidden || col >= rows) s0.x = -INFINITY;
+                if (col + 1 < hidden || col + 1 >= rows) s0.y = -INFINITY;
+                if (col + 2 < hidden || col + 2 >= rows) s1.x = -INFINITY;
+                if (col + 3 < hidden || col + 3 >= rows) s1.y = -INFINITY;
+              }
+              sum[0] = __fadd2_rn(sum[0], make_float2(ex2(s0.x), ex2(s0.y)));
+              sum[1] = __fadd2_rn(sum[1], make_float2(ex2(s1.x), ex2(s1.y)));
+            }
+          }
+          tc_fence_before();
+          mbar_arrive(bar(S_EMPTY + sb));
+          mbar_arrive(bar(L_EMPTY + sl));
+        }
+      // the second warpgroup's part to the first
+      float* give = reinterpret_cast<float*>(gen + WSmem::kSum) + (n & 1) * 128 + key;
+      const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      if (wg == 1) {
+        if (!mbar_wait(bar(X_EMPTY + (n & 1)), (n >> 1 & 1) ^ 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
+        *give = total;
+        mbar_arrive(bar(X_FULL + (n & 1)));
+      } else {
+        if (!mbar_wait(bar(X_FULL + (n & 1)), n >> 1 & 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
+        const float all = total + *give;
+        mbar_arrive(bar(X_EMPTY + (n & 1)));
+        if (mine) *w = fmaf(a.decay, old, all);
+      }
+      return true;
+    });
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 3) {
+    if (*reinterpret_cast<volatile int*>(a.err) != 0) {  // (products under way may still write there)
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+int prompt_weights(const Cache8& c, const Cache8Attn& a, const Widened& w, const float* lse2, const SeqDesc* seqs, int min_len, int max_len, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};  // one bit per device; threads may race to set it
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !((done.load(std::memory_order_acquire) >> dev) & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(cache8_prompt_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WSmem::kTotal);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  const uint64_t keys = static_cast<uint64_t>(w.n_seqs) * w.key_rows, D = c.D;
+  const uint32_t box[3] = {64, 128, 1};
+  CUtensorMap mk, mq;
+  const uint64_t kdims[3] = {D, keys, static_cast<uint64_t>(c.H)}, kstrides[2] = {D * 2, D * 2 * keys};
+  const uint64_t qdims[3] = {D, static_cast<uint64_t>(a.rows), static_cast<uint64_t>(a.Hq)}, qstrides[2] = {static_cast<uint64_t>(a.ldq) * 2, D * 2};
+  if (const int rc = encode_tensor_map_bf16(&mk, w.k, 3, kdims, kstrides, box)) return rc;
+  if (const int rc = encode_tensor_map_bf16(&mq, a.q, 3, qdims, qstrides, box)) return rc;
+  WeightsArgs t{};
+  t.c = c;
+  t.seqs = seqs;
+  t.lse2 = lse2;
+  t.n_seqs = w.n_seqs;
+  t.key_rows = w.key_rows;
+  t.tiles = w.tiles;
+  t.min_len = min_len;
+  t.max_len = max_len;
+  t.rows = a.rows;
+  t.Hq = a.Hq;
+  t.scale_log2 = a.scale * 1.4426950408889634f;
+  if (a.softcap > 0.0f) {
+    t.two_over_cap = 2.0f / a.softcap;
+    t.cap_l2 = a.softcap * 1.4426950408889634f;
+  }
+  t.decay = a.decay;
+  t.err = device_error_word();
+  if (!t.err) return TEENY_ERR_DRIVER;
+  const long long items = static_cast<long long>(w.tiles) * w.n_seqs * c.H, sms = sm_count();
+  launch_kernel(cache8_prompt_weights_kernel, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kWThreads), WSmem::kTotal, st, 1, mk, mq, t);
+  return static_cast<int>(cudaGetLastError());
+}
+
 Widened widened_of(const Cache8& c, int n_seqs, void* scratch, size_t* bytes) {
   Widened w{};
   w.key_rows = (c.cap + kTile - 1) / kTile * kTile;
@@ -141,7 +384,8 @@ int cache8_prefill(const Cache8& c, const Cache8Attn& a, float* lse2, void* scra
     launch_kernel(cache8_widen_kernel, dim3(w.tiles, 2 * c.H, w.n_seqs), dim3(256), 0, st, 1, c, w, seqs + e, min_len, max_len, a.rows);
     const bool pdl = pdl_enabled();
     pdl_set_enabled(true);
-    const int rc = attention_prefill_ragged(c, a, w.k, w.v, w.key_rows, lse2, seqs + e, w.n_seqs, min_len, max_len, st);
+    int rc = attention_prefill_ragged(c, a, w.k, w.v, w.key_rows, lse2, seqs + e, w.n_seqs, min_len, max_len, st);
+    if (rc == 0 && a.weights) rc = prompt_weights(c, a, w, lse2, seqs + e, min_len, max_len, st);
     if (rc == 0) launch_kernel(cache8_nan_kernel, dim3(c.H, w.n_seqs), dim3(128), 0, st, 1, c, a, w, seqs + e, min_len, max_len);
     pdl_set_enabled(pdl);
     if (rc) return rc;
