@@ -136,14 +136,27 @@ __device__ __forceinline__ unsigned order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 constexpr int kSelThreads = 1024, kBins = 2048;
+constexpr int kMove = 128;      // tokens that a CTA of the move takes, a multiple of every block
+constexpr int kMoveThreads = 256;
+
+struct EvictScratch {
+  unsigned* ticket;  // pieces handed out so far
+  unsigned* loaded;  // [pieces of a head][entries][kv heads][keys, values]: the piece's tokens are in registers
+};
 
 // The kept tokens of one (entry, head), in order.  The smallest kept weight is found by digits, 11, 11 and 10 bits from the top: a histogram of
-// the next digit of the keys that agree with the digits found so far.
-__global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8 c, int keep, int recent, int* kept, const SeqDesc* seqs) {
+// the next digit of the keys that agree with the digits found so far.  Each warp has a stretch of the candidates, in registers up to 32 PER of them (PER 0:
+// read again for every digit).
+template <int PER>
+__global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8 c, int keep, int recent, int* kept, const EvictScratch x, const SeqDesc* seqs) {
   __shared__ int hist[kBins], sums[32], found[2], warp_gt[32], warp_eq[32];
   const int head = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   const SeqDesc sq = seqs[blockIdx.y];
+  const int pieces = (keep + kMove - 1) / kMove;
+  for (int i = tid; i < 2 * pieces; i += kSelThreads)
+    x.loaded[(static_cast<size_t>(i >> 1) * gridDim.y + blockIdx.y) * 2 * c.H + 2 * head + (i & 1)] = 0;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *x.ticket = 0;
   int* out = kept + (static_cast<size_t>(blockIdx.y) * c.H + head) * keep;
   const bool ok = sq.slot >= 0 && sq.slot < c.slots && sq.pos >= 0 && sq.pos <= c.cap;
   const int len = ok ? sq.pos : 0;
@@ -153,17 +166,32 @@ __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8
   }
   const float* w = c.w + (static_cast<size_t>(sq.slot) * c.H + head) * c.cap;
   const int cand = len - recent, want = keep - recent;
+  const int stretch = (cand + 1023) / 1024 * 32, first = min(cand, warp * stretch), last = min(cand, first + stretch);
+  unsigned own[PER > 0 ? PER : 1];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) own[i] = first + 32 * i + lane < last ? order_key(w[first + 32 * i + lane]) : 0u;
+  // f(key, place, there) for this lane's candidates; every lane of the warp is there each time
+  auto each = [&](auto&& f) {
+    if constexpr (PER > 0) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (first + 32 * i < last) f(own[i], first + 32 * i + lane, first + 32 * i + lane < last);
+    } else {
+#pragma unroll 4
+      for (int i = first; i < last; i += 32) f(i + lane < last ? order_key(w[i + lane]) : 0u, i + lane, i + lane < last);
+    }
+  };
   unsigned prefix = 0;
   int left = want;  // of the keys that agree with the prefix, the `left` largest are kept
   if (want > 0) {
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+      hist[tid] = hist[tid + 1024] = 0;
       __syncthreads();
-      for (int i = tid; i < cand; i += kSelThreads) {
-        const unsigned key = order_key(w[i]);
-        if (pass == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1);
-      }
+      each([&](unsigned key, int, bool there) {
+        if (there && (pass == 0 || key >> (shift + bits) == prefix)) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1);
+      });
       __syncthreads();
       // counts from the largest digit down: thread t has digits 2047 - 2t and 2046 - 2t
       const int hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
@@ -175,87 +203,135 @@ __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8
       }
       if (lane == 31) sums[warp] = run;
       __syncthreads();
-      int above = run - hi - lo;
-      for (int k = 0; k < warp; ++k) above += sums[k];
+      const int before = __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0), above = run - hi - lo + before;
       if (above < left && left <= above + hi) { found[0] = kBins - 1 - 2 * tid; found[1] = above; }
       else if (above + hi < left && left <= above + hi + lo) { found[0] = kBins - 2 - 2 * tid; found[1] = above + hi; }
       __syncthreads();
       prefix = prefix << bits | static_cast<unsigned>(found[0]);
       left -= found[1];
-      __syncthreads();
     }
   }
-  // each warp has a stretch of the candidates: count, then write behind what the warps before keep
-  const int stretch = (cand + 31) / 32, first = min(cand, warp * stretch), last = min(cand, first + stretch);
+  // count, then write behind what the warps before keep
   int gt = 0, eq = 0;
-  for (int i = first; i < last; i += 32) {
-    const unsigned key = i + lane < last ? order_key(w[i + lane]) : 0u;
-    const bool in = i + lane < last && want > 0;
-    gt += __popc(__ballot_sync(0xffffffffu, in && key > prefix));
-    eq += __popc(__ballot_sync(0xffffffffu, in && key == prefix));
-  }
+  each([&](unsigned key, int, bool there) {
+    gt += __popc(__ballot_sync(0xffffffffu, there && want > 0 && key > prefix));
+    eq += __popc(__ballot_sync(0xffffffffu, there && want > 0 && key == prefix));
+  });
   if (lane == 0) { warp_gt[warp] = gt; warp_eq[warp] = eq; }
   __syncthreads();
-  int above = 0, ties = 0;
-  for (int k = 0; k < warp; ++k) { above += warp_gt[k]; ties += warp_eq[k]; }
-  for (int i = first; i < last; i += 32) {
-    const unsigned key = i + lane < last ? order_key(w[i + lane]) : 0u;
-    const bool in = i + lane < last && want > 0;
-    const unsigned g = __ballot_sync(0xffffffffu, in && key > prefix), e = __ballot_sync(0xffffffffu, in && key == prefix);
+  int above = __reduce_add_sync(0xffffffffu, lane < warp ? warp_gt[lane] : 0), ties = __reduce_add_sync(0xffffffffu, lane < warp ? warp_eq[lane] : 0);
+  each([&](unsigned key, int place, bool there) {
+    const unsigned g = __ballot_sync(0xffffffffu, there && want > 0 && key > prefix), e = __ballot_sync(0xffffffffu, there && want > 0 && key == prefix);
     const unsigned below = (1u << lane) - 1;
     const int tie = ties + __popc(e & below), at = above + __popc(g & below) + min(tie, left);
-    if ((g >> lane & 1) || ((e >> lane & 1) && tie < left)) out[at] = i + lane;
+    if ((g >> lane & 1) || ((e >> lane & 1) && tie < left)) out[at] = place;
     above += __popc(g);
     ties += __popc(e);
-  }
+  });
   for (int i = tid; i < recent; i += kSelThreads) out[want + i] = cand + i;
 }
 
-// Kept tokens to the front, block by block in order: a kept token's row is never before its place, so a block's rows are read before any
-// write reaches them.  One CTA for the keys or the values of an (entry, head).
-__global__ void __launch_bounds__(kThreads) cache8_compact_kernel(const Cache8 c, int keep, const int* kept, const SeqDesc* seqs) {
-  __shared__ float sh[kThreads / 32];
-  constexpr int kMost = kCache8Block * kCache8Head / 16 / kThreads;
+// Kept tokens to the front, in place and in parallel: a piece is 128 places of a head's keys or values, whose tokens come from there or from behind.
+// So a piece must not be written before the pieces in front of it have been read, which may be from there.  Pieces are handed out in
+// their order: a CTA reads its tokens into registers, says so, and waits, before it writes, for those in front, which are running and wait for
+// nothing before they have said it.  Each byte is read once and written once; tokens that stay where and what they are are not written.
+__global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cache8 c, int keep, int n_seqs, const int* kept, const EvictScratch x, const SeqDesc* seqs, int* err) {
+  constexpr int kMost = kMove * kCache8Head / 16 / kMoveThreads;
+  __shared__ unsigned top[kMove / 16], sm_ticket;
+  __shared__ int sm_failed;
   pdl_wait();
-  const SeqDesc sq = seqs[blockIdx.y];
-  if (sq.slot < 0 || sq.slot >= c.slots || sq.pos < 0 || sq.pos > c.cap) return;
-  const int head = blockIdx.x >> 1, of_v = blockIdx.x & 1, d = of_v ? c.V : c.D, per = d / 16, len = min(sq.pos, keep);
-  const size_t sh_row = static_cast<size_t>(sq.slot) * c.H + head;
-  uint8_t* codes = (of_v ? c.v : c.k) + sh_row * c.cap * d;
-  float* scales = (of_v ? c.vs : c.ks) + sh_row * c.blocks;
-  float* w = c.w + sh_row * c.cap;
-  const int* index = kept + (static_cast<size_t>(blockIdx.y) * c.H + head) * keep;
-  for (int t0 = 0; t0 < len; t0 += c.B) {
-    const int tokens = min(c.B, len - t0), chunks = tokens * per;
-    uint4 x[kMost];
-    float s[kMost], amax = 0.0f, wt = 0.0f;
-#pragma unroll
-    for (int m = 0; m < kMost; ++m) {
-      const int i = threadIdx.x + m * kThreads;
-      if (i >= chunks) break;
-      const int from = index[t0 + i / per];
-      x[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from) * d + i % per * 16);
-      s[m] = scales[from / c.B];
-      const uint32_t r[4] = {x[m].x, x[m].y, x[m].z, x[m].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 y = decode4(r[e]);
-        amax = fmaxf(amax, s[m] * fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
-      }
-    }
-    if (!of_v && threadIdx.x < tokens) wt = w[index[t0 + threadIdx.x]];
-    amax = block_max(amax, sh);
-    const float scale = pow2(scale_exponent(amax)), inv = pow2(127 - static_cast<int>(__float_as_uint(scale) >> 23));
-#pragma unroll
-    for (int m = 0; m < kMost; ++m) {
-      const int i = threadIdx.x + m * kThreads;
-      if (i >= chunks) break;
-      reinterpret_cast<uint4*>(codes + static_cast<size_t>(t0) * d)[i] = rescale16(x[m], s[m] * inv);
-    }
-    if (threadIdx.x == 0) scales[t0 / c.B] = scale;
-    if (!of_v && threadIdx.x < tokens) w[t0 + threadIdx.x] = wt;
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    sm_ticket = atomicAdd(x.ticket, 1u);
+    sm_failed = 0;
   }
+  if (threadIdx.x < kMove / 16) top[threadIdx.x] = 0u;
+  __syncthreads();
+  const int heads = 2 * c.H, piece = static_cast<int>(sm_ticket / (n_seqs * heads)), who = static_cast<int>(sm_ticket % (n_seqs * heads));
+  const int e = who / heads, head = who % heads >> 1, of_v = who & 1, d = of_v ? c.V : c.D, per = d / 16;
+  const SeqDesc sq = seqs[e];
+  if (sq.slot < 0 || sq.slot >= c.slots || sq.pos < 0 || sq.pos > c.cap) return;
+  const int t0 = piece * kMove, tokens = min(kMove, min(sq.pos, keep) - t0), chunks = tokens * per;
+  if (tokens <= 0) return;
+  const size_t row = static_cast<size_t>(sq.slot) * c.H + head;
+  uint8_t* codes = (of_v ? c.v : c.k) + row * c.cap * d;
+  float* scales = (of_v ? c.vs : c.ks) + row * c.blocks;
+  float* w = c.w + row * c.cap;
+  const int* index = kept + (static_cast<size_t>(e) * c.H + head) * keep + t0;
+  uint4 v[kMost];
+  float s[kMost], wt = 0.0f;
+  int from[kMost];
+#pragma unroll
+  for (int m = 0; m < kMost; ++m) {
+    const int i = threadIdx.x + m * kMoveThreads;
+    from[m] = i < chunks ? index[i / per] : 0;
+  }
+#pragma unroll
+  for (int m = 0; m < kMost; ++m) {
+    const int i = threadIdx.x + m * kMoveThreads;
+    s[m] = 0.0f;
+    v[m] = make_uint4(0u, 0u, 0u, 0u);
+    if (i >= chunks) continue;
+    v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + i % per * 16);
+    s[m] = scales[from[m] / c.B];
+  }
+  if (!of_v && threadIdx.x < tokens) wt = w[index[threadIdx.x]];
+#pragma unroll
+  for (int m = 0; m < kMost; ++m) {
+    const int i = threadIdx.x + m * kMoveThreads;
+    const uint32_t r[4] = {v[m].x, v[m].y, v[m].z, v[m].w};
+    float amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 y = decode4(r[k]);
+      amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
+    }
+    const unsigned bits = __float_as_uint(amax * s[m]);  // (>= 0: ordered like its bits)
+    if (per == 8) {  // a warp's four tokens lie in one block
+      const unsigned most = __reduce_max_sync(0xffffffffu, bits);
+      if ((threadIdx.x & 31) == 0 && i < chunks) atomicMax(&top[i / 8 / c.B], most);
+    } else if (i < chunks) {
+      atomicMax(&top[i / per / c.B], bits);
+    }
+  }
+  __syncthreads();  // (every load of the CTA has arrived)
+  unsigned* flags = x.loaded + static_cast<size_t>(who);
+  const size_t stride = static_cast<size_t>(n_seqs) * heads;
+  if (threadIdx.x == 0) {
+    __threadfence();
+    asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(flags + piece * stride) : "memory");
+  }
+  if (threadIdx.x < 32) {
+    bool fine = true;
+    uint64_t since = 0;
+    for (int p = threadIdx.x; p < piece && fine; p += 32)
+      for (unsigned it = 0;; ++it) {
+        unsigned there;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(flags + p * stride) : "memory");
+        if (there) break;
+        if ((it & 63) == 63) {
+          const uint64_t now = global_timer_ns();
+          if (since == 0) since = now;
+          if (*reinterpret_cast<volatile int*>(err) != 0 || now - since > kWaitLimitNs) {
+            atomicCAS(err, 0, DEVERR_CACHE_MOVE);
+            fine = false;
+            break;
+          }
+        }
+      }
+    if (!fine) sm_failed = 1;
+  }
+  __syncthreads();
+  if (sm_failed) return;
+#pragma unroll
+  for (int m = 0; m < kMost; ++m) {
+    const int i = threadIdx.x + m * kMoveThreads;
+    if (i >= chunks) continue;
+    const int t = i / per, k = scale_exponent(__uint_as_float(top[t / c.B]));
+    if (from[m] == t0 + t && s[m] == pow2(k)) continue;
+    reinterpret_cast<uint4*>(codes + static_cast<size_t>(t0) * d)[i] = rescale16(v[m], s[m] * pow2(-k));
+  }
+  if (threadIdx.x < (tokens + c.B - 1) / c.B) scales[t0 / c.B + threadIdx.x] = pow2(scale_exponent(__uint_as_float(top[threadIdx.x])));
+  if (!of_v && threadIdx.x < tokens) w[t0 + threadIdx.x] = wt;
 }
 
 }  // namespace
@@ -271,11 +347,25 @@ int cache8_append(const Cache8& c, const Cache8Append& a, const SeqDesc* seqs, i
   return static_cast<int>(cudaGetLastError());
 }
 
-size_t cache8_evict_scratch_bytes(const Cache8&, int, int) { return 0; }
+size_t cache8_evict_scratch_bytes(const Cache8& c, int n_seqs, int keep) {
+  return 256 + static_cast<size_t>((keep + kMove - 1) / kMove) * n_seqs * 2 * c.H * 4;
+}
 
-int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void*, const SeqDesc* seqs, int n_seqs, cudaStream_t st) {
-  launch_kernel(cache8_select_kernel, dim3(c.H, n_seqs), dim3(kSelThreads), 0, st, 1, c, keep, recent, kept, seqs);
-  launch_kernel(cache8_compact_kernel, dim3(2 * c.H, n_seqs), dim3(kThreads), 0, st, 1, c, keep, static_cast<const int*>(kept), seqs);
+int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, int n_seqs, cudaStream_t st) {
+  int* err = device_error_word();
+  if (!err) return TEENY_ERR_DRIVER;
+  const long long pieces = static_cast<long long>((keep + kMove - 1) / kMove) * n_seqs * 2 * c.H;
+  if (pieces > 0x7fffffffLL) return TEENY_ERR_BAD_ARG;
+  const EvictScratch x{static_cast<unsigned*>(scratch), reinterpret_cast<unsigned*>(static_cast<uint8_t*>(scratch) + 256)};
+  auto select = [&](auto kernel) { launch_kernel(kernel, dim3(c.H, n_seqs), dim3(kSelThreads), 0, st, 1, c, keep, recent, kept, x, seqs); };
+  const int most = c.cap - recent;  // candidates
+  if (most <= 2 * kSelThreads) select(cache8_select_kernel<2>);
+  else if (most <= 16 * kSelThreads) select(cache8_select_kernel<16>);
+  else select(cache8_select_kernel<0>);
+  const bool pdl = pdl_enabled();
+  pdl_set_enabled(true);
+  launch_kernel(cache8_move_kernel, dim3(static_cast<unsigned>(pieces)), dim3(kMoveThreads), 0, st, 1, c, keep, n_seqs, static_cast<const int*>(kept), x, seqs, err);
+  pdl_set_enabled(pdl);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -25,6 +25,7 @@ enum : int {
   DEVERR_ATTN_MMA = 0x202,
   DEVERR_ATTN_SOFTMAX = 0x203,
   DEVERR_TP_GATHER = 0x301,
+  DEVERR_CACHE_MOVE = 0x401,
 };
 
 // Host side (defined in api.cu): device address of the per-device error word.

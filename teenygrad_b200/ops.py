@@ -552,6 +552,7 @@ class StepTable:
         self.n, self.longest = len(rows), max(e[3] for e in rows)
         self.seqs = torch.tensor(rows, dtype=torch.int32, device=device)
         self.host = (C.c_int * (4 * self.n))(*[x for e in rows for x in e])
+        self._at = self.seqs.data_ptr(), C.addressof(self.host), self.n, self.longest
 
 
 def step_table(entries, device="cuda"):
@@ -580,6 +581,11 @@ class Cache8:
             raise ValueError("blocks are of 16, 32, 64 or 128 tokens, head sizes multiples of 16 up to 128")
         self.k, self.v, self.k_scale, self.v_scale, self.weights, self.block, self.device = k, v, k_scale, v_scale, weights, block, k.device
         self.shape = Cache8Shape(slots, heads, cap, dim, v.shape[-1], block)
+        # what every call passes on, as the plain integers that ctypes takes fastest
+        self.kv_heads, self.dim, self.vdim, self._index = heads, dim, v.shape[-1], k.device.index
+        self._shape_at = C.addressof(self.shape)
+        self._at = self._shape_at, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+        self._weights_at = _ptr(weights)
 
 
 def cache8(slots, kv_heads, max_len, dim, vdim=None, block=64, weights=False, device="cuda"):
@@ -590,43 +596,45 @@ def cache8(slots, kv_heads, max_len, dim, vdim=None, block=64, weights=False, de
                   of(_F32, blocks), of(_F32, blocks), block, of(_F32, max_len) if weights else None)
 
 
-def _on(device, **tensors):
+def _on(cache, *tensors):
     """Everything a call gets lies on the cache's device, which is the current one (the call goes to its current stream)."""
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the cache is on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, it is on {t.device}")
+    index = cache._index
+    if index != (torch.cuda.current_device() if _current_device is None else _current_device()):
+        raise ValueError(f"the cache is on {cache.device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"the cache is on {cache.device}, a tensor of the call on {t.device}")
 
 
 def _head_rows(t, heads, dim, name):
     """``t`` [rows, heads, dim] whose heads lie side by side -> distance of its rows."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or (dim > 1 and stride[2] != 1) or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{name} must be [rows, {heads}, {dim}] with its heads side by side")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * dim)
+    return stride[0] if shape[0] > 1 else max(stride[0], heads * dim)
 
 
 def cache8_append(cache, k, v, table):
     """Tokens k [rows, kv_heads, dim] and v [rows, kv_heads, vdim] (bf16 or f32) of the table's entries into the cache at their
     positions.  The scale of a block that already holds older tokens of the sequence never shrinks, and they are held at the new
     one; the new tokens' weights are set to zero."""
-    s = cache.shape
-    _on(cache.device, k=k, v=v, table=table.seqs)
-    _req(v, k.dtype, "v")
-    ldk, ldv = _head_rows(k, s.kv_heads, s.dim, "k"), _head_rows(v, s.kv_heads, s.vdim, "v")
-    if k.shape[0] != v.shape[0]:
+    heads = cache.kv_heads
+    _on(cache, k, v, table.seqs)
+    if v.dtype != k.dtype:
+        raise ValueError(f"v must be {k.dtype}, got {v.dtype}")
+    ldk, ldv, rows = _head_rows(k, heads, cache.dim, "k"), _head_rows(v, heads, cache.vdim, "v"), k.shape[0]
+    if rows != v.shape[0]:
         raise ValueError("k and v have different numbers of rows")
-    check(lib.teeny_cache8_append(_f32_flag(k), s, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(cache.weights),
-                                  _ptr(k), ldk, _ptr(v), ldv, k.shape[0], _ptr(table.seqs), table.host, table.n, table.longest, _stream()),
+    check(lib.teeny_cache8_append(_f32_flag(k), *cache._at, cache._weights_at, k.data_ptr(), ldk, v.data_ptr(), ldv, rows, *table._at, _stream()),
           "cache8_append")
 
 
 def cache8_attention_scratch(cache, table, q, weights=False):
     """Scratch for calls with this many entries and rows.  Calls that follow one another in a stream may share it."""
     f32, heads = _f32_flag(q), q.shape[1]
-    out = torch.empty(lib.teeny_cache8_attention_scratch_bytes(cache.shape, f32, heads, q.shape[0], table.n, table.longest, int(weights)),
+    out = torch.empty(lib.teeny_cache8_attention_scratch_bytes(cache._shape_at, f32, heads, q.shape[0], table.n, table.longest, int(weights)),
                       dtype=torch.uint8, device=cache.device)
-    out[:lib.teeny_cache8_attention_zeroed_bytes(cache.shape, f32, heads, table.n, table.longest)].zero_()
+    out[:lib.teeny_cache8_attention_zeroed_bytes(cache._shape_at, f32, heads, table.n, table.longest)].zero_()
     return out
 
 
@@ -635,21 +643,18 @@ def cache8_attention(q, cache, score_scale, table, softcap=0.0, sink=None, gate=
     already; ``softcap``, ``sink`` f32 [heads] and ``gate`` [rows, heads * vdim] as in cached_attention.  With ``weight_decay`` every live token's
     weight becomes weight_decay * weight + the probabilities it got (0.0: those alone).  ``lse`` f32 [rows, heads] receives the logarithms of the
     softmax denominators.  Returns [rows, heads, vdim]."""
-    s = cache.shape
-    _on(cache.device, q=q, table=table.seqs, sink=sink, gate=gate, lse=lse, out=out, scratch=scratch)
-    f32, heads = _f32_flag(q), q.shape[1]
-    ldq = _head_rows(q, heads, s.dim, "q")
-    rows = q.shape[0]
+    _on(cache, q, table.seqs, sink, gate, lse, out, scratch)
+    f32, (rows, heads, _), vdim = _f32_flag(q), q.shape, cache.vdim
+    ldq = _head_rows(q, heads, cache.dim, "q")
     if out is None:
-        out = torch.zeros(rows, heads, s.vdim, dtype=q.dtype, device=q.device)
-    ldo = _head_rows(_req(out, q.dtype, "out"), heads, s.vdim, "out")
-    ldg = 0
+        out = torch.zeros(rows, heads, vdim, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape[0] != rows:
+        raise ValueError(f"out must be {q.dtype} with {rows} rows")
+    ldo, ldg = _head_rows(out, heads, vdim, "out"), 0
     if gate is not None:
-        if _req(gate, q.dtype, "gate").shape != (rows, heads * s.vdim) or gate.stride(1) != 1:
-            raise ValueError(f"gate must be [{rows}, {heads * s.vdim}]")
-        ldg = gate.stride(0) if rows > 1 else heads * s.vdim
-    if out.shape[0] != rows:
-        raise ValueError(f"out must have {rows} rows")
+        if _req(gate, q.dtype, "gate").shape != (rows, heads * vdim) or gate.stride(1) != 1:
+            raise ValueError(f"gate must be [{rows}, {heads * vdim}]")
+        ldg = gate.stride(0) if rows > 1 else heads * vdim
     if sink is not None and (_req(sink, _F32, "sink").shape != (heads,) or not sink.is_contiguous()):
         raise ValueError(f"sink must be [{heads}]")
     if lse is not None and (_req(lse, _F32, "lse").shape != (rows, heads) or not lse.is_contiguous()):
@@ -659,35 +664,31 @@ def cache8_attention(q, cache, score_scale, table, softcap=0.0, sink=None, gate=
         raise ValueError("this cache has no weights")
     if scratch is None:
         scratch = cache8_attention_scratch(cache, table, q, count)
-    check(lib.teeny_cache8_attention(f32, s, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale),
-                                     _ptr(cache.weights) if count else None, float(weight_decay) if count else 0.0, _ptr(q), ldq, _ptr(out), ldo,
-                                     rows, heads, float(score_scale), float(softcap), _ptr(sink), _ptr(gate), ldg, _ptr(lse), _ptr(scratch),
-                                     scratch.numel() if scratch is not None else 0, _ptr(table.seqs), table.host, table.n, table.longest,
-                                     _stream()), "cache8_attention")
+    check(lib.teeny_cache8_attention(f32, *cache._at, cache._weights_at if count else None, weight_decay if count else 0.0, q.data_ptr(), ldq,
+                                     out.data_ptr(), ldo, rows, heads, score_scale, softcap, _ptr(sink), _ptr(gate), ldg, _ptr(lse),
+                                     scratch.data_ptr(), scratch.numel(), *table._at, _stream()), "cache8_attention")
     return out
 
 
 def cache8_evict_scratch(cache, table, keep):
-    n = lib.teeny_cache8_evict_scratch_bytes(cache.shape, table.n, keep)
-    return torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+    """Scratch for evictions of this many entries down to ``keep`` tokens.  Calls that follow one another in a stream may share it."""
+    return torch.empty(lib.teeny_cache8_evict_scratch_bytes(cache._shape_at, table.n, keep), dtype=torch.uint8, device=cache.device)
 
 
 def cache8_evict(cache, table, keep, recent, kept=None, scratch=None):
     """Thins out the slots of the table's entries, (slot, live tokens, 0, 0) each: every kv head keeps its last ``recent`` tokens and the ones with
     the largest weights of the others, ``keep`` in all, moved to the front in their order.  The slot's next token goes to position min(live
     tokens, keep).  Returns the kept tokens' indices before, int32 [entries, kv_heads, keep], -1 behind the last."""
-    s = cache.shape
     if cache.weights is None:
         raise ValueError("this cache has no weights")
-    shape = (table.n, s.kv_heads, keep)
+    shape = (table.n, cache.kv_heads, keep)
     if kept is None:
         kept = torch.empty(shape, dtype=torch.int32, device=cache.device)
-    elif _req(kept, torch.int32, "kept").shape != shape or not kept.is_contiguous():
-        raise ValueError(f"kept must be a contiguous {shape}")
+    elif kept.dtype != torch.int32 or kept.shape != shape or not kept.is_contiguous():
+        raise ValueError(f"kept must be a contiguous int32 {shape}")
     if scratch is None:
         scratch = cache8_evict_scratch(cache, table, keep)
-    _on(cache.device, table=table.seqs, kept=kept, scratch=scratch)
-    check(lib.teeny_cache8_evict(s, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(cache.weights), keep, recent,
-                                 _ptr(kept), _ptr(scratch), scratch.numel() if scratch is not None else 0, _ptr(table.seqs), table.host,
-                                 table.n, _stream()), "cache8_evict")
+    _on(cache, table.seqs, kept, scratch)
+    check(lib.teeny_cache8_evict(*cache._at, cache._weights_at, keep, recent, kept.data_ptr(), scratch.data_ptr(), scratch.numel(), *table._at[:3],
+                                 _stream()), "cache8_evict")
     return kept

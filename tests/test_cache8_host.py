@@ -25,17 +25,17 @@ def host(*entries):
 
 def append(lib, sh, table=None, n=1, rows=8, longest=8, k=P, kn=P, ldk=None, ks=P):
     ld = sh.kv_heads * sh.dim if ldk is None else ldk
-    return lib.lib.teeny_cache8_append(0, sh, k, P, ks, P, None, kn, ld, P, sh.kv_heads * sh.vdim, rows, P, table, n, longest, None)
+    return lib.lib.teeny_cache8_append(0, C.addressof(sh), k, P, ks, P, None, kn, ld, P, sh.kv_heads * sh.vdim, rows, P, table, n, longest, None)
 
 
 def attention(lib, sh, table=None, n=1, rows=8, longest=8, heads=4, q=P, out=P, weights=None, softcap=0.0, scratch=P, size=1 << 40, gate=None, ldg=0, ldq=None,
               scale=0.1):
-    return lib.lib.teeny_cache8_attention(0, sh, P, P, P, P, weights, 0.5, q, heads * sh.dim if ldq is None else ldq, out, heads * sh.vdim, rows, heads,
+    return lib.lib.teeny_cache8_attention(0, C.addressof(sh), P, P, P, P, weights, 0.5, q, heads * sh.dim if ldq is None else ldq, out, heads * sh.vdim, rows, heads,
                                           scale, softcap, None, gate, ldg, None, scratch, size, P, table, n, longest, None)
 
 
 def evict(lib, sh, table=None, n=1, keep=10, recent=2, weights=P, kept=P, scratch=P, size=1 << 40):
-    return lib.lib.teeny_cache8_evict(sh, P, P, P, P, weights, keep, recent, kept, scratch, size, P, table, n, None)
+    return lib.lib.teeny_cache8_evict(C.addressof(sh), P, P, P, P, weights, keep, recent, kept, scratch, size, P, table, n, None)
 
 
 @pytest.mark.parametrize("change", [dict(slots=0), dict(heads=0), dict(cap=0), dict(dim=0), dict(dim=72), dict(dim=144), dict(vdim=8), dict(vdim=256),
@@ -43,7 +43,7 @@ def evict(lib, sh, table=None, n=1, keep=10, recent=2, weights=P, kept=P, scratc
 def test_shapes(lib, change):
     sh = shape(lib, **change)
     assert append(lib, sh) == BAD and attention(lib, sh, heads=4) == BAD and evict(lib, sh) == BAD
-    assert lib.lib.teeny_cache8_attention_scratch_bytes(sh, 0, 4, 8, 1, 8, 1) == 0 and lib.lib.teeny_cache8_evict_scratch_bytes(sh, 1, 10) == 0
+    assert lib.lib.teeny_cache8_attention_scratch_bytes(C.addressof(sh), 0, 4, 8, 1, 8, 1) == 0 and lib.lib.teeny_cache8_evict_scratch_bytes(C.addressof(sh), 1, 10) == 0
 
 
 @pytest.mark.parametrize("table", [[(4, 0, 0, 1)], [(-1, 0, 0, 1)], [(0, -1, 0, 1)], [(0, 100, 0, 1)], [(0, 98, 0, 3)], [(0, 0, 8, 1)], [(0, 0, 6, 3)],
