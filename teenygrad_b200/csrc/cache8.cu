@@ -20,59 +20,124 @@ __device__ __forceinline__ int scale_exponent(float amax) {
   return max(-126, static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0));
 }
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<unsigned>(k + 127) << 23); }  // -126 <= k <= 127
+__device__ __forceinline__ int exponent_of(float scale) { return static_cast<int>(__float_as_uint(scale) >> 23) - 127; }
 
-__device__ __forceinline__ float finite_abs(float x) {
-  const float m = fabsf(x);
-  return m < INFINITY ? m : 0.0f;
+__device__ __forceinline__ float decode(unsigned code) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3);
+  return __half2float(*reinterpret_cast<const __half*>(&h));
 }
-// four numbers, none of them beyond 448 after scaling, as E4M3 (round to nearest even; what is not finite becomes NaN)
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
-  auto one = [&](float x) { return fabsf(x) < INFINITY ? x * inv : __uint_as_float(0x7fffffffu); };
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(one(a), one(b)), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(one(c), one(d)), __NV_SATFINITE, __NV_E4M3);
-  return lo | hi << 16;
-}
-__device__ __forceinline__ float4 decode4(uint32_t w) {
-  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
-  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ uint4 rescale16(uint4 w, float factor) {
-  uint32_t r[4] = {w.x, w.y, w.z, w.w};
+// 16 codes at another scale, 2^j times smaller: in f16 the products are exact down to 2^-24, far below the least code.
+__device__ __forceinline__ uint4 rescale16(uint4 v, int j) {
+  if (j == 0) return v;
+  uint32_t r[4] = {v.x, v.y, v.z, v.w};
+  // (a code can grow by up to 2^17: two factors)
+  const int j0 = max(-24, min(j, 14)), j1 = max(0, min(j - j0, 14));
+  const __half2 f0 = __float2half2_rn(pow2(j0)), f1 = __float2half2_rn(pow2(j1));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float4 x = decode4(r[i]);
-    r[i] = encode4(x.x, x.y, x.z, x.w, factor);
+    uint32_t out = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(r[i] >> (16 * h) & 0xffffu), __NV_E4M3);
+      const __half2 y = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&x), f0), f1);
+      out |= static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y), __NV_SATFINITE, __NV_E4M3)) << (16 * h);
+    }
+    r[i] = out;
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
-// 16 numbers of a row; vec: 16-byte pieces
-__device__ __forceinline__ void load16(const bf16* p, bool vec, float (&x)[16]) {
-  if (vec) {
+// Largest of 16 codes' magnitudes as a code (they are ordered like their numbers), NaN left out
+__device__ __forceinline__ unsigned top_code(const uint4& v) {
+  const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+  unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 w = reinterpret_cast<const uint4*>(p)[i];
-      const uint32_t r[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { x[8 * i + 2 * e] = bf16_lo(r[e]); x[8 * i + 2 * e + 1] = bf16_hi(r[e]); }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = __bfloat162float(p[e]);
+  for (int i = 0; i < 4; ++i) {
+    unsigned m = r[i] & 0x7f7f7f7fu;
+    const unsigned nan = (m + 0x01010101u) & 0x80808080u;
+    if (nan) m &= ~((nan >> 7) * 0x7fu);
+    top = __vmaxu4(top, m);
   }
+  return max(max(top & 0xffu, top >> 8 & 0xffu), max(top >> 16 & 0xffu, top >> 24));
 }
-__device__ __forceinline__ void load16(const float* p, bool vec, float (&x)[16]) {
-  if (vec) {
+
+// 16 numbers of a row as they are in memory (vec: in 16-byte pieces), their largest magnitude, and their codes
+template <typename T>
+struct Sixteen;
+template <>
+struct Sixteen<bf16> {
+  uint32_t w[8];
+  __device__ __forceinline__ void load(const bf16* p, bool vec) {
+    if (vec) {
+      const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
+    }
+  }
+  __device__ __forceinline__ float top() const {  // (of a NaN and a number the number)
+    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ __forceinline__ float2 two(int i) const { return make_float2(bf16_lo(w[i]), bf16_hi(w[i])); }
+};
+template <>
+struct Sixteen<float> {
+  float2 x[8];
+  __device__ __forceinline__ void load(const float* p, bool vec) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 w = reinterpret_cast<const float4*>(p)[i];
-      x[4 * i] = w.x; x[4 * i + 1] = w.y; x[4 * i + 2] = w.z; x[4 * i + 3] = w.w;
+      if (vec) {
+        const float4 v = reinterpret_cast<const float4*>(p)[i];
+        x[2 * i] = make_float2(v.x, v.y);
+        x[2 * i + 1] = make_float2(v.z, v.w);
+      } else {
+        x[2 * i] = make_float2(p[4 * i], p[4 * i + 1]);
+        x[2 * i + 1] = make_float2(p[4 * i + 2], p[4 * i + 3]);
+      }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = p[e];
   }
+  __device__ __forceinline__ float top() const {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+    return m;
+  }
+  __device__ __forceinline__ float2 two(int i) const { return x[i]; }
+};
+template <typename T>
+__device__ __forceinline__ float top_finite(const Sixteen<T>& x) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(x.two(i).x), b = fabsf(x.two(i).y);
+    m = fmaxf(m, fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f));
+  }
+  return m;
+}
+// none of them beyond 448 after scaling (round to nearest even); infinite: some are not finite, and become NaN
+template <typename T>
+__device__ __forceinline__ uint4 encode16(const Sixteen<T>& x, float inv, bool infinite) {
+  uint32_t r[4];
+  const float2 f = make_float2(inv, inv);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float2 y = __fmul2_rn(x.two(2 * i + h), f);
+      if (infinite) {
+        if (!(fabsf(y.x) < INFINITY)) y.x = __uint_as_float(0x7fffffffu);
+        if (!(fabsf(y.y) < INFINITY)) y.y = __uint_as_float(0x7fffffffu);
+      }
+      out |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3)) << (16 * h);
+    }
+    r[i] = out;
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 __device__ __forceinline__ float block_max(float v, float* sh) {
   v = warp_max(v);
@@ -80,52 +145,63 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
   __syncthreads();
   float m = sh[0];
   for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) m = fmaxf(m, sh[w]);
+  __syncthreads();
   return m;
 }
 
 // One CTA for the new tokens of one entry in one block of the cache: blockIdx = (block counted from the entry's first, 2 * head + (values), entry).
-template <typename T>
+// A thread holds the 16-element pieces that it reads (up to NCH) until the scale is known: each number is read once.
+template <typename T, int NCH>
 __global__ void __launch_bounds__(kThreads) cache8_append_kernel(const Cache8 c, const Cache8Append a, const SeqDesc* seqs, int max_len, int vec) {
   __shared__ float sh[kThreads / 32];
   pdl_wait();
   const SeqDesc sq = seqs[blockIdx.z];
   if (!cache8_fits(sq, c, a.rows, max_len)) return;
-  const int head = blockIdx.y >> 1, of_v = blockIdx.y & 1, d = of_v ? c.V : c.D, per = d / 16;
+  const int head = blockIdx.y >> 1, of_v = blockIdx.y & 1, d = of_v ? c.V : c.D, per = d / 16, step = blockDim.x;
   const int b = sq.pos / c.B + blockIdx.x, begin = max(sq.pos, b * c.B), end = min(sq.pos + sq.len, (b + 1) * c.B);
   if (begin >= end) return;
-  const size_t sh_row = static_cast<size_t>(sq.slot) * c.H + head;
-  uint8_t* codes = (of_v ? c.v : c.k) + sh_row * c.cap * d;
-  float* scales = (of_v ? c.vs : c.ks) + sh_row * c.blocks;
+  const size_t row = static_cast<size_t>(sq.slot) * c.H + head;
+  uint8_t* codes = (of_v ? c.v : c.k) + row * c.cap * d;
+  float* scales = (of_v ? c.vs : c.ks) + row * c.blocks;
   const long long ld = of_v ? a.ldv : a.ldk;
   const T* src = static_cast<const T*>(of_v ? a.v : a.k) + (sq.row0 + begin - sq.pos) * ld + head * d;
   const bool older = begin > b * c.B;
   const float was = older ? scales[b] : 0.0f;
   const int chunks = (end - begin) * per;
+  Sixteen<T> x[NCH];
   float amax = 0.0f;
-  for (int i = threadIdx.x; i < chunks; i += kThreads) {
-    float x[16];
-    load16(src + i / per * ld + i % per * 16, vec, x);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_abs(x[e]));
+  for (int m = 0; m < NCH; ++m) {
+    const int i = threadIdx.x + m * step;
+    if (i < chunks) x[m].load(src + i / per * ld + i % per * 16, vec);
   }
-  amax = block_max(amax, sh);
-  const float fresh = pow2(scale_exponent(amax)), scale = older ? fmaxf(fresh, was) : fresh;
-  const float inv = pow2(127 - static_cast<int>(__float_as_uint(scale) >> 23));
-  for (int i = threadIdx.x; i < chunks; i += kThreads) {
-    float x[16];
-    load16(src + i / per * ld + i % per * 16, vec, x);
-    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = encode4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3], inv);
-    reinterpret_cast<uint4*>(codes + static_cast<size_t>(begin) * d)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int m = 0; m < NCH; ++m)
+    if (threadIdx.x + m * step < chunks) amax = fmaxf(amax, x[m].top());
+  amax = block_max(amax, sh);
+  const bool infinite = amax == INFINITY;
+  if (infinite) {  // (the same for the CTA)
+    amax = 0.0f;
+#pragma unroll
+    for (int m = 0; m < NCH; ++m)
+      if (threadIdx.x + m * step < chunks) amax = fmaxf(amax, top_finite(x[m]));
+    amax = block_max(amax, sh);
+  }
+  const float fresh = pow2(scale_exponent(amax)), scale = older ? fmaxf(fresh, was) : fresh;
+  const int k = exponent_of(scale);
+#pragma unroll
+  for (int m = 0; m < NCH; ++m) {
+    const int i = threadIdx.x + m * step;
+    if (i < chunks) reinterpret_cast<uint4*>(codes + static_cast<size_t>(begin) * d)[i] = encode16(x[m], pow2(-k), infinite);
   }
   if (older && scale != was) {
     uint4* old = reinterpret_cast<uint4*>(codes + static_cast<size_t>(b) * c.B * d);
-    for (int i = threadIdx.x; i < (begin - b * c.B) * per; i += kThreads) old[i] = rescale16(old[i], was * inv);
+    const int j = exponent_of(was) - k;
+    for (int i = threadIdx.x; i < (begin - b * c.B) * per; i += step) old[i] = rescale16(old[i], j);
   }
   if (threadIdx.x == 0) scales[b] = scale;
   if (!of_v && c.w)
-    for (int t = begin + threadIdx.x; t < end; t += kThreads) c.w[sh_row * c.cap + t] = 0.0f;
+    for (int t = begin + threadIdx.x; t < end; t += step) c.w[row * c.cap + t] = 0.0f;
 }
 
 // ---- eviction ----
@@ -258,39 +334,33 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
   float* w = c.w + row * c.cap;
   const int* index = kept + (static_cast<size_t>(e) * c.H + head) * keep + t0;
   uint4 v[kMost];
-  float s[kMost], wt = 0.0f;
-  int from[kMost];
+  int from[kMost], tok[kMost], ks[kMost];  // place before, token of the piece, exponent of the scale
+  float wt = 0.0f;
 #pragma unroll
   for (int m = 0; m < kMost; ++m) {
     const int i = threadIdx.x + m * kMoveThreads;
-    from[m] = i < chunks ? index[i / per] : 0;
+    tok[m] = per == 8 ? i >> 3 : i / per;
+    from[m] = i < chunks ? index[tok[m]] : 0;
   }
 #pragma unroll
   for (int m = 0; m < kMost; ++m) {
     const int i = threadIdx.x + m * kMoveThreads;
-    s[m] = 0.0f;
+    ks[m] = -126;
     v[m] = make_uint4(0u, 0u, 0u, 0u);
     if (i >= chunks) continue;
-    v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + i % per * 16);
-    s[m] = scales[from[m] / c.B];
+    v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + (i - tok[m] * per) * 16);
+    ks[m] = exponent_of(scales[from[m] / c.B]);
   }
   if (!of_v && threadIdx.x < tokens) wt = w[index[threadIdx.x]];
 #pragma unroll
   for (int m = 0; m < kMost; ++m) {
     const int i = threadIdx.x + m * kMoveThreads;
-    const uint32_t r[4] = {v[m].x, v[m].y, v[m].z, v[m].w};
-    float amax = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float4 y = decode4(r[k]);
-      amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
-    }
-    const unsigned bits = __float_as_uint(amax * s[m]);  // (>= 0: ordered like its bits)
+    const unsigned bits = __float_as_uint(decode(top_code(v[m])) * pow2(ks[m]));  // (>= 0: ordered like its bits)
     if (per == 8) {  // a warp's four tokens lie in one block
       const unsigned most = __reduce_max_sync(0xffffffffu, bits);
-      if ((threadIdx.x & 31) == 0 && i < chunks) atomicMax(&top[i / 8 / c.B], most);
+      if ((threadIdx.x & 31) == 0 && i < chunks) atomicMax(&top[tok[m] / c.B], most);
     } else if (i < chunks) {
-      atomicMax(&top[i / per / c.B], bits);
+      atomicMax(&top[tok[m] / c.B], bits);
     }
   }
   __syncthreads();  // (every load of the CTA has arrived)
@@ -326,9 +396,9 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
   for (int m = 0; m < kMost; ++m) {
     const int i = threadIdx.x + m * kMoveThreads;
     if (i >= chunks) continue;
-    const int t = i / per, k = scale_exponent(__uint_as_float(top[t / c.B]));
-    if (from[m] == t0 + t && s[m] == pow2(k)) continue;
-    reinterpret_cast<uint4*>(codes + static_cast<size_t>(t0) * d)[i] = rescale16(v[m], s[m] * pow2(-k));
+    const int k = scale_exponent(__uint_as_float(top[tok[m] / c.B]));
+    if (from[m] == t0 + tok[m] && ks[m] == k) continue;
+    reinterpret_cast<uint4*>(codes + static_cast<size_t>(t0) * d)[i] = rescale16(v[m], ks[m] - k);
   }
   if (threadIdx.x < (tokens + c.B - 1) / c.B) scales[t0 / c.B + threadIdx.x] = pow2(scale_exponent(__uint_as_float(top[threadIdx.x])));
   if (!of_v && threadIdx.x < tokens) w[t0 + threadIdx.x] = wt;
@@ -342,8 +412,12 @@ int cache8_append(const Cache8& c, const Cache8Append& a, const SeqDesc* seqs, i
                            static_cast<uintptr_t>(a.ldv * size);
   const int vec = (rows16 & 15) == 0;
   const dim3 grid((max_len + c.B - 2) / c.B + 1, 2 * c.H, n_seqs);
-  if (a.f32) launch_kernel(cache8_append_kernel<float>, grid, dim3(kThreads), 0, st, 1, c, a, seqs, max_len, vec);
-  else launch_kernel(cache8_append_kernel<bf16>, grid, dim3(kThreads), 0, st, 1, c, a, seqs, max_len, vec);
+  // pieces of a block, and as many threads as leave each a few of them
+  const int most = (max_len < c.B ? max_len : c.B) * ((c.D > c.V ? c.D : c.V) / 16);
+  auto go = [&](auto kernel, int threads) { launch_kernel(kernel, grid, dim3(threads), 0, st, 1, c, a, seqs, max_len, vec); };
+  if (most <= 64) a.f32 ? go(cache8_append_kernel<float, 1>, 64) : go(cache8_append_kernel<bf16, 1>, 64);
+  else if (most <= 512) a.f32 ? go(cache8_append_kernel<float, 2>, 256) : go(cache8_append_kernel<bf16, 2>, 256);
+  else a.f32 ? go(cache8_append_kernel<float, 4>, 256) : go(cache8_append_kernel<bf16, 4>, 256);
   return static_cast<int>(cudaGetLastError());
 }
 
