@@ -22,42 +22,36 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<unsigned>(k + 127) << 23); }  // -126 <= k <= 127
 __device__ __forceinline__ int exponent_of(float scale) { return static_cast<int>(__float_as_uint(scale) >> 23) - 127; }
 
-__device__ __forceinline__ float decode(unsigned code) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3);
-  return __half2float(*reinterpret_cast<const __half*>(&h));
-}
-// 16 codes at another scale, 2^j times smaller: in f16 the products are exact down to 2^-24, far below the least code.
+// 16 codes times 2^j: in f16 the products are exact down to 2^-24, far below the least code.
 __device__ __forceinline__ uint4 rescale16(uint4 v, int j) {
   if (j == 0) return v;
   uint32_t r[4] = {v.x, v.y, v.z, v.w};
-  // (a code can grow by up to 2^17: two factors)
-  const int j0 = max(-24, min(j, 14)), j1 = max(0, min(j - j0, 14));
-  const __half2 f0 = __float2half2_rn(pow2(j0)), f1 = __float2half2_rn(pow2(j1));
+  const bool far = j > 14;  // (a code can grow by up to 2^17: two factors)
+  const __half2 f0 = __float2half2_rn(pow2(max(-24, min(j, 14)))), f1 = __float2half2_rn(pow2(far ? min(j - 14, 14) : 0));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t out = 0;
+    uint32_t out[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(r[i] >> (16 * h) & 0xffffu), __NV_E4M3);
-      const __half2 y = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&x), f0), f1);
-      out |= static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y), __NV_SATFINITE, __NV_E4M3)) << (16 * h);
+      __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f0);
+      if (far) y = __hmul2(y, f1);
+      out[h] = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y), __NV_SATFINITE, __NV_E4M3);
     }
-    r[i] = out;
+    r[i] = __byte_perm(out[0], out[1], 0x5410);
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
-// Largest of 16 codes' magnitudes as a code (they are ordered like their numbers), NaN left out
-__device__ __forceinline__ unsigned top_code(const uint4& v) {
+// Largest magnitude of 16 codes, NaN left out
+__device__ __forceinline__ float top_of(const uint4& v) {
   const uint32_t r[4] = {v.x, v.y, v.z, v.w};
-  unsigned top = 0;
+  __half2 top = __float2half2_rn(0.0f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    unsigned m = r[i] & 0x7f7f7f7fu;
-    const unsigned nan = (m + 0x01010101u) & 0x80808080u;
-    if (nan) m &= ~((nan >> 7) * 0x7fu);
-    top = __vmaxu4(top, m);
+  for (int i = 0; i < 8; ++i) {
+    const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(r[i >> 1] >> (16 * (i & 1)) & 0xffffu), __NV_E4M3);
+    top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&x)));
   }
-  return max(max(top & 0xffu, top >> 8 & 0xffu), max(top >> 16 & 0xffu, top >> 24));
+  return fmaxf(__low2float(top), __high2float(top));
 }
 
 // 16 numbers of a row as they are in memory (vec: in 16-byte pieces), their largest magnitude, and their codes
@@ -158,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) cache8_append_kernel(const Cache8 c,
   const SeqDesc sq = seqs[blockIdx.z];
   if (!cache8_fits(sq, c, a.rows, max_len)) return;
   const int head = blockIdx.y >> 1, of_v = blockIdx.y & 1, d = of_v ? c.V : c.D, per = d / 16, step = blockDim.x;
-  const int b = sq.pos / c.B + blockIdx.x, begin = max(sq.pos, b * c.B), end = min(sq.pos + sq.len, (b + 1) * c.B);
+  const int b = (sq.pos >> c.shift) + blockIdx.x, begin = max(sq.pos, b * c.B), end = min(sq.pos + sq.len, (b + 1) * c.B);
   if (begin >= end) return;
   const size_t row = static_cast<size_t>(sq.slot) * c.H + head;
   uint8_t* codes = (of_v ? c.v : c.k) + row * c.cap * d;
@@ -173,7 +167,10 @@ __global__ void __launch_bounds__(kThreads) cache8_append_kernel(const Cache8 c,
 #pragma unroll
   for (int m = 0; m < NCH; ++m) {
     const int i = threadIdx.x + m * step;
-    if (i < chunks) x[m].load(src + i / per * ld + i % per * 16, vec);
+    if (i < chunks) {
+      const int t = per == 8 ? i >> 3 : i / per;
+      x[m].load(src + t * ld + (i - t * per) * 16, vec);
+    }
   }
 #pragma unroll
   for (int m = 0; m < NCH; ++m)
@@ -309,99 +306,128 @@ __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8
 
 // Kept tokens to the front, in place and in parallel: a piece is 128 places of a head's keys or values, whose tokens come from there or from behind.
 // So a piece must not be written before the pieces in front of it have been read, which may be from there.  Pieces are handed out in
-// their order: a CTA reads its tokens into registers, says so, and waits, before it writes, for those in front, which are running and wait for
-// nothing before they have said it.  Each byte is read once and written once; tokens that stay where and what they are are not written.
-__global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cache8 c, int keep, int n_seqs, const int* kept, const EvictScratch x, const SeqDesc* seqs, int* err) {
+// their order: a CTA reads its tokens into registers, says so, and waits, before it writes, for those in front; whoever has one of these either has
+// said so or is about to, waiting at most for pieces further in front.  Each byte is read once and written once; tokens that stay where and what
+// they are are not written.  A piece is a chain of dependent accesses (number, indices, tokens, flags, writes; 17000 clocks with a CTA for
+// each), so CTAs stay, and ask for the next piece and its indices while they work on one.
+__global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cache8 c, int keep, int n_seqs, unsigned pieces, const int* kept, const EvictScratch x,
+                                                                      const SeqDesc* seqs, int* err) {
   constexpr int kMost = kMove * kCache8Head / 16 / kMoveThreads;
-  __shared__ unsigned top[kMove / 16], sm_ticket;
+  __shared__ unsigned sm_top[2][kMove / 16], sm_ticket;
   __shared__ int sm_failed;
+  const int heads = 2 * c.H;
+  struct Piece { int number, who, head, of_v, t0, tokens; size_t row; } p{};
+  int from[kMost];  // where the tokens of this thread's 16-byte pieces are
+  auto width = [&]() { return p.of_v ? c.V : c.D; };
+  auto token_of = [&](int i, int per) { return per == 8 ? i >> 3 : i / per; };
+  auto take = [&](unsigned ticket) {  // the piece of a ticket, and its indices under way
+    p.number = static_cast<int>(ticket / (n_seqs * heads));
+    p.who = static_cast<int>(ticket % (n_seqs * heads));
+    const int e = p.who / heads;
+    p.head = p.who % heads >> 1;
+    p.of_v = p.who & 1;
+    p.t0 = p.number * kMove;
+    const SeqDesc sq = seqs[e];
+    p.tokens = 0;
+    if (sq.slot < 0 || sq.slot >= c.slots || sq.pos < 0 || sq.pos > c.cap) return;
+    p.tokens = max(0, min(kMove, min(sq.pos, keep) - p.t0));  // (compared with thread numbers, which have no sign)
+    p.row = static_cast<size_t>(sq.slot) * c.H + p.head;
+    const int per = width() / 16, chunks = p.tokens * per;
+    const int* index = kept + (static_cast<size_t>(e) * c.H + p.head) * keep + p.t0;
+#pragma unroll
+    for (int m = 0; m < kMost; ++m) {
+      const int i = threadIdx.x + m * kMoveThreads;
+      if (i < chunks) from[m] = index[token_of(i, per)];
+    }
+  };
   pdl_wait();
   if (threadIdx.x == 0) {
     sm_ticket = atomicAdd(x.ticket, 1u);
     sm_failed = 0;
   }
-  if (threadIdx.x < kMove / 16) top[threadIdx.x] = 0u;
+  if (threadIdx.x < 2 * (kMove / 16)) sm_top[threadIdx.x / (kMove / 16)][threadIdx.x % (kMove / 16)] = 0u;
   __syncthreads();
-  const int heads = 2 * c.H, piece = static_cast<int>(sm_ticket / (n_seqs * heads)), who = static_cast<int>(sm_ticket % (n_seqs * heads));
-  const int e = who / heads, head = who % heads >> 1, of_v = who & 1, d = of_v ? c.V : c.D, per = d / 16;
-  const SeqDesc sq = seqs[e];
-  if (sq.slot < 0 || sq.slot >= c.slots || sq.pos < 0 || sq.pos > c.cap) return;
-  const int t0 = piece * kMove, tokens = min(kMove, min(sq.pos, keep) - t0), chunks = tokens * per;
-  if (tokens <= 0) return;
-  const size_t row = static_cast<size_t>(sq.slot) * c.H + head;
-  uint8_t* codes = (of_v ? c.v : c.k) + row * c.cap * d;
-  float* scales = (of_v ? c.vs : c.ks) + row * c.blocks;
-  float* w = c.w + row * c.cap;
-  const int* index = kept + (static_cast<size_t>(e) * c.H + head) * keep + t0;
-  uint4 v[kMost];
-  int from[kMost], tok[kMost], ks[kMost];  // place before, token of the piece, exponent of the scale
-  float wt = 0.0f;
+  unsigned ticket = sm_ticket;
+  if (ticket < pieces) take(ticket);
+  for (int round = 0; ticket < pieces; ++round) {
+    const Piece q = p;
+    const int d = width(), per = d / 16, chunks = q.tokens * per;
+    uint8_t* codes = (q.of_v ? c.v : c.k) + q.row * c.cap * d;
+    float* scales = (q.of_v ? c.vs : c.ks) + q.row * c.blocks;
+    float* w = c.w + q.row * c.cap;
+    unsigned* top = sm_top[round & 1];
+    uint4 v[kMost];
+    int ks[kMost];  // exponents of the tokens' scales; where they stay, kStays more
+    constexpr int kStays = 1024;
+    float wt = 0.0f;
 #pragma unroll
-  for (int m = 0; m < kMost; ++m) {
-    const int i = threadIdx.x + m * kMoveThreads;
-    tok[m] = per == 8 ? i >> 3 : i / per;
-    from[m] = i < chunks ? index[tok[m]] : 0;
-  }
-#pragma unroll
-  for (int m = 0; m < kMost; ++m) {
-    const int i = threadIdx.x + m * kMoveThreads;
-    ks[m] = -126;
-    v[m] = make_uint4(0u, 0u, 0u, 0u);
-    if (i >= chunks) continue;
-    v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + (i - tok[m] * per) * 16);
-    ks[m] = exponent_of(scales[from[m] / c.B]);
-  }
-  if (!of_v && threadIdx.x < tokens) wt = w[index[threadIdx.x]];
-#pragma unroll
-  for (int m = 0; m < kMost; ++m) {
-    const int i = threadIdx.x + m * kMoveThreads;
-    const unsigned bits = __float_as_uint(decode(top_code(v[m])) * pow2(ks[m]));  // (>= 0: ordered like its bits)
-    if (per == 8) {  // a warp's four tokens lie in one block
-      const unsigned most = __reduce_max_sync(0xffffffffu, bits);
-      if ((threadIdx.x & 31) == 0 && i < chunks) atomicMax(&top[tok[m] / c.B], most);
-    } else if (i < chunks) {
-      atomicMax(&top[tok[m] / c.B], bits);
+    for (int m = 0; m < kMost; ++m) {
+      const int i = threadIdx.x + m * kMoveThreads, t = token_of(i, per);
+      ks[m] = -126;
+      v[m] = make_uint4(0u, 0u, 0u, 0u);
+      if (i >= chunks) continue;
+      v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + (i - t * per) * 16);
+      ks[m] = exponent_of(scales[from[m] >> c.shift]) + (from[m] == q.t0 + t ? kStays : 0);
     }
-  }
-  __syncthreads();  // (every load of the CTA has arrived)
-  unsigned* flags = x.loaded + static_cast<size_t>(who);
-  const size_t stride = static_cast<size_t>(n_seqs) * heads;
-  if (threadIdx.x == 0) {
-    __threadfence();
-    asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(flags + piece * stride) : "memory");
-  }
-  if (threadIdx.x < 32) {
-    bool fine = true;
-    uint64_t since = 0;
-    for (int p = threadIdx.x; p < piece && fine; p += 32)
-      for (unsigned it = 0;; ++it) {
-        unsigned there;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(flags + p * stride) : "memory");
-        if (there) break;
-        if ((it & 63) == 63) {
-          const uint64_t now = global_timer_ns();
-          if (since == 0) since = now;
-          if (*reinterpret_cast<volatile int*>(err) != 0 || now - since > kWaitLimitNs) {
-            atomicCAS(err, 0, DEVERR_CACHE_MOVE);
-            fine = false;
-            break;
+    if (!q.of_v && static_cast<int>(threadIdx.x) < q.tokens) wt = w[kept[(static_cast<size_t>(q.who / heads) * c.H + q.head) * keep + q.t0 + threadIdx.x]];
+    unsigned next = 0;
+    if (threadIdx.x == 0) next = atomicAdd(x.ticket, 1u);
+#pragma unroll
+    for (int m = 0; m < kMost; ++m) {
+      const int i = threadIdx.x + m * kMoveThreads, block = token_of(i, per) >> c.shift;
+      const unsigned bits = __float_as_uint(top_of(v[m]) * pow2(ks[m] > 512 ? ks[m] - kStays : ks[m]));  // (>= 0: ordered like its bits)
+      if (per == 8) {  // a warp's four tokens lie in one block
+        const unsigned most = __reduce_max_sync(0xffffffffu, bits);
+        if ((threadIdx.x & 31) == 0 && i < chunks) atomicMax(&top[block], most);
+      } else if (i < chunks) {
+        atomicMax(&top[block], bits);
+      }
+    }
+    if (threadIdx.x == 0) sm_ticket = next;
+    asm volatile("" ::"f"(wt) : "memory");
+    __syncthreads();  // every load of the CTA has arrived: what they gave has been used
+    unsigned* flags = x.loaded + q.who;
+    const size_t stride = static_cast<size_t>(n_seqs) * heads;
+    // (nothing written is told by this flag, only that the reads are done: no fence, which would wait for the last piece's stores)
+    if (threadIdx.x == 0 && q.tokens > 0) asm volatile("st.relaxed.gpu.global.u32 [%0], 1;" ::"l"(flags + q.number * stride) : "memory");
+    ticket = sm_ticket;
+    if (ticket < pieces) take(ticket);
+    if (threadIdx.x < 32 && q.tokens > 0) {
+      bool fine = true;
+      uint64_t since = 0;
+      for (int f = threadIdx.x; f < q.number && fine; f += 32)
+        for (unsigned it = 0;; ++it) {
+          unsigned there;
+          asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(flags + f * stride) : "memory");
+          if (there) break;
+          if ((it & 63) == 63) {
+            const uint64_t now = global_timer_ns();
+            if (since == 0) since = now;
+            if (*reinterpret_cast<volatile int*>(err) != 0 || now - since > kWaitLimitNs) {
+              atomicCAS(err, 0, DEVERR_CACHE_MOVE);
+              fine = false;
+              break;
+            }
           }
         }
-      }
-    if (!fine) sm_failed = 1;
-  }
-  __syncthreads();
-  if (sm_failed) return;
+      if (!fine) sm_failed = 1;
+    }
+    __syncthreads();
+    if (sm_failed) return;
 #pragma unroll
-  for (int m = 0; m < kMost; ++m) {
-    const int i = threadIdx.x + m * kMoveThreads;
-    if (i >= chunks) continue;
-    const int k = scale_exponent(__uint_as_float(top[tok[m] / c.B]));
-    if (from[m] == t0 + tok[m] && ks[m] == k) continue;
-    reinterpret_cast<uint4*>(codes + static_cast<size_t>(t0) * d)[i] = rescale16(v[m], ks[m] - k);
+    for (int m = 0; m < kMost; ++m) {
+      const int i = threadIdx.x + m * kMoveThreads;
+      if (i >= chunks) continue;
+      const int k = scale_exponent(__uint_as_float(top[token_of(i, per) >> c.shift]));
+      if (ks[m] == k + kStays) continue;
+      reinterpret_cast<uint4*>(codes + static_cast<size_t>(q.t0) * d)[i] = rescale16(v[m], (ks[m] > 512 ? ks[m] - kStays : ks[m]) - k);
+    }
+    if (static_cast<int>(threadIdx.x) < (q.tokens + c.B - 1) >> c.shift) scales[(q.t0 >> c.shift) + threadIdx.x] = pow2(scale_exponent(__uint_as_float(top[threadIdx.x])));
+    if (!q.of_v && static_cast<int>(threadIdx.x) < q.tokens) w[q.t0 + threadIdx.x] = wt;
+    // the other round's maxima: everyone has passed two barriers since they were read
+    if (threadIdx.x < kMove / 16) sm_top[(round & 1) ^ 1][threadIdx.x] = 0u;
+    __syncthreads();
   }
-  if (threadIdx.x < (tokens + c.B - 1) / c.B) scales[t0 / c.B + threadIdx.x] = pow2(scale_exponent(__uint_as_float(top[threadIdx.x])));
-  if (!of_v && threadIdx.x < tokens) w[t0 + threadIdx.x] = wt;
 }
 
 }  // namespace
@@ -438,7 +464,9 @@ int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch
   else select(cache8_select_kernel<0>);
   const bool pdl = pdl_enabled();
   pdl_set_enabled(true);
-  launch_kernel(cache8_move_kernel, dim3(static_cast<unsigned>(pieces)), dim3(kMoveThreads), 0, st, 1, c, keep, n_seqs, static_cast<const int*>(kept), x, seqs, err);
+  const long long stay = 4ll * sm_count();
+  launch_kernel(cache8_move_kernel, dim3(static_cast<unsigned>(pieces < stay ? pieces : stay)), dim3(kMoveThreads), 0, st, 1, c, keep, n_seqs,
+                static_cast<unsigned>(pieces), static_cast<const int*>(kept), x, seqs, err);
   pdl_set_enabled(pdl);
   return static_cast<int>(cudaGetLastError());
 }
@@ -451,7 +479,8 @@ bool cache_of(const teeny_cache8_shape* s, Cache8* c) {
       (s->block != 16 && s->block != 32 && s->block != 64 && s->block != 128))
     return false;
   *c = Cache8{nullptr, nullptr, nullptr, nullptr, nullptr, s->slots, s->kv_heads, s->max_cached, s->dim, s->vdim, s->block,
-              (s->max_cached + s->block - 1) / s->block};
+              (s->max_cached + s->block - 1) / s->block,
+              s->block == 16 ? 4 : s->block == 32 ? 5 : s->block == 64 ? 6 : 7};
   return true;
 }
 int bind_cache(Cache8* c, void* k, void* v, float* ks, float* vs, float* w) {

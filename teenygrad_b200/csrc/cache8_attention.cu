@@ -330,7 +330,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     if (lane < 4) {  // scales of the slice's two groups of 16 keys; blocks behind the last key may hold anything: zero is written
       const int key = key0 + 16 * (lane & 1);
       const uint32_t bytes = key < load.limit ? 4 : 0;
-      const float* src = (lane < 2 ? s.c.ks : s.c.vs) + (static_cast<size_t>(load.sq.slot) * s.c.H + load.hk) * s.c.blocks + (bytes ? key / s.c.B : 0);
+      const float* src = (lane < 2 ? s.c.ks : s.c.vs) + (static_cast<size_t>(load.sq.slot) * s.c.H + load.hk) * s.c.blocks + (bytes ? key >> s.c.shift : 0);
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n\tcp.async.mbarrier.arrive.noinc.shared::cta.b64 [%3];"
                    ::"r"(base + V::kScales + st * 16 + lane * 4), "l"(src), "r"(bytes), "r"(bar) : "memory");
     }
@@ -756,8 +756,8 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
           widen(w.w, ka[u][4 * h + 3][half], ka[u][4 * h + 3][2 + half]);
         }
       }
-    ks[0] = s.c.ks[head * s.c.blocks + kb / s.c.B];
-    ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + (kb + 16) / s.c.B] : 0.0f;
+    ks[0] = s.c.ks[head * s.c.blocks + (kb >> s.c.shift)];
+    ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + ((kb + 16) >> s.c.shift)] : 0.0f;
     float sum[4] = {};
     const int rows = sq.len * s.G;
     for (int r0 = max(0, kb - sq.pos) * s.G / 8 * 8; r0 < rows; r0 += 8) {

@@ -54,12 +54,12 @@ __global__ void __launch_bounds__(256) cache8_widen_kernel(const Cache8 c, const
   const int chunks = kTile * per;
 #pragma unroll 4
   for (int i = threadIdx.x; i < chunks; i += 256) {
-    const int t = t0 + i / per;
+    const int t = t0 + (per == 8 ? i >> 3 : i / per);
     uint4 w = make_uint4(0u, 0u, 0u, 0u);
     float scale = 0.0f;
     if (t < live) {
       w = src[i];
-      scale = scales[t / c.B];
+      scale = scales[t >> c.shift];
     }
     if (of_v && t >= sq.pos) {
       uint32_t word[4] = {w.x, w.y, w.z, w.w};

@@ -510,7 +510,7 @@ int f32_to_bf16(const float* x, bf16* y, long long n, cudaStream_t st);
 struct Cache8 {
   uint8_t *k, *v;
   float *ks, *vs, *w;  // scales; weights or null
-  int slots, H, cap, D, V, B, blocks;  // B tokens a block, `blocks` of them a slot and head
+  int slots, H, cap, D, V, B, blocks, shift;  // B = 2^shift tokens a block, `blocks` of them a slot and head
 };
 constexpr int kCache8Head = 128;   // largest dim and vdim
 constexpr int kCache8Block = 128;  // largest block
