@@ -334,11 +334,9 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
     p.row = static_cast<size_t>(sq.slot) * c.H + p.head;
     const int per = width() / 16, chunks = p.tokens * per;
     const int* index = kept + (static_cast<size_t>(e) * c.H + p.head) * keep + p.t0;
+    if (chunks > 0)
 #pragma unroll
-    for (int m = 0; m < kMost; ++m) {
-      const int i = threadIdx.x + m * kMoveThreads;
-      if (i < chunks) from[m] = index[token_of(i, per)];
-    }
+      for (int m = 0; m < kMost; ++m) from[m] = index[token_of(min(static_cast<int>(threadIdx.x) + m * kMoveThreads, chunks - 1), per)];
   };
   pdl_wait();
   if (threadIdx.x == 0) {
@@ -360,26 +358,33 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
     int ks[kMost];  // exponents of the tokens' scales; where they stay, kStays more
     constexpr int kStays = 1024;
     float wt = 0.0f;
+    // (a thread without a 16-byte piece of its own reads the last one again: straight-line code, all loads at once)
+    if (q.tokens > 0) {
+      float sc[kMost];
 #pragma unroll
-    for (int m = 0; m < kMost; ++m) {
-      const int i = threadIdx.x + m * kMoveThreads, t = token_of(i, per);
-      ks[m] = -126;
-      v[m] = make_uint4(0u, 0u, 0u, 0u);
-      if (i >= chunks) continue;
-      v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + (i - t * per) * 16);
-      ks[m] = exponent_of(scales[from[m] >> c.shift]) + (from[m] == q.t0 + t ? kStays : 0);
+      for (int m = 0; m < kMost; ++m) {
+        const int i = min(static_cast<int>(threadIdx.x) + m * kMoveThreads, chunks - 1), t = token_of(i, per);
+        v[m] = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(from[m]) * d + (i - t * per) * 16);
+        sc[m] = scales[from[m] >> c.shift];
+      }
+#pragma unroll
+      for (int m = 0; m < kMost; ++m) {
+        const int i = min(static_cast<int>(threadIdx.x) + m * kMoveThreads, chunks - 1);
+        ks[m] = exponent_of(sc[m]) + (from[m] == q.t0 + token_of(i, per) ? kStays : 0);
+      }
     }
     if (!q.of_v && static_cast<int>(threadIdx.x) < q.tokens) wt = w[kept[(static_cast<size_t>(q.who / heads) * c.H + q.head) * keep + q.t0 + threadIdx.x]];
     unsigned next = 0;
     if (threadIdx.x == 0) next = atomicAdd(x.ticket, 1u);
 #pragma unroll
     for (int m = 0; m < kMost; ++m) {
-      const int i = threadIdx.x + m * kMoveThreads, block = token_of(i, per) >> c.shift;
+      if (q.tokens == 0) break;
+      const int i = min(static_cast<int>(threadIdx.x) + m * kMoveThreads, chunks - 1), block = token_of(i, per) >> c.shift;
       const unsigned bits = __float_as_uint(top_of(v[m]) * pow2(ks[m] > 512 ? ks[m] - kStays : ks[m]));  // (>= 0: ordered like its bits)
       if (per == 8) {  // a warp's four tokens lie in one block
         const unsigned most = __reduce_max_sync(0xffffffffu, bits);
-        if ((threadIdx.x & 31) == 0 && i < chunks) atomicMax(&top[block], most);
-      } else if (i < chunks) {
+        if ((threadIdx.x & 31) == 0) atomicMax(&top[block], most);
+      } else {
         atomicMax(&top[block], bits);
       }
     }
