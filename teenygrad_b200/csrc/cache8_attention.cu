@@ -9,11 +9,12 @@
 // registers.  Probabilities are f16 numbers times 2^14 (f32: two terms as well), so that a key is lost only 2^-38 below the row's
 // maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to the largest so far, the probabilities.
 //
-// The call is bound by reading the cache.  Every warp works alone: it takes slices of 32 keys of one sequence and head, and keeps the next ones in
-// flight itself (keys and values by TMA, their scales by 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry
-// after entry, head after head, row group after row group, each warp takes the same number of consecutive slices of all of them, whatever
-// the lengths.  A sequence that lies in several warps' shares leaves partial results in scratch, at most two for each warp; the last CTA to have
-// stored its part of a sequence adds them (a second kernel for it cost 4 to 10 us a call).  No warp waits for another CTA's.
+// The call is bound by reading the cache.  A CTA is four warps, each with slices of 32 keys of its own in flight (keys and values by TMA, their scales by
+// 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry after entry, head after head, row group after row
+// group, each CTA takes the same number of consecutive slices of all of them, whatever the lengths, and its warps take them in turn.  Where
+// a sequence ends or a share does, the warps' sums are added through shared memory.  A sequence that lies in several CTAs' shares leaves partial
+// results in scratch, at most two for each CTA; the last one to have stored its part adds them (a second kernel for it cost 4 to 10 us a
+// call; parts of single warps, four times as many, up to 14 us).  No CTA waits for another.
 #include <atomic>
 #include <type_traits>
 
@@ -31,21 +32,22 @@ constexpr int kBox = kSlice * kCache8Head;     // 4 KB: their keys, or their val
 constexpr int kStage = 2 * kBox;
 constexpr int kWarps = 4;                      // of a CTA
 
-// Variant of the kernel: RT tiles of eight query rows in TERMS f16 terms (bf16: 1, f32: 2).  Up to two column tiles fit 168 registers, with which an SM
-// has twelve warps; more take eight.
+// Variant of the kernel: RT tiles of eight query rows in TERMS f16 terms (bf16: 1, f32: 2).  One tile in one term fits 168 registers, with which an SM
+// has three CTAs; more take two.
 template <int RT_, int TERMS_>
 struct Variant {
-  static constexpr int RT = RT_, TERMS = TERMS_, NT = RT * TERMS, kRows = 8 * RT, kCtas = NT <= 2 ? 3 : 2, kStages = 2;
-  static constexpr bool kQRegs = NT <= 2;
+  static constexpr int RT = RT_, TERMS = TERMS_, NT = RT * TERMS, kRows = 8 * RT, kCtas = NT == 1 ? 3 : 2, kStages = 2;
   using T = typename std::conditional<TERMS == 2, float, bf16>::type;
-  // a warp's part of shared memory: stages, scales f32 [stages][4], queries uint2 [column tiles][8 steps][32 lanes] (up to two tiles: in registers), int [128]
-  // first NaN value of each dimension, barriers
-  static constexpr int kScales = kStages * kStage;
-  static constexpr int kNan = kScales + kStages * 16;
-  static constexpr int kBars = kNan + 128 * 4;
-  static constexpr int kQ = kBars + kStages * 8;
-  static constexpr int kWarpBytes = (kQ + (kQRegs ? 0 : NT * 8 * 32 * 8) + 1023) / 1024 * 1024;
-  static constexpr int kBytes = kWarps * kWarpBytes + 1024;
+  // shared memory: stages of the warps, scales f32 [warps][stages][4], int [128] first NaN value of each dimension, maximum and sum of a row [warps][rows][2],
+  // barriers, factors [rows], queries uint2 [row tiles][8 steps][32 lanes] (one row tile: in registers), sums on their way f32 [2][RT * 32][32 lanes]
+  static constexpr int kScales = kWarps * kStages * kStage;
+  static constexpr int kNan = kScales + kWarps * kStages * 16;
+  static constexpr int kML = kNan + 128 * 4;
+  static constexpr int kBars = kML + kWarps * kRows * 8;
+  static constexpr int kFactor = kBars + kWarps * kStages * 8;
+  static constexpr int kQ = kFactor + kRows * 4;
+  static constexpr int kMerge = kQ + (RT == 1 ? 0 : RT * 8 * 32 * 8);
+  static constexpr int kBytes = kMerge + 2 * RT * 32 * 32 * 4 + 1024;
   static_assert((kBytes + 1024) * kCtas <= 233472, "shared memory");
 };
 
@@ -95,13 +97,13 @@ struct Shared {  // what a call's kernels share
   const SeqDesc* seqs;
   int n_seqs, max_len, G;
   float scale_log2, two_over_cap, cap_l2;
-  float* part_o;   // [2 * warps][rows of a unit][128]
-  float* part_ml;  // [2 * warps][rows of a unit][2]
+  float* part_o;   // [2 * CTAs][rows of a unit][128]
+  float* part_ml;  // [2 * CTAs][rows of a unit][2]
   unsigned* arrivals;  // [entries][kv heads][max_groups]: CTAs that have stored their parts, zero between calls
   int max_groups;
   float* lse2;     // [rows][Hq], base 2, or null
   float* scores;   // [entries][Hq][cap] base 2, or null
-  int parts;       // warps of the main kernel
+  int parts;       // CTAs of the main kernel
   int vec_q, vec_o;
   int* err;
 };
@@ -117,12 +119,12 @@ __device__ __forceinline__ EntryShape entry_shape(const Shared& s, const SeqDesc
   e.all = e.slices * e.groups * s.c.H;
   return e;
 }
-// How the slices are shared: none of `parts` warps takes less than two, nor are there many more than 256 to a unit, whose parts have to be added
-// again.  The first `more` warps take one slice more than the others' `each`.
+// How the slices are shared: none of `parts` CTAs takes less than a slice for each warp, nor are there many more than 64 to a unit, whose parts have to
+// be added again.  The first `more` CTAs take one slice more than the others' `each`.
 struct Shares {
   int parts, each, more;
   __device__ __forceinline__ Shares(int most, int total, int units) {
-    const int least = max(2, total / 256 / units), all = (total + least - 1) / least;
+    const int least = max(kWarps, total / 64 / units), all = (total + least - 1) / least;
     parts = min(most, all);
     each = total / parts;
     more = total - parts * each;
@@ -169,38 +171,38 @@ __device__ __forceinline__ void store16(float* p, const float (&x)[16], bool vec
   }
 }
 
-// A query row, of which this lane (c = lane % 4) has the dimensions 32 c .. 32 c + 31, scaled, as f16 pairs: word w is dimensions 32 c + 2 w, + 1.
-// term[1]: the rest.  Returns the factor that takes scores back (base 2).
-template <typename T, int TERMS>
-__device__ __forceinline__ float split_row(const T* q, int dim, bool valid, bool vec, int c, float scale_log2, uint32_t (&term)[TERMS][16]) {
-  float x[32];
+// A query row, of which this lane (c = lane % 4) has the dimensions 32 c .. 32 c + 31.
+template <typename T>
+__device__ __forceinline__ void load_row(const T* q, int dim, bool valid, bool vec, int c, float (&x)[32]) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) x[i] = 0.0f;
-  if (valid) {
+  for (int h = 0; h < 2; ++h) {
+    const int d0 = 32 * c + 16 * h;
+    if (!valid || d0 >= dim) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int d0 = 32 * c + 16 * h;
-      if (d0 >= dim) continue;
-      if (vec && sizeof(T) == 2) {
+      for (int i = 0; i < 16; ++i) x[16 * h + i] = 0.0f;
+    } else if (vec && sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + d0 + 8 * i);
-          const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+      for (int i = 0; i < 2; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + d0 + 8 * i);
+        const uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { x[16 * h + 8 * i + 2 * e] = bf16_lo(r[e]); x[16 * h + 8 * i + 2 * e + 1] = bf16_hi(r[e]); }
-        }
-      } else if (vec) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + d0 + 4 * i);
-          x[16 * h + 4 * i] = w.x; x[16 * h + 4 * i + 1] = w.y; x[16 * h + 4 * i + 2] = w.z; x[16 * h + 4 * i + 3] = w.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[16 * h + i] = load_one(q + d0 + i);
+        for (int e = 0; e < 4; ++e) { x[16 * h + 8 * i + 2 * e] = bf16_lo(r[e]); x[16 * h + 8 * i + 2 * e + 1] = bf16_hi(r[e]); }
       }
+    } else if (vec) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + d0 + 4 * i);
+        x[16 * h + 4 * i] = w.x; x[16 * h + 4 * i + 1] = w.y; x[16 * h + 4 * i + 2] = w.z; x[16 * h + 4 * i + 3] = w.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[16 * h + i] = load_one(q + d0 + i);
     }
   }
+}
+// ... scaled, as f16 pairs: word w is dimensions 32 c + 2 w, + 1; term[1]: the rest.  Returns the factor that takes scores back (base 2).
+template <int TERMS>
+__device__ __forceinline__ float split_row(const float (&x)[32], float scale_log2, uint32_t (&term)[TERMS][16]) {
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
@@ -256,28 +258,27 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   constexpr int R = V::kRows, ST = V::kStages, RT = V::RT, TERMS = V::TERMS, NT = V::NT;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t offset = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw) + warp * V::kWarpBytes;
-  const uint32_t base = smem_u32(smem_raw) + offset;
-  uint8_t* gen = smem_raw + offset;
-  // parts that this CTA's warps have left: of their first and of their last unit (entry, head, row group, slices, first slice of all)
-  __shared__ struct Left { int begin, e, hk, rg, slices; } sm_left[2 * kWarps];
-  __shared__ int sm_c0[2 * kWarps], sm_c1[2 * kWarps];  // warps whose parts are to be added here (none: c1 < c0)
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t ring = base + warp * (ST * kStage), bars = base + V::kBars + warp * (ST * 8), scale_at = base + V::kScales + warp * (ST * 16);
+  // parts that this CTA has left: of its first and of its last unit (entry, head, row group, slices, first slice of all)
+  __shared__ struct Left { int begin, e, hk, rg, slices; } sm_left[2];
+  __shared__ int sm_c0[2], sm_c1[2];  // CTAs whose parts are to be added here (none: c1 < c0)
   if (lane == 0) {
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
-    for (int st = 0; st < ST; ++st) mbar_init(base + V::kBars + 8 * st, 1 + 4);
+    for (int st = 0; st < ST; ++st) mbar_init(bars + 8 * st, 1 + 4);
     mbar_fence_init();
-    sm_left[2 * warp].slices = sm_left[2 * warp + 1].slices = 0;
   }
+  if (threadIdx.x < 2) sm_left[threadIdx.x].slices = 0;
   __syncwarp();
   pdl_wait();
-  // ---- this warp's share ----
-  const int part = blockIdx.x * kWarps + warp;
-  Piece load;
-  int left = 0;  // slices of the share that are still to be loaded
-  int total = 0, units = 0, unit_begin = 0;
+  // ---- this CTA's share (each warp works it out) ----
+  const int part = blockIdx.x;
+  int total = 0, units = 0, mine = 0;  // mine: of this lane's entry among the first 32
   for (int e = lane; e < s.n_seqs; e += 32) {
     const EntryShape es = entry_shape(s, s.seqs[e], R);
+    if (e < 32) mine = es.all;
     total += es.all;
     units += es.groups * s.c.H;
   }
@@ -285,13 +286,13 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   units = warp_sum_int(units);
   if (total == 0) return;
   const Shares shares(s.parts, total, units);
-  if (static_cast<int>(blockIdx.x) * kWarps >= shares.parts) return;
-  if (part < shares.parts) {
-    const int t0 = shares.begin(part);
-    left = shares.begin(part + 1) - t0;
+  if (part >= shares.parts) return;
+  const int t0 = shares.begin(part), share = shares.begin(part + 1) - t0;
+  Piece p;
+  {
     int before = 0, at = 0, found = -1;
     for (int e0 = 0; found < 0; e0 += 32) {
-      const int mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
+      if (e0 > 0) mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
       int run = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -306,78 +307,95 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       found = e0 + src;
       at = t0 - __shfl_sync(0xffffffffu, end - mine, src);
     }
-    load.e = found;
-    load.sq = s.seqs[found];
-    const EntryShape es = entry_shape(s, load.sq, R);
-    load.slices = es.slices;
-    load.groups = es.groups;
+    p.e = found;
+    p.sq = s.seqs[found];
+    const EntryShape es = entry_shape(s, p.sq, R);
+    p.slices = es.slices;
+    p.groups = es.groups;
     const int unit = at / es.slices;
-    load.hk = unit / es.groups;
-    load.rg = unit - load.hk * es.groups;
-    load.first = true;
-    piece_range(s, load, R, at - unit * es.slices, left);
-    unit_begin = t0 - load.j;
+    p.hk = unit / es.groups;
+    p.rg = unit - p.hk * es.groups;
+    p.first = true;
+    piece_range(s, p, R, at - unit * es.slices, share);
   }
   pdl_trigger();
-  Piece p = load;
-  int rest = left;  // slices of the share that are still to be computed
-  int issued = 0, count = 0;
+  // Row g of the row tile that this warp makes ready (with one, every warp does): the first piece's is asked for in front of the cache's slices, behind
+  // which it would queue for 5000 clocks.
+  const int rt_mine = RT == 1 ? 0 : warp;
+  float raw[32];
+  auto ask_row = [&](const Piece& of) {
+    if (RT > 1 && warp >= RT) return;
+    const int r = of.rg * R + rt_mine * 8 + g, i = r / s.G, hq = of.hk * s.G + r - i * s.G;
+    const bool valid = i < of.sq.len;
+    load_row(static_cast<const T*>(s.a.q) + static_cast<size_t>(of.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, valid, s.vec_q, c, raw);
+  };
+  ask_row(p);
+  // the slices that this warp asks for: every fourth of the share
+  Piece load = p;
+  int load_rest = share, load_j = p.j + warp, load_at = warp, issued = 0, count = 0;
   auto load_next = [&]() {
-    if (left == 0) return;
-    if (load.j == load.end) next_piece(s, load, R, left);
-    const int st = issued & (ST - 1), key0 = load.j * kSlice;
-    const uint32_t bar = base + V::kBars + 8 * st;
+    if (load_at >= share) return;
+    while (load_j >= load.end) {
+      const int over = load_j - load.end;
+      load_rest -= load.end - load.j;
+      next_piece(s, load, R, load_rest);
+      load_j = over;
+    }
+    const int st = issued & (ST - 1), key0 = load_j * kSlice;
+    const uint32_t bar = bars + 8 * st;
     if (lane < 4) {  // scales of the slice's two groups of 16 keys; blocks behind the last key may hold anything: zero is written
       const int key = key0 + 16 * (lane & 1);
       const uint32_t bytes = key < load.limit ? 4 : 0;
       const float* src = (lane < 2 ? s.c.ks : s.c.vs) + (static_cast<size_t>(load.sq.slot) * s.c.H + load.hk) * s.c.blocks + (bytes ? key >> s.c.shift : 0);
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n\tcp.async.mbarrier.arrive.noinc.shared::cta.b64 [%3];"
-                   ::"r"(base + V::kScales + st * 16 + lane * 4), "l"(src), "r"(bytes), "r"(bar) : "memory");
+                   ::"r"(scale_at + st * 16 + lane * 4), "l"(src), "r"(bytes), "r"(bar) : "memory");
     }
     if (lane == 0) {
       mbar_expect_tx(bar, kStage);
-      tma_load_4d(base + st * kStage, &tmap_k, bar, 0, key0, load.hk, load.sq.slot);
-      tma_load_4d(base + st * kStage + kBox, &tmap_v, bar, 0, key0, load.hk, load.sq.slot);
+      tma_load_4d(ring + st * kStage, &tmap_k, bar, 0, key0, load.hk, load.sq.slot);
+      tma_load_4d(ring + st * kStage + kBox, &tmap_v, bar, 0, key0, load.hk, load.sq.slot);
     }
-    ++load.j;
+    load_j += kWarps;
+    load_at += kWarps;
     ++issued;
-    --left;
   };
 #pragma unroll
   for (int st = 0; st < ST; ++st) load_next();
 
   int* sm_nan = reinterpret_cast<int*>(gen + V::kNan);
+  float* sm_ml = reinterpret_cast<float*>(gen + V::kML);
+  float* sm_factor = reinterpret_cast<float*>(gen + V::kFactor);
   bool ok = true;
-  while (rest > 0) {
+  int done = 0, unit_begin = t0 - p.j;  // slices of the share in front of the piece; of the call in front of its unit
+  for (;;) {
     // ---- queries as B fragments: row g of tile rt is column g ----
     float factor[RT][2];      // of the rows 2c, 2c + 1, whose scores this lane gets
     int rows_limit[RT][2];    // keys that they see
-    uint2 q_regs[V::kQRegs ? NT * 8 : 1];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = p.rg * R + rt * 8 + g, i = r / s.G, hq = p.hk * s.G + r - i * s.G;
-      const bool valid = i < p.sq.len;
-      const T* q = static_cast<const T*>(s.a.q) + static_cast<size_t>(p.sq.row0 + (valid ? i : 0)) * s.a.ldq + static_cast<size_t>(hq) * s.c.D;
-      uint32_t term[TERMS][16];
-      const float f = split_row<T, TERMS>(q, s.c.D, valid, s.vec_q, c, s.scale_log2, term);
-      const int see = valid ? p.sq.pos + i + 1 : p.limit;
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        factor[rt][z] = __shfl_sync(0xffffffffu, f, (2 * c + z) * 4);
-        rows_limit[rt][z] = __shfl_sync(0xffffffffu, see, (2 * c + z) * 4);
-      }
+    uint2 q_regs[RT == 1 ? NT * 8 : 1];
+    uint32_t term[TERMS][16];
+    const float f = split_row<TERMS>(raw, s.scale_log2, term);
+    if (RT > 1 || p.sq.len > 1) __syncthreads();  // the piece before is finished with what is written here
+    if (p.sq.len > 1) sm_nan[threadIdx.x] = 0x7fffffff;
+    if (RT == 1) {
 #pragma unroll
       for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-        for (int step = 0; step < 8; ++step) {
-          const uint2 b = make_uint2(term[t][2 * step], term[t][2 * step + 1]);
-          if (V::kQRegs) q_regs[V::kQRegs ? (rt * TERMS + t) * 8 + step : 0] = b;
-          else reinterpret_cast<uint2*>(gen + V::kQ)[((rt * TERMS + t) * 8 + step) * 32 + lane] = b;
-        }
+        for (int step = 0; step < 8; ++step) q_regs[RT == 1 ? t * 8 + step : 0] = make_uint2(term[t][2 * step], term[t][2 * step + 1]);
+    } else if (warp < RT) {
+#pragma unroll
+      for (int step = 0; step < 8; ++step)
+        reinterpret_cast<uint2*>(gen + V::kQ)[(warp * 8 + step) * 32 + lane] = make_uint2(term[0][2 * step], term[0][2 * step + 1]);
+      if (c == 0) sm_factor[warp * 8 + g] = f;
     }
-    if (p.sq.len > 1)
-      for (int d = lane; d < 128; d += 32) sm_nan[d] = 0x7fffffff;
-    __syncwarp();
+    if (RT > 1 || p.sq.len > 1) __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const int i = (p.rg * R + rt * 8 + 2 * c + z) / s.G;
+        factor[rt][z] = RT == 1 ? __shfl_sync(0xffffffffu, f, (2 * c + z) * 4) : sm_factor[rt * 8 + 2 * c + z];
+        rows_limit[rt][z] = i < p.sq.len ? p.sq.pos + i + 1 : p.limit;
+      }
 
     // acc[tile][j]: dimensions 16 g + 2j (rows 2c, 2c + 1), 16 g + 2j + 1 (the same), in units of vref * 2^-14
     float m[RT][2], l[RT][2], acc[NT][8][4];
@@ -393,17 +411,14 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.0f;
-    rest -= p.end - p.j;
-    for (; p.j < p.end; ++p.j, ++count) {
-      const int st = count & (ST - 1), kb = p.j * kSlice;
-      if (!mbar_wait(base + V::kBars + 8 * st, count / ST & 1, s.err, DEVERR_ATTN_SOFTMAX)) {
-        // (nothing that this warp asked for may arrive after it has gone: the barriers are waited for once more, within their limit)
-        for (int i = count; i < issued; ++i) mbar_wait(base + V::kBars + 8 * (i & (ST - 1)), i / ST & 1, s.err, DEVERR_ATTN_SOFTMAX);
+    for (int sj = p.j + ((warp - done) & (kWarps - 1)); sj < p.end && ok; sj += kWarps, ++count) {
+      const int st = count & (ST - 1), kb = sj * kSlice;
+      if (!mbar_wait(bars + 8 * st, count / ST & 1, s.err, DEVERR_ATTN_SOFTMAX)) {
         ok = false;
         break;
       }
       if (kb < p.limit) {
-        const uint32_t kt = base + st * kStage + g * 128, vt = base + st * kStage + kBox, sc = base + V::kScales + st * 16;
+        const uint32_t kt = ring + st * kStage + g * 128, vt = ring + st * kStage + kBox, sc = scale_at + st * 16;
         const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + 8), vs1 = lds32(sc + 12);
         const bool masked = kb + kSlice > p.sq.pos + 1;
         // ---- scores: keys 16 u + g and 16 u + 8 + g of the slice are rows g and g + 8 of tile u; lane c reads the dimensions that it holds of the query ----
@@ -422,7 +437,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             uint2 qb[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              qb[nt] = V::kQRegs ? q_regs[V::kQRegs ? nt * 8 + 4 * h + i : 0] : reinterpret_cast<const uint2*>(gen + V::kQ)[(nt * 8 + 4 * h + i) * 32 + lane];
+              qb[nt] = RT == 1 ? q_regs[RT == 1 ? nt * 8 + 4 * h + i : 0] : reinterpret_cast<const uint2*>(gen + V::kQ)[(nt * 8 + 4 * h + i) * 32 + lane];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               uint32_t a[4];
@@ -572,85 +587,121 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       load_next();
     }
 
-    if (!ok) break;
-
-    // ---- the rows' results, or this warp's part of them ----
-    if (!p.whole && lane == 0) {
-      Left& of = sm_left[2 * warp + (p.first ? 0 : 1)];
-      of.begin = unit_begin;
-      of.e = p.e;
-      of.hk = p.hk;
-      of.rg = p.rg;
-      of.slices = p.slices;
-    }
+    // ---- the warps' sums together, and the rows' results or this CTA's part of them ----
+    done += p.end - p.j;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        float ll = l[rt][z];
-        const float mm = m[rt][z];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
-        const int r_in = rt * 8 + 2 * c + z;
-        const int r = p.rg * R + r_in, i = r / s.G, hq = p.hk * s.G + r - i * s.G;
-        if (i >= p.sq.len) continue;
-        float o[16];
-        const float unit = vref * (1.0f / 16384.0f);
+        for (int o = 4; o < 32; o <<= 1) l[rt][z] += __shfl_xor_sync(0xffffffffu, l[rt][z], o);
+        if (g == 0) *reinterpret_cast<float2*>(&sm_ml[(warp * R + rt * 8 + 2 * c + z) * 2]) = make_float2(m[rt][z], l[rt][z]);
+      }
+    __syncthreads();
+    float o[RT][2][16];  // rows 2c + z of tile rt, dimensions 16 g ..
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        float2 ml[kWarps];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) ml[w] = *reinterpret_cast<const float2*>(&sm_ml[(w * R + rt * 8 + 2 * c + z) * 2]);
+        const float mm = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), to = mm == -INFINITY ? 0.0f : mm;
+        const float f = ex2(m[rt][z] - to) * (vref * (1.0f / 16384.0f));
+        float ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) ll = fmaf(ml[w].y, ex2(ml[w].x - to), ll);
+        m[rt][z] = mm;
+        l[rt][z] = ll;
 #pragma unroll
         for (int d = 0; d < 16; ++d) {
-          o[d] = acc[rt * TERMS][d >> 1][2 * (d & 1) + z];
-          if (TERMS == 2) o[d] = fmaf(acc[rt * TERMS + TERMS - 1][d >> 1][2 * (d & 1) + z], 1.0f / 2048.0f, o[d]);
-          o[d] *= unit;
+          float x = acc[rt * TERMS][d >> 1][2 * (d & 1) + z];
+          if (TERMS == 2) x = fmaf(acc[rt * TERMS + TERMS - 1][d >> 1][2 * (d & 1) + z], 1.0f / 2048.0f, x);
+          o[rt][z][d] = x * f;
         }
-        if (p.sq.len > 1) {
-#pragma unroll
-          for (int d = 0; d < 16; ++d)
-            if (rows_limit[rt][z] > sm_nan[16 * g + d]) o[d] = __uint_as_float(0x7fffffffu);
-        }
-        if (!p.whole) {
-          const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + r_in;
-          if (g == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(mm, ll);
-          store16(s.part_o + slot * 128 + 16 * g, o, true);
-          continue;
-        }
-        const size_t row = static_cast<size_t>(p.sq.row0) + i;
-        if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
-        if (g == 0) note_lse(s, row, hq, mm + log2f(ll));
-        if (16 * g >= s.c.V) continue;
-        const float inv = 1.0f / ll;
-#pragma unroll
-        for (int d = 0; d < 16; ++d) o[d] = finished<T>(s, row, hq, 16 * g + d, o[d], inv);
-        store16(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 16 * g, o, s.vec_o);
       }
-    if (rest == 0) break;
+    float* merge = reinterpret_cast<float*>(gen + V::kMerge) + (warp & 1) * (RT * 32 * 32) + lane;
+    auto give = [&]() {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) merge[(rt * 32 + i) * 32] = o[rt][i >> 4][i & 15];
+    };
+    if (warp >= 2) give();
+    __syncthreads();
+    if (warp == 1) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) merge[(rt * 32 + i) * 32] += o[rt][i >> 4][i & 15];
+    } else if (warp == 0) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[rt][i >> 4][i & 15] += merge[(rt * 32 + i) * 32];
+    }
+    __syncthreads();
+    if (warp == 0) {
+      if (!p.whole && lane == 0) sm_left[p.first ? 0 : 1] = Left{unit_begin, p.e, p.hk, p.rg, p.slices};
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int r_in = rt * 8 + 2 * c + z, r = p.rg * R + r_in, i = r / s.G, hq = p.hk * s.G + r - i * s.G;
+          if (i >= p.sq.len) continue;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) o[rt][z][d] += merge[(RT * 32 + rt * 32 + z * 16 + d) * 32];
+          if (p.sq.len > 1) {
+#pragma unroll
+            for (int d = 0; d < 16; ++d)
+              if (rows_limit[rt][z] > sm_nan[16 * g + d]) o[rt][z][d] = __uint_as_float(0x7fffffffu);
+          }
+          if (!p.whole) {
+            const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + r_in;
+            if (g == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(m[rt][z], l[rt][z]);
+            store16(s.part_o + slot * 128 + 16 * g, o[rt][z], true);
+            continue;
+          }
+          float ll = l[rt][z];
+          const float mm = m[rt][z];
+          const size_t row = static_cast<size_t>(p.sq.row0) + i;
+          if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
+          if (g == 0) note_lse(s, row, hq, mm + log2f(ll));
+          if (16 * g >= s.c.V) continue;
+          const float inv = 1.0f / ll;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) o[rt][z][d] = finished<T>(s, row, hq, 16 * g + d, o[rt][z][d], inv);
+          store16(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 16 * g, o[rt][z], s.vec_o);
+        }
+    }
+    if (done >= share) break;
     unit_begin += p.slices;
-    next_piece(s, p, R, rest);
-    __syncwarp();
+    next_piece(s, p, R, share - done);
+    ask_row(p);
   }
-  (void)ok;  // (the error word is set: what the call leaves is not a result)
+  if (!ok) {  // (the error word is set and what the call leaves is not a result; copies on their way may still arrive)
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < 2000000ull) __nanosleep(1000);
+  }
 
   // ---- units whose parts this CTA completes ----
   __syncthreads();
-  if (threadIdx.x < 2 * kWarps) {
+  if (threadIdx.x < 2) {
     const Left u = sm_left[threadIdx.x];
-    bool mine = u.slices > 0;
-    for (int k = 0; k < static_cast<int>(threadIdx.x); ++k) mine = mine && !(sm_left[k].slices > 0 && sm_left[k].begin == u.begin);  // (said before)
     int c0 = 0, c1 = -1;
-    if (mine) {
+    if (u.slices > 0) {
       c0 = shares.owner(u.begin);
       c1 = shares.owner(u.begin + u.slices - 1);
-      const int ctas = c1 / kWarps - c0 / kWarps + 1;
-      if (ctas > 1) {  // (the counter goes back to zero with the last arrival)
-        __threadfence();
-        mine = atomicInc(s.arrivals + (static_cast<size_t>(u.e) * s.c.H + u.hk) * s.max_groups + u.rg, ctas - 1) == static_cast<unsigned>(ctas - 1);
-        __threadfence();
-      }
+      __threadfence();
+      // (the counter goes back to zero with the last arrival)
+      if (atomicInc(s.arrivals + (static_cast<size_t>(u.e) * s.c.H + u.hk) * s.max_groups + u.rg, c1 - c0) != static_cast<unsigned>(c1 - c0)) c1 = -1;
+      __threadfence();
     }
     sm_c0[threadIdx.x] = c0;
-    sm_c1[threadIdx.x] = mine ? c1 : -1;
+    sm_c1[threadIdx.x] = c1;
   }
   __syncthreads();
-  for (int k = 0; k < 2 * kWarps; ++k) {
+  for (int k = 0; k < 2; ++k) {
     const int c0 = sm_c0[k], c1 = sm_c1[k];
     if (c1 < c0) continue;
     const Left u = sm_left[k];
@@ -658,7 +709,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     const int slot0 = 2 * c0 + (shares.begin(c0) == u.begin ? 0 : 1);
     const int rows = min(R, sq.len * s.G - u.rg * R);
     const int wpr = rows >= 4 ? 1 : rows >= 2 ? 2 : 4;  // warps for a row
-    float4* sm_o = reinterpret_cast<float4*>(smem_raw + ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));  // [warps][32]: the stages are done with
+    float4* sm_o = reinterpret_cast<float4*>(gen);  // [warps][32]: the stages are done with
     float* sm_ml = reinterpret_cast<float*>(sm_o + kWarps * 32);
     for (int r0 = 0; r0 < rows; r0 += kWarps / wpr) {
       const int r_in = r0 + warp / wpr;
@@ -764,8 +815,9 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
       const int r = r0 + g, at = min(r, rows - 1), i = at / s.G, hq = hk * s.G + at - i * s.G;
       const size_t row = static_cast<size_t>(sq.row0) + i;
       uint32_t term[TERMS][16];
-      const float f = split_row<T, TERMS>(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c,
-                                          s.scale_log2, term);
+      float raw[32];
+      load_row(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c, raw);
+      const float f = split_row<TERMS>(raw, s.scale_log2, term);
       const float lse = s.lse2[row * s.a.Hq + hq];
       const int see = r < rows ? sq.pos + i + 1 - kb : 0;
       float factor[2], z2[2];
@@ -831,7 +883,7 @@ Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len
     for_variant(p.kind, [&](auto v) {
       using V = decltype(v);
       p.rows = V::kRows;
-      p.parts = sm_count() * V::kCtas * kWarps;  // the warps that are resident at once
+      p.parts = sm_count() * V::kCtas;  // the CTAs that are resident at once
     });
     p.groups = static_cast<int>((unit + p.rows - 1) / p.rows);
     return static_cast<size_t>(2) * p.parts * p.rows;
@@ -941,7 +993,7 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   if (any_short)
     for_variant(p.kind, [&](auto v) {
       using V = decltype(v);
-      launch_kernel(cache8_attention_kernel<V>, dim3(p.parts / kWarps), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
+      launch_kernel(cache8_attention_kernel<V>, dim3(p.parts), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
     });
   if (a.weights && any_short) {
     const PdlScope behind;
