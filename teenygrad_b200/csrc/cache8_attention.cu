@@ -38,12 +38,12 @@ template <int RT_, int TERMS_>
 struct Variant {
   static constexpr int RT = RT_, TERMS = TERMS_, NT = RT * TERMS, kRows = 8 * RT, kCtas = NT == 1 ? 3 : 2, kStages = 2;
   using T = typename std::conditional<TERMS == 2, float, bf16>::type;
-  // shared memory: stages of the warps, scales f32 [warps][stages][4], int [128] first NaN value of each dimension, maximum and sum of a row [warps][rows][2],
+  // shared memory: stages of the warps, scales f32 [warps][stages][4], int [128] first NaN value of each dimension, maximum and sum of a row [2][warps][rows][2],
   // barriers, factors [rows], queries uint2 [row tiles][8 steps][32 lanes] (one row tile: in registers), sums on their way f32 [2][RT * 32][32 lanes]
   static constexpr int kScales = kWarps * kStages * kStage;
   static constexpr int kNan = kScales + kWarps * kStages * 16;
   static constexpr int kML = kNan + 128 * 4;
-  static constexpr int kBars = kML + kWarps * kRows * 8;
+  static constexpr int kBars = kML + 2 * kWarps * kRows * 8;
   static constexpr int kFactor = kBars + kWarps * kStages * 8;
   static constexpr int kQ = kFactor + kRows * 4;
   static constexpr int kMerge = kQ + (RT == 1 ? 0 : RT * 8 * 32 * 8);
@@ -53,14 +53,14 @@ struct Variant {
 
 // D (16 x 8) += A (16 x 16) B
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // 8 x 8 16-bit numbers: lane (g, c) gives (row g, columns 2c, 2c + 1) and gets (rows 2c, 2c + 1 of column g)
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 // Four E4M3 numbers as two f16 pairs
@@ -75,16 +75,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t rest_f16x2(uint32_t two, float x, float y) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
   return pack_f16x2((x - f.x) * 2048.0f, (y - f.y) * 2048.0f);
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float lds32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
 }
 __device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -138,36 +128,32 @@ struct Shares {
 
 __device__ __forceinline__ int warp_sum_int(int v) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(v))); }
 
-// Output element of query head h in row `row`: o unnormalised, l the row sum (with the sink's part).
-template <typename T>
-__device__ __forceinline__ float finished(const Shared& s, size_t row, int h, int d, float o, float inv) {
-  o *= inv;
-  if (s.a.gate) o *= sigmoid_f(load_one(static_cast<const T*>(s.a.gate) + row * s.a.ldg + static_cast<size_t>(h) * s.c.V + d));
-  return o;
-}
 __device__ __forceinline__ void note_lse(const Shared& s, size_t row, int h, float lse2) {
   if (s.lse2) s.lse2[row * s.a.Hq + h] = lse2;
   if (s.a.lse) s.a.lse[row * s.a.Hq + h] = lse2 * kLn2;
 }
-// 16 finished numbers of a row
-__device__ __forceinline__ void store16(bf16* p, const float (&x)[16], bool vec) {
-  if (vec) {
+// The results of row r (counted in its entry) of kv head hk, dimensions 4 lane ..: x unnormalised, relative to the maximum m (base 2), l the row sum.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Shared& s, const SeqDesc& sq, int hk, int r, int lane, const float4& x, float m, float l) {
+  const int i = r / s.G, hq = hk * s.G + r - i * s.G;
+  const size_t row = static_cast<size_t>(sq.row0) + i;
+  if (s.a.sink) l += ex2(fmaf(s.a.sink[hq], kLog2e, -m));
+  if (lane == 0) note_lse(s, row, hq, m + log2f(l));
+  if (4 * lane >= s.c.V) return;
+  const float inv = 1.0f / l;
+  float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+  if (s.a.gate) {
+    const T* gate = static_cast<const T*>(s.a.gate) + row * s.a.ldg + static_cast<size_t>(hq) * s.c.V + 4 * lane;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      reinterpret_cast<uint4*>(p)[i] = make_uint4(pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
-                                                  pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) store_one(p + i, x[i]);
+    for (int d = 0; d < 4; ++d) y[d] *= sigmoid_f(load_one(gate + d));
   }
-}
-__device__ __forceinline__ void store16(float* p, const float (&x)[16], bool vec) {
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 4 * lane;
+  if (s.vec_o) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    else *reinterpret_cast<float4*>(out) = make_float4(y[0], y[1], y[2], y[3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) p[i] = x[i];
+    for (int d = 0; d < 4; ++d) store_one(out + d, y[d]);
   }
 }
 
@@ -366,7 +352,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   float* sm_ml = reinterpret_cast<float*>(gen + V::kML);
   float* sm_factor = reinterpret_cast<float*>(gen + V::kFactor);
   bool ok = true;
-  int done = 0, unit_begin = t0 - p.j;  // slices of the share in front of the piece; of the call in front of its unit
+  int flip = 0, done = 0, unit_begin = t0 - p.j;  // slices of the share in front of the piece; of the call in front of its unit
   for (;;) {
     // ---- queries as B fragments: row g of tile rt is column g ----
     float factor[RT][2];      // of the rows 2c, 2c + 1, whose scores this lane gets
@@ -418,8 +404,9 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         break;
       }
       if (kb < p.limit) {
-        const uint32_t kt = ring + st * kStage + g * 128, vt = ring + st * kStage + kBox, sc = scale_at + st * 16;
-        const float ks0 = lds32(sc), ks1 = lds32(sc + 4), vs0 = lds32(sc + 8), vs1 = lds32(sc + 12);
+        const uint8_t *kt = gen + warp * (ST * kStage) + st * kStage + g * 128, *vt = gen + warp * (ST * kStage) + st * kStage + kBox;
+        const float4 scales = *reinterpret_cast<const float4*>(gen + V::kScales + (warp * ST + st) * 16);
+        const float ks0 = scales.x, ks1 = scales.y, vs0 = scales.z, vs1 = scales.w;
         const bool masked = kb + kSlice > p.sq.pos + 1;
         // ---- scores: keys 16 u + g and 16 u + 8 + g of the slice are rows g and g + 8 of tile u; lane c reads the dimensions that it holds of the query ----
         float x[NT][2][4];
@@ -431,7 +418,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         for (int h = 0; h < 2; ++h) {
           uint4 kw[4];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) kw[t] = lds128(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
+          for (int t = 0; t < 4; ++t) kw[t] = *reinterpret_cast<const uint4*>(kt + t * 1024 + (((2 * c + h) ^ g) << 4));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint2 qb[NT];
@@ -539,7 +526,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int row = 2 * c + (i & 1) + 8 * (i >> 1);
-          vw[i] = lds128(vt + row * 128 + ((g ^ (row & 7)) << 4));
+          vw[i] = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
         }
         if (masked) {
 #pragma unroll
@@ -589,90 +576,75 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
     // ---- the warps' sums together, and the rows' results or this CTA's part of them ----
     done += p.end - p.j;
+    float* ml = sm_ml + flip * (kWarps * R * 2);  // (a fast warp is at the next piece's while a slow one reads this one's)
+    flip ^= 1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[rt][z] += __shfl_xor_sync(0xffffffffu, l[rt][z], o);
-        if (g == 0) *reinterpret_cast<float2*>(&sm_ml[(warp * R + rt * 8 + 2 * c + z) * 2]) = make_float2(m[rt][z], l[rt][z]);
+        if (g == 0) *reinterpret_cast<float2*>(&ml[(warp * R + rt * 8 + 2 * c + z) * 2]) = make_float2(m[rt][z], l[rt][z]);
       }
     __syncthreads();
-    float o[RT][2][16];  // rows 2c + z of tile rt, dimensions 16 g ..
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        float2 ml[kWarps];
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) ml[w] = *reinterpret_cast<const float2*>(&sm_ml[(w * R + rt * 8 + 2 * c + z) * 2]);
-        const float mm = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), to = mm == -INFINITY ? 0.0f : mm;
-        const float f = ex2(m[rt][z] - to) * (vref * (1.0f / 16384.0f));
-        float ll = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) ll = fmaf(ml[w].y, ex2(ml[w].x - to), ll);
-        m[rt][z] = mm;
-        l[rt][z] = ll;
-#pragma unroll
-        for (int d = 0; d < 16; ++d) {
-          float x = acc[rt * TERMS][d >> 1][2 * (d & 1) + z];
-          if (TERMS == 2) x = fmaf(acc[rt * TERMS + TERMS - 1][d >> 1][2 * (d & 1) + z], 1.0f / 2048.0f, x);
-          o[rt][z][d] = x * f;
-        }
-      }
-    float* merge = reinterpret_cast<float*>(gen + V::kMerge) + (warp & 1) * (RT * 32 * 32) + lane;
-    auto give = [&]() {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) merge[(rt * 32 + i) * 32] = o[rt][i >> 4][i & 15];
-    };
-    if (warp >= 2) give();
-    __syncthreads();
-    if (warp == 1) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) merge[(rt * 32 + i) * 32] += o[rt][i >> 4][i & 15];
-    } else if (warp == 0) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[rt][i >> 4][i & 15] += merge[(rt * 32 + i) * 32];
-    }
-    __syncthreads();
-    if (warp == 0) {
-      if (!p.whole && lane == 0) sm_left[p.first ? 0 : 1] = Left{unit_begin, p.e, p.hk, p.rg, p.slices};
+    // warps 2 and 3 give theirs to 0 and 1: float4 [rt * 8 + 4 z + i][lane] are dimensions 16 g + 4 i .. of row 8 rt + 2 c + z
+    float4* merge = reinterpret_cast<float4*>(gen + V::kMerge);
+    auto pass = [&](bool add) {
+      float4* at = merge + (warp & 1) * (RT * 8 * 32) + lane;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          const int r_in = rt * 8 + 2 * c + z, r = p.rg * R + r_in, i = r / s.G, hq = p.hk * s.G + r - i * s.G;
-          if (i >= p.sq.len) continue;
+          const float mm = fmaxf(fmaxf(ml[(rt * 8 + 2 * c + z) * 2], ml[(R + rt * 8 + 2 * c + z) * 2]),
+                                 fmaxf(ml[(2 * R + rt * 8 + 2 * c + z) * 2], ml[(3 * R + rt * 8 + 2 * c + z) * 2]));
+          const float f = ex2(m[rt][z] - (mm == -INFINITY ? 0.0f : mm)) * (vref * (1.0f / 16384.0f));
 #pragma unroll
-          for (int d = 0; d < 16; ++d) o[rt][z][d] += merge[(RT * 32 + rt * 32 + z * 16 + d) * 32];
-          if (p.sq.len > 1) {
+          for (int i = 0; i < 4; ++i) {
+            float x[4];
 #pragma unroll
-            for (int d = 0; d < 16; ++d)
-              if (rows_limit[rt][z] > sm_nan[16 * g + d]) o[rt][z][d] = __uint_as_float(0x7fffffffu);
+            for (int k = 0; k < 4; ++k) {
+              const int d = 4 * i + k;
+              x[k] = acc[rt * TERMS][d >> 1][2 * (d & 1) + z];
+              if (TERMS == 2) x[k] = fmaf(acc[rt * TERMS + TERMS - 1][d >> 1][2 * (d & 1) + z], 1.0f / 2048.0f, x[k]);
+            }
+            float4& to = at[(rt * 8 + 4 * z + i) * 32];
+            const float4 y = add ? to : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            to = make_float4(fmaf(x[0], f, y.x), fmaf(x[1], f, y.y), fmaf(x[2], f, y.z), fmaf(x[3], f, y.w));
           }
-          if (!p.whole) {
-            const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + r_in;
-            if (g == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(m[rt][z], l[rt][z]);
-            store16(s.part_o + slot * 128 + 16 * g, o[rt][z], true);
-            continue;
-          }
-          float ll = l[rt][z];
-          const float mm = m[rt][z];
-          const size_t row = static_cast<size_t>(p.sq.row0) + i;
-          if (s.a.sink) ll += ex2(fmaf(s.a.sink[hq], kLog2e, -mm));
-          if (g == 0) note_lse(s, row, hq, mm + log2f(ll));
-          if (16 * g >= s.c.V) continue;
-          const float inv = 1.0f / ll;
-#pragma unroll
-          for (int d = 0; d < 16; ++d) o[rt][z][d] = finished<T>(s, row, hq, 16 * g + d, o[rt][z][d], inv);
-          store16(static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 16 * g, o[rt][z], s.vec_o);
         }
+    };
+    if (warp >= 2) pass(false);
+    __syncthreads();
+    if (warp < 2) pass(true);
+    __syncthreads();
+    if (!p.whole && threadIdx.x == 0) sm_left[p.first ? 0 : 1] = Left{unit_begin, p.e, p.hk, p.rg, p.slices};
+    const int rows = min(R, p.sq.len * s.G - p.rg * R);
+#pragma unroll 1
+    for (int r_in = warp; r_in < rows; r_in += kWarps) {  // (a lane: four dimensions)
+      const float4* at = merge + ((r_in >> 3) * 8 + 4 * (r_in & 1) + (lane & 3)) * 32 + (lane >> 2) * 4 + ((r_in & 7) >> 1);
+      const float4 x0 = at[0], x1 = at[RT * 8 * 32];
+      float x[4] = {x0.x + x1.x, x0.y + x1.y, x0.z + x1.z, x0.w + x1.w};
+      float2 of[kWarps];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) of[w] = *reinterpret_cast<const float2*>(&ml[(w * R + r_in) * 2]);
+      const float mm = fmaxf(fmaxf(of[0].x, of[1].x), fmaxf(of[2].x, of[3].x)), to = mm == -INFINITY ? 0.0f : mm;
+      float ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) ll = fmaf(of[w].y, ex2(of[w].x - to), ll);
+      if (p.sq.len > 1) {
+        const int limit = p.sq.pos + (p.rg * R + r_in) / s.G + 1;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          if (limit > sm_nan[4 * lane + d]) x[d] = __uint_as_float(0x7fffffffu);
+      }
+      const float4 o = make_float4(x[0], x[1], x[2], x[3]);
+      if (p.whole) {
+        finish_row<T>(s, p.sq, p.hk, p.rg * R + r_in, lane, o, mm, ll);
+      } else {
+        const size_t slot = (2 * static_cast<size_t>(part) + (p.first ? 0 : 1)) * R + r_in;
+        if (lane == 0) *reinterpret_cast<float2*>(s.part_ml + slot * 2) = make_float2(mm, ll);
+        *reinterpret_cast<float4*>(s.part_o + slot * 128 + 4 * lane) = o;
+      }
     }
     if (done >= share) break;
     unit_begin += p.slices;
@@ -708,56 +680,63 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     const SeqDesc sq = s.seqs[u.e];
     const int slot0 = 2 * c0 + (shares.begin(c0) == u.begin ? 0 : 1);
     const int rows = min(R, sq.len * s.G - u.rg * R);
-    const int wpr = rows >= 4 ? 1 : rows >= 2 ? 2 : 4;  // warps for a row
-    float4* sm_o = reinterpret_cast<float4*>(gen);  // [warps][32]: the stages are done with
-    float* sm_ml = reinterpret_cast<float*>(sm_o + kWarps * 32);
-    for (int r0 = 0; r0 < rows; r0 += kWarps / wpr) {
-      const int r_in = r0 + warp / wpr;
-      float m = -INFINITY, l = 0.0f;
-      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      auto join = [&](float pm, float pl, const float4& x) {
-        const float top = fmaxf(m, pm), to = top == -INFINITY ? 0.0f : top, a = ex2(m - to), f = ex2(pm - to);
-        m = top;
-        l = fmaf(pl, f, l * a);
-        o.x = fmaf(x.x, f, o.x * a); o.y = fmaf(x.y, f, o.y * a); o.z = fmaf(x.z, f, o.z * a); o.w = fmaf(x.w, f, o.w * a);
-      };
-      if (r_in < rows)
-        for (int q0 = c0 + warp % wpr; q0 <= c1; q0 += 8 * wpr) {
-          float2 ml[8];
-          float4 x[8];
+    // eight parts at a time: of a row, with more than four rows of two
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float4 o[2] = {};
+    auto join = [&](int k, float pm, float pl, const float4& x) {
+      const float top = fmaxf(m[k], pm), to = top == -INFINITY ? 0.0f : top, a = ex2(m[k] - to), f = ex2(pm - to);
+      m[k] = top;
+      l[k] = fmaf(pl, f, l[k] * a);
+      o[k].x = fmaf(x.x, f, o[k].x * a); o[k].y = fmaf(x.y, f, o[k].y * a); o[k].z = fmaf(x.z, f, o[k].z * a); o[k].w = fmaf(x.w, f, o[k].w * a);
+    };
+    float2 ml[8];
+    float4 x[8];
+    auto ask = [&](int i, int q, int r_in) {
+      ml[i] = make_float2(-INFINITY, 0.0f);
+      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (q > c1 || r_in >= rows) return;
+      const size_t slot = static_cast<size_t>(q == c0 ? slot0 : 2 * q) * R + r_in;
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(s.part_ml + slot * 2));
+      x[i] = __ldcg(reinterpret_cast<const float4*>(s.part_o + slot * 128 + 4 * lane));
+    };
+    if (rows > 4) {
+#pragma unroll 1
+      for (int r0 = warp; r0 < rows; r0 += 2 * kWarps) {
+#pragma unroll 1
+        for (int q0 = c0; q0 <= c1; q0 += 4) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int q = q0 + wpr * i;
-            ml[i] = make_float2(-INFINITY, 0.0f);
-            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (q > c1) continue;
-            const size_t slot = static_cast<size_t>(q == c0 ? slot0 : 2 * q) * R + r_in;
-            ml[i] = __ldcg(reinterpret_cast<const float2*>(s.part_ml + slot * 2));
-            x[i] = __ldcg(reinterpret_cast<const float4*>(s.part_o + slot * 128 + 4 * lane));
-          }
+          for (int i = 0; i < 8; ++i) ask(i, q0 + (i & 3), r0 + (i >> 2) * kWarps);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) join(ml[i].x, ml[i].y, x[i]);
+          for (int i = 0; i < 8; ++i) join(i >> 2, ml[i].x, ml[i].y, x[i]);
         }
+        finish_row<T>(s, sq, u.hk, u.rg * R + r0, lane, o[0], m[0], l[0]);
+        if (r0 + kWarps < rows) finish_row<T>(s, sq, u.hk, u.rg * R + r0 + kWarps, lane, o[1], m[1], l[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          m[i] = -INFINITY;
+          l[i] = 0.0f;
+          o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+    } else {
+      const int wpr = rows >= 3 ? 1 : rows == 2 ? 2 : 4, r_in = warp / wpr;  // warps for a row
+#pragma unroll 1
+      for (int q0 = c0 + warp % wpr; q0 <= c1; q0 += 8 * wpr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ask(i, q0 + i * wpr, r_in);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) join(0, ml[i].x, ml[i].y, x[i]);
+      }
       if (wpr > 1) {
-        sm_o[warp * 32 + lane] = o;
-        if (lane == 0) { sm_ml[2 * warp] = m; sm_ml[2 * warp + 1] = l; }
+        float4* sm_o = reinterpret_cast<float4*>(gen);  // [warps][32]: the stages are done with
+        sm_o[warp * 32 + lane] = o[0];
+        if (lane == 0) { sm_ml[2 * warp] = m[0]; sm_ml[2 * warp + 1] = l[0]; }
         __syncthreads();
         if (warp % wpr == 0)
-          for (int w = warp + 1; w < warp + wpr; ++w) join(sm_ml[2 * w], sm_ml[2 * w + 1], sm_o[w * 32 + lane]);
+          for (int w = warp + 1; w < warp + wpr; ++w) join(0, sm_ml[2 * w], sm_ml[2 * w + 1], sm_o[w * 32 + lane]);
         __syncthreads();
-        if (warp % wpr) continue;
       }
-      if (r_in >= rows) continue;
-      const int r = u.rg * R + r_in, i = r / s.G, hq = u.hk * s.G + r - i * s.G;
-      const size_t row = static_cast<size_t>(sq.row0) + i;
-      if (s.a.sink) l += ex2(fmaf(s.a.sink[hq], kLog2e, -m));
-      if (lane == 0) note_lse(s, row, hq, m + log2f(l));
-      if (4 * lane >= s.c.V) continue;
-      const float inv = 1.0f / l;
-      T* out = static_cast<T*>(s.a.out) + row * s.a.ldo + static_cast<size_t>(hq) * s.c.V + 4 * lane;
-      const float y[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-      for (int d = 0; d < 4; ++d) store_one(out + d, finished<T>(s, row, hq, 4 * lane + d, y[d], inv));
+      if (warp % wpr == 0 && r_in < rows) finish_row<T>(s, sq, u.hk, u.rg * R + r_in, lane, o[0], m[0], l[0]);
     }
   }
 }
