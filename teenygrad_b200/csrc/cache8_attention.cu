@@ -86,13 +86,14 @@ struct Shared {  // what a call's kernels share
   Cache8Attn a;
   const SeqDesc* seqs;
   int n_seqs, max_len, G;
-  float scale_log2, two_over_cap, cap_l2;
+  float scale_log2, one_over_cap, cap_l2;  // (the cap in base 2, like the scores)
   float* part_o;   // [2 * CTAs][rows of a unit][128]
   float* part_ml;  // [2 * CTAs][rows of a unit][2]
   unsigned* arrivals;  // [entries][kv heads][max_groups]: CTAs that have stored their parts, zero between calls
   int max_groups;
   float* lse2;     // [rows][Hq], base 2, or null
-  float* scores;   // [entries][Hq][cap] base 2, or null
+  float* scores;   // [entries][Hq][score_row] base 2, or null
+  int score_row;   // cap, rounded up to whole fours
   int parts;       // CTAs of the main kernel
   int vec_q, vec_o;
   int* err;
@@ -465,7 +466,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) y[t][z] = softcap_log2(y[t][z], s.two_over_cap, s.cap_l2);
+              for (int z = 0; z < 2; ++z) y[t][z] = cap_score(y[t][z], s.one_over_cap, s.cap_l2);
           }
           if (masked) {
 #pragma unroll
@@ -477,7 +478,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const int r = p.rg * R + rt * 8 + 2 * c + z;  // (single tokens: a row is a query head of the group)
-              float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.c.cap + kb + g;
+              float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.score_row + kb + g;
 #pragma unroll
               for (int t = 0; t < 4; ++t)
                 if (r < s.G && kb + 8 * t + g < p.limit) to[8 * t] = y[t][z];
@@ -741,19 +742,31 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   }
 }
 
-// Weights of single tokens' calls, from the scores that the attention kernel left: blockIdx = (share of the keys, kv head, entry).
+// Weights of single tokens' calls, from the scores that the attention kernel left: blockIdx = (share of the keys, kv head, entry), four keys a thread.
 __global__ void __launch_bounds__(256) cache8_weights_kernel(const __grid_constant__ Shared s) {
   pdl_wait();
   const int e = blockIdx.z, hk = blockIdx.y;
   const SeqDesc sq = s.seqs[e];
   if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return;
   float* w = s.c.w + (static_cast<size_t>(sq.slot) * s.c.H + hk) * s.c.cap;
-  const float* x = s.scores + (static_cast<size_t>(e) * s.a.Hq + hk * s.G) * s.c.cap;
+  const float* x = s.scores + (static_cast<size_t>(e) * s.a.Hq + hk * s.G) * s.score_row;
   const float* z = s.lse2 + static_cast<size_t>(sq.row0) * s.a.Hq + hk * s.G;
-  for (int j = blockIdx.x * 256 + threadIdx.x; j <= sq.pos; j += gridDim.x * 256) {
-    float sum = 0.0f;
-    for (int h = 0; h < s.G; ++h) sum += ex2(x[static_cast<size_t>(h) * s.c.cap + j] - z[h]);
-    w[j] = s.a.decay == 0.0f ? sum : fmaf(s.a.decay, w[j], sum);
+  for (int j = 4 * (blockIdx.x * 256 + threadIdx.x); j <= sq.pos; j += gridDim.x * 1024) {
+    float sum[4] = {}, old[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) old[k] = s.a.decay != 0.0f && j + k <= sq.pos ? w[j + k] : 0.0f;
+#pragma unroll 4
+    for (int h = 0; h < s.G; ++h) {
+      const float4 y = *reinterpret_cast<const float4*>(x + static_cast<size_t>(h) * s.score_row + j);  // (rows of whole fours)
+      const float lse = z[h];
+      sum[0] += ex2(y.x - lse);
+      sum[1] += ex2(y.y - lse);
+      sum[2] += ex2(y.z - lse);
+      sum[3] += ex2(y.w - lse);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (j + k <= sq.pos) w[j + k] = fmaf(s.a.decay, old[k], sum[k]);
   }
 }
 
@@ -822,7 +835,7 @@ __global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_c
             float v = d[0][2 * half + z];
             if (TERMS == 2) v = fmaf(d[TERMS - 1][2 * half + z], 1.0f / 2048.0f, v);
             v *= factor[z] * ks[u];
-            if (s.cap_l2 > 0.0f) v = softcap_log2(v, s.two_over_cap, s.cap_l2);
+            if (s.cap_l2 > 0.0f) v = cap_score(v, s.one_over_cap, s.cap_l2);
             if (16 * u + 8 * half + g < sees[z]) sum[2 * u + half] += ex2(v - z2[z]);
           }
       }
@@ -880,7 +893,7 @@ Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len
   p.part_o = take(part_rows * 128 * 4);
   p.part_ml = take(part_rows * 2 * 4);
   p.lse2 = weights ? take(static_cast<size_t>(rows) * Hq * 4) : 0;
-  p.scores = weights && call_len == 1 ? take(static_cast<size_t>(n_seqs) * Hq * c.cap * 4) : 0;
+  p.scores = weights && call_len == 1 ? take(static_cast<size_t>(n_seqs) * Hq * ((c.cap + 3) / 4 * 4) * 4) : 0;
   p.widened = prompts ? take(cache8_prefill_scratch_bytes(c, n_seqs)) : 0;
   return p;
 }
@@ -947,11 +960,12 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   s.seqs = seqs;
   s.n_seqs = n_seqs;
   s.max_len = max_len;
+  s.score_row = (c.cap + 3) / 4 * 4;
   s.G = a.Hq / c.H;
   s.scale_log2 = a.scale * kLog2e;
   if (a.softcap > 0.0f) {
-    s.two_over_cap = 2.0f / a.softcap;
     s.cap_l2 = a.softcap * kLog2e;
+    s.one_over_cap = 1.0f / s.cap_l2;
   }
   uint8_t* scratch = static_cast<uint8_t*>(a.scratch);
   s.arrivals = reinterpret_cast<unsigned*>(scratch + p.arrivals);
@@ -976,7 +990,7 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
     });
   if (a.weights && any_short) {
     const PdlScope behind;
-    const int shares = (c.cap + 255) / 256, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
+    const int shares = call_len == 1 ? (c.cap + 1023) / 1024 : (c.cap + 127) / 128, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
     if (call_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);
     else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float>, grid, dim3(128), 0, st, 1, s);

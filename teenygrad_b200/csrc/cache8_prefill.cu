@@ -2,6 +2,7 @@
 // scratch once (exact: an E4M3 number times a power of two) and the tcgen05 kernel of attention_prefill.cu runs on those.  Widening
 // reads one byte and writes two for each number, 0.8 KB a token and kv head at head size 128, against len * group * 512 multiply-adds.
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -113,7 +114,7 @@ constexpr int kWThreads = 384, kWQ = 3, kWLse = 4, kWS = 4;
 struct WSmem {
   static constexpr int kK = 0;                                // two key tiles, two boxes of [128][64] each
   static constexpr int kQ = kK + 2 * 32768;                   // ring of query tiles
-  static constexpr int kLse = kQ + kWQ * 32768;               // f32 [kWLse][128]
+  static constexpr int kLse = kQ + kWQ * 32768;               // f32 [kWLse][128], negated
   static constexpr int kSum = kLse + kWLse * 512;             // f32 [2][128]: what the second warpgroup hands over, by item
   static constexpr int kBar = kSum + 2 * 512;
   static constexpr int kTotal = kBar + 256 + 1024;
@@ -123,10 +124,11 @@ struct WeightsArgs {
   const SeqDesc* seqs;
   const float* lse2;  // [rows][Hq]
   int n_seqs, key_rows, tiles, min_len, max_len, rows, Hq;
-  float scale_log2, two_over_cap, cap_l2, decay;
+  float scale_log2, one_over_cap, cap_l2, decay;
   int* err;
 };
 
+template <bool CAP>
 __global__ void __launch_bounds__(kWThreads, 1)
 cache8_prompt_weights_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ WeightsArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -218,7 +220,7 @@ cache8_prompt_weights_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int i = q * 128 + x * 32 + lane;
-            to[x * 32 + lane] = i < sq.len ? a.lse2[(static_cast<size_t>(sq.row0) + i) * a.Hq + hk * G + g] : 0.0f;
+            to[x * 32 + lane] = i < sq.len ? -a.lse2[(static_cast<size_t>(sq.row0) + i) * a.Hq + hk * G + g] : 0.0f;
           }
           mbar_arrive(bar(L_FULL + sl));
         }
@@ -228,7 +230,15 @@ cache8_prompt_weights_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
     const int wg = (warp - 4) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-    int t = 0;
+    int t = 0, last_n = -1;
+    float *last_w = nullptr, last_sum = 0.0f;  // the first warpgroup's last item, but for the other's part
+    auto finish = [&](int n) {
+      if (!mbar_wait(bar(X_FULL + (n & 1)), n >> 1 & 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
+      const float other = reinterpret_cast<const float*>(gen + WSmem::kSum)[(n & 1) * 128 + key];
+      mbar_arrive(bar(X_EMPTY + (n & 1)));
+      if (last_w) *last_w = last_sum + other;
+      return true;
+    };
     walk([&](int n, int, const SeqDesc& sq, int hk, int key0, int q0, int q1) {
       const bool mine = key0 + key < sq.pos + sq.len;
       float* w = a.c.w + (static_cast<size_t>(sq.slot) * a.c.H + hk) * a.c.cap + key0 + key;
@@ -245,52 +255,58 @@ cache8_prompt_weights_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
           const int rows = sq.len - q * 128;  // columns from this one on are not the entry's
           const bool masked = key0 + 127 > sq.pos + q * 128 || rows < 128;
           const float4* lse = reinterpret_cast<const float4*>(gen + WSmem::kLse + sl * 512);
+          // (the masked tiles have a loop of their own: a test at every element kept the others' from being worked on side by side)
+          auto add = [&](auto with_mask) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t r[32];
-            tmem_ld_32x32(tmem + lane_addr + sb * 128 + x * 32, r);
-            tmem_wait_ld();
-            if (a.cap_l2 > 0.0f) {
+            for (int x = 0; x < 4; ++x) {
+              uint32_t r[32];
+              tmem_ld_32x32(tmem + lane_addr + sb * 128 + x * 32, r);
+              tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(softcap_log2(__uint_as_float(r[i]) * a.scale_log2, a.two_over_cap, a.cap_l2));
-            }
+              for (int i = 0; i < 8; ++i) {
+                const float4 z = lse[x * 8 + i];
+                float2 p[2] = {make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]))};
+                const float2 minus[2] = {make_float2(z.x, z.y), make_float2(z.z, z.w)};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 z = lse[x * 8 + i];
-              float2 s0 = make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), s1 = make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-              const float2 z0 = make_float2(-z.x, -z.y), z1 = make_float2(-z.z, -z.w);
-              s0 = a.cap_l2 > 0.0f ? __fadd2_rn(s0, z0) : __ffma2_rn(s0, sc2, z0);
-              s1 = a.cap_l2 > 0.0f ? __fadd2_rn(s1, z1) : __ffma2_rn(s1, sc2, z1);
-              if (masked) {
-                const int col = x * 32 + 4 * i;
-                if (col < hidden || col >= rows) s0.x = -INFINITY;
-                if (col + 1 < hidden || col + 1 >= rows) s0.y = -INFINITY;
-                if (col + 2 < hidden || col + 2 >= rows) s1.x = -INFINITY;
-                if (col + 3 < hidden || col + 3 >= rows) s1.y = -INFINITY;
+                for (int k = 0; k < 2; ++k) {
+                  if (CAP) {
+                    p[k].x = cap_score(p[k].x * a.scale_log2, a.one_over_cap, a.cap_l2);
+                    p[k].y = cap_score(p[k].y * a.scale_log2, a.one_over_cap, a.cap_l2);
+                    p[k] = __fadd2_rn(p[k], minus[k]);
+                  } else {
+                    p[k] = __ffma2_rn(p[k], sc2, minus[k]);
+                  }
+                  if (with_mask.value) {
+                    const int col = x * 32 + 4 * i + 2 * k;
+                    if (col < hidden || col >= rows) p[k].x = -INFINITY;
+                    if (col + 1 < hidden || col + 1 >= rows) p[k].y = -INFINITY;
+                  }
+                  sum[k] = __fadd2_rn(sum[k], make_float2(ex2(p[k].x), ex2(p[k].y)));
+                }
               }
-              sum[0] = __fadd2_rn(sum[0], make_float2(ex2(s0.x), ex2(s0.y)));
-              sum[1] = __fadd2_rn(sum[1], make_float2(ex2(s1.x), ex2(s1.y)));
             }
-          }
+          };
+          if (masked) add(std::true_type{});
+          else add(std::false_type{});
           tc_fence_before();
           mbar_arrive(bar(S_EMPTY + sb));
           mbar_arrive(bar(L_EMPTY + sl));
         }
-      // the second warpgroup's part to the first
-      float* give = reinterpret_cast<float*>(gen + WSmem::kSum) + (n & 1) * 128 + key;
+      // the second warpgroup's part to the first, which adds it an item later: by then it is there
       const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       if (wg == 1) {
         if (!mbar_wait(bar(X_EMPTY + (n & 1)), (n >> 1 & 1) ^ 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
-        *give = total;
+        reinterpret_cast<float*>(gen + WSmem::kSum)[(n & 1) * 128 + key] = total;
         mbar_arrive(bar(X_FULL + (n & 1)));
-      } else {
-        if (!mbar_wait(bar(X_FULL + (n & 1)), n >> 1 & 1, a.err, DEVERR_ATTN_SOFTMAX)) return false;
-        const float all = total + *give;
-        mbar_arrive(bar(X_EMPTY + (n & 1)));
-        if (mine) *w = fmaf(a.decay, old, all);
+        return true;
       }
+      if (n > 0 && !finish(n - 1)) return false;
+      last_w = mine ? w : nullptr;
+      last_sum = fmaf(a.decay, old, total);
+      last_n = n;
       return true;
     });
+    if (wg == 0 && last_n >= 0) finish(last_n);
   }
   tc_fence_before();
   __syncthreads();
@@ -309,7 +325,8 @@ int prompt_weights(const Cache8& c, const Cache8Attn& a, const Widened& w, const
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !((done.load(std::memory_order_acquire) >> dev) & 1ull)) {
-    const cudaError_t e = cudaFuncSetAttribute(cache8_prompt_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WSmem::kTotal);
+    cudaError_t e = cudaFuncSetAttribute(cache8_prompt_weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, WSmem::kTotal);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache8_prompt_weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, WSmem::kTotal);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   }
@@ -333,14 +350,14 @@ int prompt_weights(const Cache8& c, const Cache8Attn& a, const Widened& w, const
   t.Hq = a.Hq;
   t.scale_log2 = a.scale * 1.4426950408889634f;
   if (a.softcap > 0.0f) {
-    t.two_over_cap = 2.0f / a.softcap;
     t.cap_l2 = a.softcap * 1.4426950408889634f;
+    t.one_over_cap = 1.0f / t.cap_l2;
   }
   t.decay = a.decay;
   t.err = device_error_word();
   if (!t.err) return TEENY_ERR_DRIVER;
   const long long items = static_cast<long long>(w.tiles) * w.n_seqs * c.H, sms = sm_count();
-  launch_kernel(cache8_prompt_weights_kernel, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kWThreads), WSmem::kTotal, st, 1, mk, mq, t);
+  launch_kernel(a.softcap > 0.0f ? cache8_prompt_weights_kernel<true> : cache8_prompt_weights_kernel<false>, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kWThreads), WSmem::kTotal, st, 1, mk, mq, t);
   return static_cast<int>(cudaGetLastError());
 }
 
