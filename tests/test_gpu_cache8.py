@@ -273,6 +273,156 @@ def test_an_entry_that_does_not_fit_is_left_out(dtype):
             assert torch.equal(t, b), bad
 
 
+@pytest.mark.parametrize("dtype,shape,lens,weights,want", [
+    (BF, (8, 2, 128, 128, 64), [1, 1], False, {"cache8_attention_kernel"}),
+    (BF, (8, 2, 128, 128, 64), [1, 1], True, {"cache8_attention_kernel", "cache8_weights_kernel"}),
+    (F32, (8, 2, 64, 64, 64), [130, 1], True, {"cache8_attention_kernel", "cache8_rows_weights_kernel"}),
+    (BF, (8, 2, 128, 128, 64), [9, 1], True, {"cache8_attention_kernel", "cache8_rows_weights_kernel"}),
+    (BF, (8, 2, 128, 128, 64), [130, 140], False, {"cache8_widen_kernel", "attention_prefill_kernel", "cache8_nan_kernel"}),
+    (BF, (8, 2, 128, 128, 64), [130, 1], True, {"cache8_widen_kernel", "attention_prefill_kernel", "cache8_nan_kernel", "cache8_prompt_weights_kernel",
+                                                "cache8_attention_kernel", "cache8_rows_weights_kernel"}),
+])
+def test_which_kernels_run(dtype, shape, lens, weights, want):
+    from kernel_names import kernels
+    from teenygrad_b200 import ops
+    heads, kv, dim, vdim, block = shape
+    cache, _ = filled(1, len(lens), kv, 300, dim, vdim, block, weights=weights)
+    table, rows = rows_of(lens, range(len(lens)), [20] * len(lens))
+    on, q = ops.step_table(table), rnd(2, rows, heads, dim).to(dtype).cuda()
+    scratch, out = ops.cache8_attention_scratch(cache, on, q, weights), torch.zeros(rows, heads, vdim, dtype=dtype, device="cuda")
+    got = kernels(lambda: ops.cache8_attention(q, cache, 0.1, on, weight_decay=0.5 if weights else None, out=out, scratch=scratch))
+    assert all(any(w in name for name in got) for w in want) and all(any(w in name for w in want) for name in got), got
+
+
+@DTYPES
+def test_many_entries(dtype):
+    """More entries than a warp counts at once, with empty ones in between, in slots far apart."""
+    from teenygrad_b200 import ops
+    n, slots, heads, kv, dim = 300, 70, 2, 1, 32
+    cache, want = filled(3, slots, kv, 80, dim, dim, 16)
+    table, row = [], 0
+    for i in range(n):
+        m = (1, 0, 2, 1, 1)[i % 5]
+        table.append(((i * 37) % slots, (i * 11) % 78, row, m))
+        row += m
+    q = rnd(4, row, heads, dim).to(dtype)
+    out = ops.cache8_attention(q.cuda(), cache, 0.2, ops.step_table(table))
+    check(out, None, want.attention(q, 0.2, table), dtype, q, dim, 80, 0.0, table)
+
+
+def test_prompts_of_more_entries_than_a_launch_takes():
+    """130 prompts (128 to a launch), a few tokens between them, and slots so long that their widened tokens are held one at a time."""
+    from teenygrad_b200 import ops
+    heads, kv, dim = 6, 1, 16  # (prompts from 32 tokens on)
+    cache, want = filled(5, 130, kv, 40, dim, dim, 16, weights=True)
+    table, rows = rows_of([33 + i % 5 if i % 7 else 3 for i in range(130)], [(i * 3) % 130 for i in range(130)], [i % 3 for i in range(130)])
+    q = rnd(6, rows, heads, dim).to(BF)
+    out = ops.cache8_attention(q.cuda(), cache, 0.2, ops.step_table(table), weight_decay=0.0)
+    ref = want.attention(q, 0.2, table, decay=0.0)
+    check(out, None, ref, BF, q, dim, 40, 0.0, table)
+    for slot, at, _, m in table:
+        a, b = cache.weights[slot, 0, :at + m].double().cpu(), want.weights[slot, 0, :at + m]
+        assert float(((a - b).abs() / (b + 1e-30)).max()) < 1e-4
+    long, plain = filled(7, 3, 2, 40000, 32, 16, 128)
+    table, rows = rows_of([70, 130, 65], [2, 0, 1], [300, 0, 39935])
+    plain.k, plain.v = plain.k[:, :1], plain.v[:, :1]
+    q = rnd(8, rows, 8, 32).to(BF)
+    out = ops.cache8_attention(q.cuda(), long, 0.2, ops.step_table(table))
+    ref = plain.attention(q[:, :4], 0.2, table)  # (the first kv head's query heads)
+    check(out[:, :4], None, ref, BF, q[:, :4], 32, 40000, 0.0, table)
+
+
+@DTYPES
+@pytest.mark.parametrize("n", [1, 70])
+def test_a_cache_of_more_than_four_billion_bytes(dtype, n):
+    """The last slot of a cache whose offsets need more than 32 bits: append, attention, eviction."""
+    from teenygrad_b200 import ops
+    heads, kv, dim, slots, cap = 4, 2, 128, 3, 6_000_000
+    cache = ops.cache8(slots, kv, cap, dim, 16, 128, weights=True)
+    want = oc.Cache(torch.zeros(1, kv, n + 9, dim, dtype=torch.uint8), torch.zeros(1, kv, n + 9, 16, dtype=torch.uint8), torch.zeros(1, kv, 1), torch.zeros(1, kv, 1),
+                    128, torch.zeros(1, kv, n + 9))
+    q, k, v = (rnd(90 + i, n, h, d).to(dtype) for i, (h, d) in enumerate(((heads, dim), (kv, dim), (kv, 16))))
+    far, near = ops.step_table([(2, 0, 0, n)]), [(0, 0, 0, n)]
+    ops.cache8_append(cache, k.cuda(), v.cuda(), far)
+    want.append(k, v, near)
+    out = ops.cache8_attention(q.cuda(), cache, 0.1, far, weight_decay=0.0)
+    check(out, None, want.attention(q, 0.1, near, decay=0.0), dtype, q, dim, n, 0.0, near)
+    assert float((cache.weights[2, :, :n].double().cpu() - want.weights[0, :, :n]).abs().max()) < 1e-4
+    want.weights[0, :, :n] = cache.weights[2, :, :n].double().cpu()
+    kept = ops.cache8_evict(cache, ops.step_table([(2, n, 0, 0)]), max(1, n // 2), n // 8)
+    assert torch.equal(kept.cpu(), want.evict([(0, n, 0, 0)], max(1, n // 2), n // 8))
+    assert torch.equal(cache.k[2, :, :n].view(torch.uint8).cpu() & 127, want.k[0, :, :n] & 127)
+    del cache
+    torch.cuda.empty_cache()
+
+
+@DTYPES
+@pytest.mark.parametrize("offset", [0, 1, 2])
+@pytest.mark.parametrize("lens", [[1, 1], [5, 150]])
+def test_views_of_queries_outputs_and_gates(dtype, offset, lens):
+    """Rows inside wider ones, and rows that do not start on 16 bytes."""
+    from teenygrad_b200 import ops
+    heads, kv, dim, vdim = 4, 2, 64, 48
+    cache, want = filled(9, 2, kv, 200, dim, vdim, 32)
+    table, rows = rows_of(lens, [1, 0], [40, 7])
+    wide = rnd(10, rows, heads * (dim + 2 * vdim) + 8 + offset).to(dtype).cuda()
+    q = wide[:, offset:offset + heads * dim].unflatten(1, (heads, dim))
+    out = wide[:, offset + heads * dim:offset + heads * (dim + vdim)].unflatten(1, (heads, vdim))
+    gate = wide[:, offset + heads * (dim + vdim):offset + heads * (dim + 2 * vdim)]
+    qc, gc, rest = q.cpu().clone(), gate.cpu().clone(), wide[:, offset + heads * (dim + 2 * vdim):].clone()
+    ops.cache8_attention(q, cache, 0.1, ops.step_table(table), gate=gate, out=out)
+    check(out, None, want.attention(qc, 0.1, table, gate=gc), dtype, qc, dim, 200, 0.0, table)
+    assert torch.equal(q.cpu(), qc) and torch.equal(gate.cpu(), gc) and torch.equal(rest, wide[:, offset + heads * (dim + 2 * vdim):])
+
+
+@DTYPES
+@pytest.mark.parametrize("lens", [[1, 3], [140, 2]])
+def test_without_the_hosts_table(dtype, lens):
+    """The C entry points with the table on the device alone: the same bits."""
+    from teenygrad_b200 import ops
+    from teenygrad_b200._lib import lib
+    heads, kv, dim = 8, 2, 64
+    cache, _ = filled(11, 2, kv, 200, dim, dim, 32)
+    table, rows = rows_of(lens, [1, 0], [40, 7])
+    on, q = ops.step_table(table), rnd(12, rows, heads, dim).to(dtype).cuda()
+    scratch = ops.cache8_attention_scratch(cache, on, q)
+    want, got = ops.cache8_attention(q, cache, 0.1, on, scratch=scratch), torch.zeros(rows, heads, dim, dtype=dtype, device="cuda")
+    args = [int(dtype == F32), *cache._at, None, 0.0, q.data_ptr(), heads * dim, got.data_ptr(), heads * dim, rows, heads, 0.1, 0.0, None, None, 0, None,
+            scratch.data_ptr(), scratch.numel(), on.seqs.data_ptr(), None, on.n, on.longest, ops._stream()]
+    assert lib.teeny_cache8_attention(*args) == 0
+    assert torch.equal(want, got)
+
+
+@DTYPES
+@pytest.mark.parametrize("lens", [[1, 1, 1], [4, 140, 1]])
+def test_the_same_call_gives_the_same_bits(dtype, lens):
+    from teenygrad_b200 import ops
+    cache, _ = filled(13, 3, 2, 900, 128, 128, 64, weights=True)
+    table, rows = rows_of(lens, [1, 0, 2], [700, 300, 5])
+    on, q = ops.step_table(table), rnd(14, rows, 8, 128).to(dtype).cuda()
+    scratch = ops.cache8_attention_scratch(cache, on, q, True)
+    first = ops.cache8_attention(q, cache, 0.1, on, weight_decay=0.0, scratch=scratch)
+    w = cache.weights.clone()
+    for _ in range(20):
+        assert torch.equal(ops.cache8_attention(q, cache, 0.1, on, weight_decay=0.0, scratch=scratch), first) and torch.equal(cache.weights, w)
+
+
+def test_a_soft_cap_far_above_the_scores():
+    """tanh near zero: the capped scores are the scores, up to f32's roundings."""
+    from teenygrad_b200 import ops
+    for lens in ([1, 1], [120, 1]):
+        cache, want = filled(15, 2, 2, 200, 64, 64, 32, weights=True)
+        table, rows = rows_of(lens, [1, 0], [60, 150])
+        for dtype in (F32, BF):
+            q = rnd(16, rows, 8, 64).to(dtype)
+            ops.cache8_attention(q.cuda(), cache, 0.1, ops.step_table(table), softcap=3e4, weight_decay=0.0)
+            ref = want.attention(q, 0.1, table, 3e4, decay=0.0)
+            near = float(bounds(dtype, ref, q, 64, 200, 0.0)[2].max()) + (rows * 4 + 4) * 2.0 ** -24  # (no term for the cap)
+            for slot, at, _, m in table:
+                a, b = cache.weights[slot, :, :at + m].double().cpu(), want.weights[slot, :, :at + m]
+                assert float(((a - b).abs() / b).max()) < near
+
+
 # ------------------------------------------------------------------------------------------------ evict
 @pytest.mark.parametrize("block", [16, 64, 128])
 @pytest.mark.parametrize("keep,recent", [(1, 0), (1, 1), (50, 0), (50, 50), (130, 17), (299, 5), (300, 10)])
@@ -299,6 +449,21 @@ def test_evict_ties_and_weights_that_are_not_numbers():
     table = [(1, 4999, 0, 0), (0, 5000, 0, 0)]
     kept = ops.cache8_evict(cache, ops.step_table(table), 1500, 100)
     assert torch.equal(kept.cpu(), want.evict(table, 1500, 100))
+    same(cache, want)
+
+
+@pytest.mark.parametrize("n,keep,recent", [(3000, 2999, 7), (17000, 40, 0), (40000, 20000, 64)])
+def test_evict_long(n, keep, recent):
+    """Candidates that a thread holds 16 of, and more than it holds at all; pieces that wait for many others."""
+    from teenygrad_b200 import ops
+    cache, want = filled(n, 2, 1, n, 32, 16, 128, weights=True)
+    w = torch.exp(2 * rnd(1, 2, 1, n))
+    w[:, :, 3:n // 2:2] = 0.25  # (many equal ones around the border)
+    want.weights.copy_(w)
+    cache.weights.copy_(w)
+    table = [(1, n, 0, 0), (0, n - 1, 0, 0)]
+    kept = ops.cache8_evict(cache, ops.step_table(table), keep, recent)
+    assert torch.equal(kept.cpu(), want.evict(table, keep, recent))
     same(cache, want)
 
 
