@@ -110,13 +110,16 @@ __device__ __forceinline__ EntryShape entry_shape(const Shared& s, const SeqDesc
   e.all = e.slices * e.groups * s.c.H;
   return e;
 }
-// How the slices are shared: none of `parts` CTAs takes less than a slice for each warp, nor are there many more than 64 to a unit, whose parts have to
-// be added again.  The first `more` CTAs take one slice more than the others' `each`.
+// How the slices are shared.  With many units each of the CTAs takes the same number of consecutive slices, whatever units they are of: the first `more`
+// take one more than the others' `each`.  With few, a unit is cut into parts of `cut` slices and each CTA takes one: the end of a unit inside a
+// share costs a CTA 5000 clocks.  No share is less than a slice for each warp (unless its unit is), nor are there many more than 64 to a
+// unit, whose parts have to be added again.
 struct Shares {
-  int parts, each, more;
+  int parts, each, more, cut;
   __device__ __forceinline__ Shares(int most, int total, int units) {
-    const int least = max(kWarps, total / 64 / units), all = (total + least - 1) / least;
-    parts = min(most, all);
+    const int least = max(kWarps, total / 64 / units);
+    cut = units * 4 <= most ? max(least, (total + most - units - 1) / (most - units)) : 0;
+    parts = min(most, max((total + least - 1) / least, min(units, total)));
     each = total / parts;
     more = total - parts * each;
   }
@@ -125,6 +128,7 @@ struct Shares {
     const int big = more * (each + 1);
     return slice < big ? slice / (each + 1) : more + (slice - big) / each;
   }
+  __device__ __forceinline__ int cuts(int slices) const { return (slices + cut - 1) / cut; }
 };
 
 __device__ __forceinline__ int warp_sum_int(int v) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(v))); }
@@ -248,16 +252,15 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t ring = base + warp * (ST * kStage), bars = base + V::kBars + warp * (ST * 8), scale_at = base + V::kScales + warp * (ST * 16);
-  // parts that this CTA has left: of its first and of its last unit (entry, head, row group, slices, first slice of all)
-  __shared__ struct Left { int begin, e, hk, rg, slices; } sm_left[2];
-  __shared__ int sm_c0[2], sm_c1[2];  // CTAs whose parts are to be added here (none: c1 < c0)
+  // units of which this CTA has left a part: its first and its last
+  __shared__ struct Left { int c0, c1, slot0, e, hk, rg; } sm_left[2];  // c0 .. c1: the CTAs that have parts of it (none: c1 < c0)
   if (lane == 0) {
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
     for (int st = 0; st < ST; ++st) mbar_init(bars + 8 * st, 1 + 4);
     mbar_fence_init();
   }
-  if (threadIdx.x < 2) sm_left[threadIdx.x].slices = 0;
+  if (threadIdx.x < 2) sm_left[threadIdx.x] = Left{0, -1, 0, 0, 0, 0};
   __syncwarp();
   pdl_wait();
   // ---- this CTA's share (each warp works it out) ----
@@ -273,13 +276,19 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   units = warp_sum_int(units);
   if (total == 0) return;
   const Shares shares(s.parts, total, units);
-  if (part >= shares.parts) return;
-  const int t0 = shares.begin(part), share = shares.begin(part + 1) - t0;
+  // (counted in slices, or with cut units in their parts)
+  const int t0 = shares.cut ? part : part < shares.parts ? shares.begin(part) : total;
+  int share, cuts = 1;
   Piece p;
   {
     int before = 0, at = 0, found = -1;
     for (int e0 = 0; found < 0; e0 += 32) {
+      if (e0 >= s.n_seqs) return;  // nothing is left for this CTA
       if (e0 > 0) mine = e0 + lane < s.n_seqs ? entry_shape(s, s.seqs[e0 + lane], R).all : 0;
+      if (shares.cut && mine > 0) {
+        const EntryShape es = entry_shape(s, s.seqs[e0 + lane], R);
+        mine = shares.cuts(es.slices) * es.groups * s.c.H;
+      }
       int run = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -299,11 +308,13 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     const EntryShape es = entry_shape(s, p.sq, R);
     p.slices = es.slices;
     p.groups = es.groups;
-    const int unit = at / es.slices;
+    if (shares.cut) cuts = shares.cuts(es.slices);
+    const int per_unit = shares.cut ? cuts : es.slices, unit = at / per_unit, inside = at - unit * per_unit;
     p.hk = unit / es.groups;
     p.rg = unit - p.hk * es.groups;
     p.first = true;
-    piece_range(s, p, R, at - unit * es.slices, share);
+    share = shares.cut ? min(shares.cut, es.slices - inside * shares.cut) : shares.begin(part + 1) - t0;
+    piece_range(s, p, R, shares.cut ? inside * shares.cut : inside, share);
   }
   pdl_trigger();
   // Row g of the row tile that this warp makes ready (with one, every warp does): the first piece's is asked for in front of the cache's slices, behind
@@ -618,7 +629,19 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     __syncthreads();
     if (warp < 2) pass(true);
     __syncthreads();
-    if (!p.whole && threadIdx.x == 0) sm_left[p.first ? 0 : 1] = Left{unit_begin, p.e, p.hk, p.rg, p.slices};
+    if (!p.whole && threadIdx.x == 0) {
+      Left u{0, 0, 0, p.e, p.hk, p.rg};
+      if (shares.cut) {
+        u.c0 = part - p.j / shares.cut;
+        u.c1 = u.c0 + cuts - 1;
+        u.slot0 = 2 * u.c0;
+      } else {
+        u.c0 = shares.owner(unit_begin);
+        u.c1 = shares.owner(unit_begin + p.slices - 1);
+        u.slot0 = 2 * u.c0 + (shares.begin(u.c0) == unit_begin ? 0 : 1);
+      }
+      sm_left[p.first ? 0 : 1] = u;
+    }
     const int rows = min(R, p.sq.len * s.G - p.rg * R);
 #pragma unroll 1
     for (int r_in = warp; r_in < rows; r_in += kWarps) {  // (a lane: four dimensions)
@@ -661,25 +684,20 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   __syncthreads();
   if (threadIdx.x < 2) {
     const Left u = sm_left[threadIdx.x];
-    int c0 = 0, c1 = -1;
-    if (u.slices > 0) {
-      c0 = shares.owner(u.begin);
-      c1 = shares.owner(u.begin + u.slices - 1);
+    if (u.c1 > u.c0) {
       __threadfence();
       // (the counter goes back to zero with the last arrival)
-      if (atomicInc(s.arrivals + (static_cast<size_t>(u.e) * s.c.H + u.hk) * s.max_groups + u.rg, c1 - c0) != static_cast<unsigned>(c1 - c0)) c1 = -1;
+      if (atomicInc(s.arrivals + (static_cast<size_t>(u.e) * s.c.H + u.hk) * s.max_groups + u.rg, u.c1 - u.c0) != static_cast<unsigned>(u.c1 - u.c0))
+        sm_left[threadIdx.x].c1 = -1;
       __threadfence();
     }
-    sm_c0[threadIdx.x] = c0;
-    sm_c1[threadIdx.x] = c1;
   }
   __syncthreads();
   for (int k = 0; k < 2; ++k) {
-    const int c0 = sm_c0[k], c1 = sm_c1[k];
-    if (c1 < c0) continue;
     const Left u = sm_left[k];
+    const int c0 = u.c0, c1 = u.c1, slot0 = u.slot0;
+    if (c1 <= c0) continue;
     const SeqDesc sq = s.seqs[u.e];
-    const int slot0 = 2 * c0 + (shares.begin(c0) == u.begin ? 0 : 1);
     const int rows = min(R, sq.len * s.G - u.rg * R);
     // eight parts at a time: of a row, with more than four rows of two
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -770,84 +788,99 @@ __global__ void __launch_bounds__(256) cache8_weights_kernel(const __grid_consta
   }
 }
 
-// Weights of calls with several tokens: the scores once more, from the rows' lse.  A warp takes 32 keys of a (kv head, entry) and goes through the
-// rows, eight at a time.
+// Weights of calls with several tokens: the scores once more, from the rows' lse.  WR of a CTA's eight warps take the same 32 keys of a (kv head, entry),
+// each every WR-th eight of the rows, and add their sums through shared memory.
 template <typename T>
-__global__ void __launch_bounds__(128) cache8_rows_weights_kernel(const __grid_constant__ Shared s) {
+__global__ void __launch_bounds__(256) cache8_rows_weights_kernel(const __grid_constant__ Shared s, int WR) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  __shared__ float sums[8][32];
   pdl_wait();
   const int e = blockIdx.z, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const SeqDesc sq = s.seqs[e];
   if (!cache8_fits(sq, s.c, s.a.rows, s.max_len)) return;
-  const int live = sq.pos + sq.len;
+  const int live = sq.pos + sq.len, rows = sq.len * s.G, at_once = 8 / WR;
   const size_t head = static_cast<size_t>(sq.slot) * s.c.H + hk;
-  for (int kb = (blockIdx.x * 4 + warp) * 32; kb < live; kb += gridDim.x * 128) {
-    uint32_t ka[2][8][4];  // the keys' A fragments
-    float ks[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int key = kb + 16 * u + 8 * half + g;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int d0 = 16 * (2 * c + h);
-          const uint4 w = key < live && d0 < s.c.D ? *reinterpret_cast<const uint4*>(s.c.k + (head * s.c.cap + key) * s.c.D + d0) : make_uint4(0u, 0u, 0u, 0u);
-          widen(w.x, ka[u][4 * h][half], ka[u][4 * h][2 + half]);
-          widen(w.y, ka[u][4 * h + 1][half], ka[u][4 * h + 1][2 + half]);
-          widen(w.z, ka[u][4 * h + 2][half], ka[u][4 * h + 2][2 + half]);
-          widen(w.w, ka[u][4 * h + 3][half], ka[u][4 * h + 3][2 + half]);
-        }
-      }
-    ks[0] = s.c.ks[head * s.c.blocks + (kb >> s.c.shift)];
-    ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + ((kb + 16) >> s.c.shift)] : 0.0f;
+  for (int first = blockIdx.x * at_once; first * kSlice < live; first += gridDim.x * at_once) {
+    const int kb = (first + warp / WR) * kSlice;
     float sum[4] = {};
-    const int rows = sq.len * s.G;
-    for (int r0 = max(0, kb - sq.pos) * s.G / 8 * 8; r0 < rows; r0 += 8) {
-      const int r = r0 + g, at = min(r, rows - 1), i = at / s.G, hq = hk * s.G + at - i * s.G;
-      const size_t row = static_cast<size_t>(sq.row0) + i;
-      uint32_t term[TERMS][16];
-      float raw[32];
-      load_row(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c, raw);
-      const float f = split_row<TERMS>(raw, s.scale_log2, term);
-      const float lse = s.lse2[row * s.a.Hq + hq];
-      const int see = r < rows ? sq.pos + i + 1 - kb : 0;
-      float factor[2], z2[2];
-      int sees[2];
+    if (kb < live) {
+      uint32_t ka[2][8][4];  // the keys' A fragments
+      float ks[2];
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        factor[z] = __shfl_sync(0xffffffffu, f, (2 * c + z) * 4);
-        z2[z] = __shfl_sync(0xffffffffu, lse, (2 * c + z) * 4);
-        sees[z] = __shfl_sync(0xffffffffu, see, (2 * c + z) * 4);
-      }
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float d[TERMS][4] = {};
+        for (int half = 0; half < 2; ++half) {
+          const int key = kb + 16 * u + 8 * half + g;
 #pragma unroll
-        for (int step = 0; step < 8; ++step)
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-            mma_f16_16816(d[t], ka[u][step][0], ka[u][step][1], ka[u][step][2], ka[u][step][3], term[t][2 * step], term[t][2 * step + 1]);
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            float v = d[0][2 * half + z];
-            if (TERMS == 2) v = fmaf(d[TERMS - 1][2 * half + z], 1.0f / 2048.0f, v);
-            v *= factor[z] * ks[u];
-            if (s.cap_l2 > 0.0f) v = cap_score(v, s.one_over_cap, s.cap_l2);
-            if (16 * u + 8 * half + g < sees[z]) sum[2 * u + half] += ex2(v - z2[z]);
+          for (int h = 0; h < 2; ++h) {
+            const int d0 = 16 * (2 * c + h);
+            const uint4 w = key < live && d0 < s.c.D ? *reinterpret_cast<const uint4*>(s.c.k + (head * s.c.cap + key) * s.c.D + d0) : make_uint4(0u, 0u, 0u, 0u);
+            widen(w.x, ka[u][4 * h][half], ka[u][4 * h][2 + half]);
+            widen(w.y, ka[u][4 * h + 1][half], ka[u][4 * h + 1][2 + half]);
+            widen(w.z, ka[u][4 * h + 2][half], ka[u][4 * h + 2][2 + half]);
+            widen(w.w, ka[u][4 * h + 3][half], ka[u][4 * h + 3][2 + half]);
           }
+        }
+      ks[0] = s.c.ks[head * s.c.blocks + (kb >> s.c.shift)];
+      ks[1] = kb + 16 < live ? s.c.ks[head * s.c.blocks + ((kb + 16) >> s.c.shift)] : 0.0f;
+      float raw[32], lse = 0.0f;
+      int see = 0;  // keys of the slice that the row sees
+      auto ask = [&](int r0) {
+        const int r = r0 + g, at = min(r, rows - 1), i = at / s.G, hq = hk * s.G + at - i * s.G;
+        const size_t row = static_cast<size_t>(sq.row0) + i;
+        load_row(static_cast<const T*>(s.a.q) + row * s.a.ldq + static_cast<size_t>(hq) * s.c.D, s.c.D, r < rows, s.vec_q, c, raw);
+        lse = s.lse2[row * s.a.Hq + hq];
+        see = r < rows ? sq.pos + i + 1 - kb : 0;
+      };
+      int r0 = max(0, kb - sq.pos) * s.G / 8 * 8 + 8 * (warp % WR);
+      if (r0 < rows) ask(r0);
+      for (; r0 < rows; r0 += 8 * WR) {
+        uint32_t term[TERMS][16];
+        const float f = split_row<TERMS>(raw, s.scale_log2, term);
+        float factor[2], z2[2];
+        int sees[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          factor[z] = __shfl_sync(0xffffffffu, f, (2 * c + z) * 4);
+          z2[z] = __shfl_sync(0xffffffffu, lse, (2 * c + z) * 4);
+          sees[z] = __shfl_sync(0xffffffffu, see, (2 * c + z) * 4);
+        }
+        if (r0 + 8 * WR < rows) ask(r0 + 8 * WR);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float d[TERMS][4] = {};
+#pragma unroll
+          for (int step = 0; step < 8; ++step)
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t)
+              mma_f16_16816(d[t], ka[u][step][0], ka[u][step][1], ka[u][step][2], ka[u][step][3], term[t][2 * step], term[t][2 * step + 1]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              float v = d[0][2 * half + z];
+              if (TERMS == 2) v = fmaf(d[TERMS - 1][2 * half + z], 1.0f / 2048.0f, v);
+              v *= factor[z] * ks[u];
+              if (s.cap_l2 > 0.0f) v = cap_score(v, s.one_over_cap, s.cap_l2);
+              if (16 * u + 8 * half + g < sees[z]) sum[2 * u + half] += ex2(v - z2[z]);
+            }
+        }
       }
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 1);
       sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 2);
-      const int key = kb + 8 * t + g;
-      float* w = s.c.w + head * s.c.cap + key;
-      if (c == 0 && key < live) *w = s.a.decay == 0.0f ? sum[t] : fmaf(s.a.decay, *w, sum[t]);
+      if (c == 0) sums[warp][8 * t + g] = sum[t];
     }
+    __syncthreads();
+    if (warp % WR == 0 && kb + lane < live) {
+      float all = 0.0f;
+      for (int w = 0; w < WR; ++w) all += sums[warp + w][lane];
+      float* w = s.c.w + head * s.c.cap + kb + lane;
+      *w = s.a.decay == 0.0f ? all : fmaf(s.a.decay, *w, all);
+    }
+    __syncthreads();
   }
 }
 
@@ -990,11 +1023,14 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
     });
   if (a.weights && any_short) {
     const PdlScope behind;
-    const int shares = call_len == 1 ? (c.cap + 1023) / 1024 : (c.cap + 127) / 128, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
+    // warps for the same keys: as many as share rows usefully
+    const long long eights = (static_cast<long long>(s.G) * max_len + 7) / 8;
+    const int WR = eights >= 8 ? 8 : eights >= 4 ? 4 : eights >= 2 ? 2 : 1, keys = call_len == 1 ? 1024 : 8 / WR * kSlice;
+    const int shares = (c.cap + keys - 1) / keys, most = (4 * sm_count() + n_seqs * c.H - 1) / (n_seqs * c.H);
     const dim3 grid(shares < most ? shares : most, c.H, n_seqs);
     if (call_len == 1) launch_kernel(cache8_weights_kernel, grid, dim3(256), 0, st, 1, s);
-    else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float>, grid, dim3(128), 0, st, 1, s);
-    else launch_kernel(cache8_rows_weights_kernel<bf16>, grid, dim3(128), 0, st, 1, s);
+    else if (a.f32) launch_kernel(cache8_rows_weights_kernel<float>, grid, dim3(256), 0, st, 1, s, WR);
+    else launch_kernel(cache8_rows_weights_kernel<bf16>, grid, dim3(256), 0, st, 1, s, WR);
   }
   return static_cast<int>(cudaGetLastError());
 }
