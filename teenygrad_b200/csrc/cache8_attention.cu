@@ -461,49 +461,63 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
               for (int z = 0; z < 4; ++z) acc[nt][j][z] *= down;
         }
         const float inv = vref > 0.0f ? 16384.0f / vref : 0.0f, r0 = vs0 * inv, r1 = vs1 * inv;
-        uint32_t pb[NT][4];  // B fragments of the values' product, by blocks of eight keys
+        float y[RT][4][2];  // [row tile][keys 8 t + g][rows 2c, 2c + 1]
+        bool grows = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          float y[4][2];  // [keys 8 t + g][rows 2c, 2c + 1]
 #pragma unroll
           for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               float v = x[rt * TERMS][t >> 1][2 * (t & 1) + z];
               if (TERMS == 2) v = fmaf(x[rt * TERMS + TERMS - 1][t >> 1][2 * (t & 1) + z], 1.0f / 2048.0f, v);
-              y[t][z] = v * (factor[rt][z] * (t < 2 ? ks0 : ks1));
+              y[rt][t][z] = v * (factor[rt][z] * (t < 2 ? ks0 : ks1));
             }
-          if (s.cap_l2 > 0.0f) {
+        }
+        if (s.cap_l2 > 0.0f) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) y[t][z] = cap_score(y[t][z], s.one_over_cap, s.cap_l2);
-          }
-          if (masked) {
+              for (int z = 0; z < 2; ++z) y[rt][t][z] = cap_score(y[rt][t][z], s.one_over_cap, s.cap_l2);
+        }
+        if (masked) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) y[t][z] = kb + 8 * t + g < rows_limit[rt][z] ? y[t][z] : -INFINITY;
-          }
-          if (s.scores) {
+              for (int z = 0; z < 2; ++z) y[rt][t][z] = kb + 8 * t + g < rows_limit[rt][z] ? y[rt][t][z] : -INFINITY;
+        }
+        if (s.scores) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const int r = p.rg * R + rt * 8 + 2 * c + z;  // (single tokens: a row is a query head of the group)
               float* to = s.scores + (static_cast<size_t>(p.e) * s.a.Hq + p.hk * s.G + r) * s.score_row + kb + g;
 #pragma unroll
               for (int t = 0; t < 4; ++t)
-                if (r < s.G && kb + 8 * t + g < p.limit) to[8 * t] = y[t][z];
+                if (r < s.G && kb + 8 * t + g < p.limit) to[8 * t] = y[rt][t][z];
             }
-          }
-          float top[2];
+        }
+        float top[RT][2];
 #pragma unroll
-          for (int z = 0; z < 2; ++z) top[z] = fmaxf(fmaxf(y[0][z], y[1][z]), fmaxf(y[2][z], y[3][z]));
-          if (__any_sync(0xffffffffu, top[0] > m[rt][0] || top[1] > m[rt][1])) {  // (rare once a sequence is under way)
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            top[rt][z] = fmaxf(fmaxf(y[rt][0][z], y[rt][1][z]), fmaxf(y[rt][2][z], y[rt][3][z]));
+            grows = grows || top[rt][z] > m[rt][z];
+          }
+        if (__any_sync(0xffffffffu, grows)) {  // (rare once a sequence is under way; one test for all rows leaves straight-line code)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) top[z] = fmaxf(top[z], __shfl_xor_sync(0xffffffffu, top[z], o));
-              const float m_new = fmaxf(m[rt][z], top[z]), alpha = ex2(m[rt][z] - (m_new == -INFINITY ? 0.0f : m_new));
+              for (int o = 4; o < 32; o <<= 1) top[rt][z] = fmaxf(top[rt][z], __shfl_xor_sync(0xffffffffu, top[rt][z], o));
+              const float m_new = fmaxf(m[rt][z], top[rt][z]), alpha = ex2(m[rt][z] - (m_new == -INFINITY ? 0.0f : m_new));
               m[rt][z] = m_new;
               l[rt][z] *= alpha;
 #pragma unroll
@@ -514,22 +528,24 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                   acc[rt * TERMS + t][j][2 + z] *= alpha;
                 }
             }
-          }
+        }
+        uint32_t pb[NT][4];  // B fragments of the values' product, by blocks of eight keys
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
             const float from = m[rt][z] == -INFINITY ? 0.0f : m[rt][z];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              y[t][z] = ex2(y[t][z] - from);
-              l[rt][z] += y[t][z];
-              y[t][z] *= t < 2 ? r0 : r1;
-            }
+            for (int t = 0; t < 4; ++t) y[rt][t][z] = ex2(y[rt][t][z] - from);
+            l[rt][z] += (y[rt][0][z] + y[rt][1][z]) + (y[rt][2][z] + y[rt][3][z]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) y[rt][t][z] *= t < 2 ? r0 : r1;
           }
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            const uint32_t two = pack_f16x2(y[t][0], y[t][1]);
+            const uint32_t two = pack_f16x2(y[rt][t][0], y[rt][t][1]);
             pb[rt * TERMS][t] = transposed(two);
-            if (TERMS == 2) pb[rt * TERMS + TERMS - 1][t] = transposed(rest_f16x2(two, y[t][0], y[t][1]));
+            if (TERMS == 2) pb[rt * TERMS + TERMS - 1][t] = transposed(rest_f16x2(two, y[rt][t][0], y[rt][t][1]));
           }
         }
         // ---- values: lane (g, c) reads the dimensions 16 g .. 16 g + 15 of the keys 2c, 2c + 1 of the four blocks; pairs of keys by bytes, then
