@@ -33,6 +33,8 @@ typedef struct {
   int slots, kv_heads, max_cached, dim, vdim, block;
 } teeny_cache8_shape;
 
+enum { TEENY_CACHE8_COUNTER_BYTES = 4096 };
+
 /* Tokens k [rows, ldk], v [rows, ldv] of every entry into the cache, at its position and behind.  A block that holds older tokens of
  * the entry (those before its position) keeps at least its scale, and they are rounded to the new one; what a block held at or behind
  * the entry's position does not count.  NaN and infinities become NaN and do not count for the scale.  weights (or null) are set to zero for the new tokens. */
@@ -47,10 +49,10 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
  * weights <- weight_decay * weights + the probabilities that the entry's tokens and query heads gave it; with weight_decay 0 what
  * was there is not read.  The gate does not count there.  Rows of out that belong to no entry stay as they are.  Sums are made in
  * a fixed order: the same call gives the same bits.
- * scratch: its first teeny_cache8_attention_zeroed_bytes bytes (counters) are zero before the first call, and every call leaves them zero. */
+ * scratch: its first TEENY_CACHE8_COUNTER_BYTES are zero before the first call, and every call leaves them zero (after a device error they have to be
+ * made zero again).  Calls of any sizes may share it, evictions among them, as long as they follow one another.  out must not overlap q. */
 size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int f32, int heads, int rows, int n_seqs, int max_len,
                                             int with_weights);
-size_t teeny_cache8_attention_zeroed_bytes(const teeny_cache8_shape* shape, int f32, int heads, int n_seqs, int max_len);
 int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void* k, const void* v, const float* k_scale,
                            const float* v_scale, float* weights, float weight_decay, const void* q, long long ldq, void* out,
                            long long ldo, int rows, int heads, float score_scale, float softcap, const float* sink, const void* gate,

@@ -210,6 +210,7 @@ pub const TEENY_HYBRID_BUF_HISTORY: c_int = 2;
 pub const TEENY_HYBRID_BUF_STATE: c_int = 3;
 pub const TEENY_HYBRID_BUF_RESIDUAL: c_int = 4;
 pub const TEENY_HYBRID_BUF_LAST_DELTA: c_int = 5;
+pub const TEENY_CACHE8_COUNTER_BYTES: c_int = 4096;
 #[link(name = "teeny_b200")]
 extern "C" {
     pub fn teeny_version() -> c_int;
@@ -302,7 +303,6 @@ extern "C" {
     pub fn teeny_latent_attention(f32: c_int, q: *const c_void, ldq: c_longlong, rows: c_int, cache: *const c_void, slots: c_int, max_cached: c_int, out: *mut c_void, ldo: c_longlong, heads: c_int, dim: c_int, vdim: c_int, score_scale: f32, scratch: *mut c_void, scratch_bytes: usize, seqs: *const c_int, n_seqs: c_int, max_len: c_int, stream: CUstream) -> c_int;
     pub fn teeny_cache8_append(f32: c_int, shape: *const TeenyCache8Shape, k: *mut c_void, v: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, weights: *mut f32, k_new: *const c_void, ldk: c_longlong, v_new: *const c_void, ldv: c_longlong, rows: c_int, seqs: *const c_int, host_seqs: *const c_int, n_seqs: c_int, max_len: c_int, stream: CUstream) -> c_int;
     pub fn teeny_cache8_attention_scratch_bytes(shape: *const TeenyCache8Shape, f32: c_int, heads: c_int, rows: c_int, n_seqs: c_int, max_len: c_int, with_weights: c_int) -> usize;
-    pub fn teeny_cache8_attention_zeroed_bytes(shape: *const TeenyCache8Shape, f32: c_int, heads: c_int, n_seqs: c_int, max_len: c_int) -> usize;
     pub fn teeny_cache8_attention(f32: c_int, shape: *const TeenyCache8Shape, k: *const c_void, v: *const c_void, k_scale: *const f32, v_scale: *const f32, weights: *mut f32, weight_decay: f32, q: *const c_void, ldq: c_longlong, out: *mut c_void, ldo: c_longlong, rows: c_int, heads: c_int, score_scale: f32, softcap: f32, sink: *const f32, gate: *const c_void, ldg: c_longlong, lse: *mut f32, scratch: *mut c_void, scratch_bytes: usize, seqs: *const c_int, host_seqs: *const c_int, n_seqs: c_int, max_len: c_int, stream: CUstream) -> c_int;
     pub fn teeny_cache8_evict_scratch_bytes(shape: *const TeenyCache8Shape, n_seqs: c_int, keep: c_int) -> usize;
     pub fn teeny_cache8_evict(shape: *const TeenyCache8Shape, k: *mut c_void, v: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, weights: *mut f32, keep: c_int, recent: c_int, kept: *mut c_int, scratch: *mut c_void, scratch_bytes: usize, seqs: *const c_int, host_seqs: *const c_int, n_seqs: c_int, stream: CUstream) -> c_int;

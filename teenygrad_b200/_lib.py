@@ -91,7 +91,6 @@ SIGNATURES = {
     # the 8-bit key/value cache (include/teeny_cache8.h)
     "teeny_cache8_append": (i32, [i32, vp] + [vp] * 5 + [vp, i64, vp, i64, i32, vp, vp, i32, i32, vp]),
     "teeny_cache8_attention_scratch_bytes": (sz, [vp] + [i32] * 6),
-    "teeny_cache8_attention_zeroed_bytes": (sz, [vp] + [i32] * 4),
     "teeny_cache8_attention": (i32, [i32, vp] + [vp] * 5 + [f32, vp, i64, vp, i64, i32, i32, f32, f32, vp, vp, i64, vp,
                                      vp, sz, vp, vp, i32, i32, vp]),
     "teeny_cache8_evict_scratch_bytes": (sz, [vp, i32, i32]),

@@ -218,8 +218,8 @@ struct EvictScratch {
 };
 
 // The kept tokens of one (entry, head), in order.  The smallest kept weight is found by digits, 11, 11 and 10 bits from the top: a histogram of
-// the next digit of the keys that agree with the digits found so far.  Each warp has a stretch of the candidates, in registers up to 32 PER of them (PER 0:
-// read again for every digit).
+// the next digit of the keys that agree with the digits found so far.  Each warp has a stretch of the candidates, in registers up to 32 PER of them (of
+// more they are read again for every digit).
 template <int PER>
 __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8 c, int keep, int recent, int* kept, const EvictScratch x, const SeqDesc* seqs) {
   __shared__ int hist[kBins], sums[32], found[2], warp_gt[32], warp_eq[32];
@@ -240,12 +240,13 @@ __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8
   const float* w = c.w + (static_cast<size_t>(sq.slot) * c.H + head) * c.cap;
   const int cand = len - recent, want = keep - recent;
   const int stretch = (cand + 1023) / 1024 * 32, first = min(cand, warp * stretch), last = min(cand, first + stretch);
-  unsigned own[PER > 0 ? PER : 1];
+  const bool held = stretch <= 32 * PER;
+  unsigned own[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) own[i] = first + 32 * i + lane < last ? order_key(w[first + 32 * i + lane]) : 0u;
   // f(key, place, there) for this lane's candidates; every lane of the warp is there each time
   auto each = [&](auto&& f) {
-    if constexpr (PER > 0) {
+    if (held) {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
         if (first + 32 * i < last) f(own[i], first + 32 * i + lane, first + 32 * i + lane < last);
@@ -453,20 +454,22 @@ int cache8_append(const Cache8& c, const Cache8Append& a, const SeqDesc* seqs, i
 }
 
 size_t cache8_evict_scratch_bytes(const Cache8& c, int n_seqs, int keep) {
-  return 256 + static_cast<size_t>((keep + kMove - 1) / kMove) * n_seqs * 2 * c.H * 4;
+  return TEENY_CACHE8_COUNTER_BYTES + 256 + static_cast<size_t>((keep + kMove - 1) / kMove) * n_seqs * 2 * c.H * 4;
 }
 
-int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, int n_seqs, cudaStream_t st) {
+int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, cudaStream_t st) {
   int* err = device_error_word();
   if (!err) return TEENY_ERR_DRIVER;
   const long long pieces = static_cast<long long>((keep + kMove - 1) / kMove) * n_seqs * 2 * c.H;
   if (pieces > 0x7fffffffLL) return TEENY_ERR_BAD_ARG;
-  const EvictScratch x{static_cast<unsigned*>(scratch), reinterpret_cast<unsigned*>(static_cast<uint8_t*>(scratch) + 256)};
+  // (the place of the attention's counters is left alone: the calls may share scratch)
+  uint8_t* own = static_cast<uint8_t*>(scratch) + TEENY_CACHE8_COUNTER_BYTES;
+  const EvictScratch x{reinterpret_cast<unsigned*>(own), reinterpret_cast<unsigned*>(own + 256)};
   auto select = [&](auto kernel) { launch_kernel(kernel, dim3(c.H, n_seqs), dim3(kSelThreads), 0, st, 1, c, keep, recent, kept, x, seqs); };
-  const int most = c.cap - recent;  // candidates
-  if (most <= 2 * kSelThreads) select(cache8_select_kernel<2>);
-  else if (most <= 16 * kSelThreads) select(cache8_select_kernel<16>);
-  else select(cache8_select_kernel<0>);
+  int most = 0;  // candidates
+  for (int i = 0; host && i < n_seqs; ++i) most = host[i].pos - recent > most ? host[i].pos - recent : most;
+  if (host && most <= 2 * kSelThreads) select(cache8_select_kernel<2>);
+  else select(cache8_select_kernel<16>);
   const bool pdl = pdl_enabled();
   pdl_set_enabled(true);
   const long long stay = 4ll * sm_count();
@@ -552,12 +555,6 @@ size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int
   return cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, with_weights != 0);
 }
 
-size_t teeny_cache8_attention_zeroed_bytes(const teeny_cache8_shape* shape, int f32, int heads, int n_seqs, int max_len) {
-  Cache8 c;
-  if (!cache_of(shape, &c) || heads <= 0 || heads % c.H || !step_sizes(1, n_seqs, max_len)) return 0;
-  return cache8_attention_zeroed_bytes(c, f32 != 0, heads, n_seqs, max_len);
-}
-
 int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void* k, const void* v, const float* k_scale,
                            const float* v_scale, float* weights, float weight_decay, const void* q, long long ldq, void* out,
                            long long ldo, int rows, int heads, float score_scale, float softcap, const float* sink, const void* gate,
@@ -604,7 +601,8 @@ int teeny_cache8_evict(const teeny_cache8_shape* shape, void* k, void* v, float*
   const size_t need = cache8_evict_scratch_bytes(c, n_seqs, keep);
   if (need && (!scratch || scratch_bytes < need)) return TEENY_ERR_SCRATCH;
   if (reinterpret_cast<uintptr_t>(scratch) & 15) return TEENY_ERR_ALIGNMENT;
-  return cache8_evict(c, keep, recent, kept, scratch, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, reinterpret_cast<cudaStream_t>(stream));
+  return cache8_evict(c, keep, recent, kept, scratch, reinterpret_cast<const SeqDesc*>(seqs), reinterpret_cast<const SeqDesc*>(host_seqs), n_seqs,
+                      reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -18,6 +18,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "../../include/teeny_cache8.h"
 #include "common.cuh"
 #include "kernels.h"
 #include "mma.cuh"
@@ -89,8 +90,7 @@ struct Shared {  // what a call's kernels share
   float scale_log2, one_over_cap, cap_l2;  // (the cap in base 2, like the scores)
   float* part_o;   // [2 * CTAs][rows of a unit][128]
   float* part_ml;  // [2 * CTAs][rows of a unit][2]
-  unsigned* arrivals;  // [entries][kv heads][max_groups]: CTAs that have stored their parts, zero between calls
-  int max_groups;
+  unsigned* arrivals;  // [CTAs]: how many have stored their part of the unit that begins in a CTA's share and goes on behind it, zero between calls
   float* lse2;     // [rows][Hq], base 2, or null
   float* scores;   // [entries][Hq][score_row] base 2, or null
   int score_row;   // cap, rounded up to whole fours
@@ -703,7 +703,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     if (u.c1 > u.c0) {
       __threadfence();
       // (the counter goes back to zero with the last arrival)
-      if (atomicInc(s.arrivals + (static_cast<size_t>(u.e) * s.c.H + u.hk) * s.max_groups + u.rg, u.c1 - u.c0) != static_cast<unsigned>(u.c1 - u.c0))
+      if (atomicInc(s.arrivals + u.c0, u.c1 - u.c0) != static_cast<unsigned>(u.c1 - u.c0))
         sm_left[threadIdx.x].c1 = -1;
       __threadfence();
     }
@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(256) cache8_rows_weights_kernel(const __grid_c
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   int kind, rows, parts, groups;
-  size_t arrivals, part_o, part_ml, lse2, scores, widened, bytes;
+  size_t part_o, part_ml, lse2, scores, widened, bytes;
 };
 template <typename F>
 void for_variant(int kind, F&& f) {  // rows in tiles of eight, or 0 for f32
@@ -925,20 +925,20 @@ Plan plan_of(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len
       using V = decltype(v);
       p.rows = V::kRows;
       p.parts = sm_count() * V::kCtas;  // the CTAs that are resident at once
+      if (p.parts > TEENY_CACHE8_COUNTER_BYTES / 4) p.parts = TEENY_CACHE8_COUNTER_BYTES / 4;
     });
     p.groups = static_cast<int>((unit + p.rows - 1) / p.rows);
     return static_cast<size_t>(2) * p.parts * p.rows;
   };
   const bool prompts = !f32 && call_len >= cache8_prefill_min_len(c, Hq);
   size_t part_rows = divide(call_len);
-  const size_t groups = p.groups;
   if (prompts) {
     const size_t n = divide(cache8_prefill_min_len(c, Hq) - 1);
     part_rows = part_rows > n ? part_rows : n;
   }
   divide(max_len);
   auto take = [&](size_t n) { const size_t at = p.bytes; p.bytes += (n + 255) / 256 * 256; return at; };
-  p.arrivals = take(static_cast<size_t>(n_seqs) * c.H * groups * 4);
+  take(TEENY_CACHE8_COUNTER_BYTES);  // the counters' place is the same for every call, so that calls of any sizes may share scratch
   p.part_o = take(part_rows * 128 * 4);
   p.part_ml = take(part_rows * 2 * 4);
   p.lse2 = weights ? take(static_cast<size_t>(rows) * Hq * 4) : 0;
@@ -980,10 +980,6 @@ size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows
   return plan_of(c, f32, Hq, rows, n_seqs, max_len, max_len, weights).bytes;
 }
 
-size_t cache8_attention_zeroed_bytes(const Cache8& c, int f32, int Hq, int n_seqs, int max_len) {
-  return plan_of(c, f32, Hq, 1, n_seqs, max_len, max_len, false).part_o;
-}
-
 int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int call_len, cudaStream_t st) {
   if (const int rc = prepare()) return rc;
   // Entries of many tokens go to the kernels of cache8_prefill.cu, the others to this file's: by their lengths on the device, the host only
@@ -1017,8 +1013,7 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
     s.one_over_cap = 1.0f / s.cap_l2;
   }
   uint8_t* scratch = static_cast<uint8_t*>(a.scratch);
-  s.arrivals = reinterpret_cast<unsigned*>(scratch + p.arrivals);
-  s.max_groups = p.groups;
+  s.arrivals = reinterpret_cast<unsigned*>(scratch);
   s.part_o = reinterpret_cast<float*>(scratch + p.part_o);
   s.part_ml = reinterpret_cast<float*>(scratch + p.part_ml);
   if (a.weights) s.lse2 = reinterpret_cast<float*>(scratch + p.lse2);

@@ -544,7 +544,6 @@ struct Cache8Attn {
   size_t scratch_bytes;
 };
 size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights);
-size_t cache8_attention_zeroed_bytes(const Cache8& c, int f32, int Hq, int n_seqs, int max_len);
 int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int max_len, cudaStream_t st);
 // Causal attention of the entries with at least min_len tokens (128 entries at most) over bf16 keys and values [kv heads, n_seqs * key_rows, .], entry e's
 // from row e * key_rows on (attention_prefill.cu).  lse2 [rows, Hq] or null: like t.lse, base 2.
@@ -556,6 +555,6 @@ int cache8_prefill_min_len(const Cache8& c, int Hq);
 size_t cache8_prefill_scratch_bytes(const Cache8& c, int n_seqs);
 int cache8_prefill(const Cache8& c, const Cache8Attn& a, float* lse2, void* scratch, const SeqDesc* seqs, int n_seqs, int max_len, cudaStream_t st);
 size_t cache8_evict_scratch_bytes(const Cache8& c, int n_seqs, int keep);
-int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, int n_seqs, cudaStream_t st);
+int cache8_evict(const Cache8& c, int keep, int recent, int* kept, void* scratch, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, cudaStream_t st);
 
 }  // namespace teeny

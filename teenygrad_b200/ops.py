@@ -629,12 +629,15 @@ def cache8_append(cache, k, v, table):
           "cache8_append")
 
 
+_CACHE8_COUNTER_BYTES = 4096  # TEENY_CACHE8_COUNTER_BYTES
+
+
 def cache8_attention_scratch(cache, table, q, weights=False):
-    """Scratch for calls with this many entries and rows.  Calls that follow one another in a stream may share it."""
-    f32, heads = _f32_flag(q), q.shape[1]
-    out = torch.empty(lib.teeny_cache8_attention_scratch_bytes(cache._shape_at, f32, heads, q.shape[0], table.n, table.longest, int(weights)),
+    """Scratch for calls with this many entries and rows.  Calls that follow one another in a stream may share the largest one's, evictions among
+    them."""
+    out = torch.empty(lib.teeny_cache8_attention_scratch_bytes(cache._shape_at, _f32_flag(q), q.shape[1], q.shape[0], table.n, table.longest, int(weights)),
                       dtype=torch.uint8, device=cache.device)
-    out[:lib.teeny_cache8_attention_zeroed_bytes(cache._shape_at, f32, heads, table.n, table.longest)].zero_()
+    out[:_CACHE8_COUNTER_BYTES].zero_()
     return out
 
 

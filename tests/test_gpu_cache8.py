@@ -394,6 +394,33 @@ def test_without_the_hosts_table(dtype, lens):
 
 
 @DTYPES
+def test_calls_of_any_sizes_share_scratch(dtype):
+    from teenygrad_b200 import ops
+    cache, want = filled(17, 6, 2, 700, 64, 64, 16, weights=True)
+    calls = []
+    for lens, pos in (([1] * 6, [699, 0, 64, 300, 31, 500]), ([1], [650]), ([9, 1, 140, 2, 0, 3], [100, 5, 300, 690, 7, 400]), ([200], [3]), ([5, 5], [600, 2])):
+        table, rows = rows_of(lens, range(len(lens)), pos)
+        calls.append((table, ops.step_table(table), rnd(18 + rows, rows, 8, 64).to(dtype)))
+    size = max((ops.cache8_attention_scratch(cache, on, q, True) for _, on, q in calls), key=lambda t: t.numel())
+    scratch = torch.full((size.numel(),), 255, dtype=torch.uint8, device="cuda")
+    scratch[:4096] = 0
+    gone = ops.step_table([(5, 60, 0, 0)])
+    for turn in range(3):
+        for i in (0, 2, 1, 3, 0, 4, 2):
+            table, on, q = calls[i]
+            out = ops.cache8_attention(q.cuda(), cache, 0.1, on, weight_decay=0.0, scratch=scratch)
+            if turn == 0:
+                check(out, None, want.attention(q, 0.1, table), dtype, q, 64, 700, 0.0, table)
+                calls[i] = (table, on, q)
+            if i == 1:
+                ops.cache8_evict(cache, gone, 60, 0, scratch=scratch)  # (all of them are kept)
+                if turn == 0:
+                    want.weights.copy_(cache.weights)
+                    want.evict([(5, 60, 0, 0)], 60, 0)
+    assert not bool(scratch[:4096].any())
+
+
+@DTYPES
 @pytest.mark.parametrize("lens", [[1, 1, 1], [4, 140, 1]])
 def test_the_same_call_gives_the_same_bits(dtype, lens):
     from teenygrad_b200 import ops
