@@ -5,7 +5,7 @@
 // them.  (mma.sync on E4M3 operands is made of the same f16 products here, with additions of its own behind each: 0.19 m16n8k32 a clock
 // and SM, where the f16 pairs run at 0.42 / 2.)  The 16 rows of a product are keys, then dimensions of the values; its eight columns are query rows,
 // so that few query heads waste nothing.  A query row is scaled by a power of two so that its largest number is in [2^14, 2^15): a bf16
-// number below 2^-28 of that loses bits, no other.  f32 rows are two f16 terms, 22 bits, in two columns tiles whose sums lie in the same thread's
+// number below 2^-28 of that loses bits, no other.  f32 rows are two f16 terms, 22 bits, in two column tiles whose sums lie in the same thread's
 // registers.  Probabilities are f16 numbers times 2^14 (f32: two terms as well), so that a key is lost only 2^-38 below the row's
 // maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to the largest so far, the probabilities.
 //
@@ -54,14 +54,14 @@ struct Variant {
 
 // D (16 x 8) += A (16 x 16) B
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // 8 x 8 16-bit numbers: lane (g, c) gives (row g, columns 2c, 2c + 1) and gets (rows 2c, 2c + 1 of column g)
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 // Four E4M3 numbers as two f16 pairs
