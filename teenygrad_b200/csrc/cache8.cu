@@ -315,17 +315,24 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
                                                                       const SeqDesc* seqs, int* err) {
   constexpr int kMost = kMove * kCache8Head / 16 / kMoveThreads;
   __shared__ unsigned sm_top[2][kMove / 16], sm_ticket;
+  __shared__ int sm_number, sm_who, sm_entry;  // the ticket's piece: thread 0 divides
   __shared__ int sm_failed;
   const int heads = 2 * c.H;
-  struct Piece { int number, who, head, of_v, t0, tokens; size_t row; } p{};
+  struct Piece { int number, who, entry, head, of_v, t0, tokens; size_t row; } p{};
   int from[kMost];  // where the tokens of this thread's 16-byte pieces are
   auto width = [&]() { return p.of_v ? c.V : c.D; };
   auto token_of = [&](int i, int per) { return per == 8 ? i >> 3 : i / per; };
-  auto take = [&](unsigned ticket) {  // the piece of a ticket, and its indices under way
-    p.number = static_cast<int>(ticket / (n_seqs * heads));
-    p.who = static_cast<int>(ticket % (n_seqs * heads));
-    const int e = p.who / heads;
-    p.head = p.who % heads >> 1;
+  auto hand_out = [&](unsigned ticket) {
+    sm_ticket = ticket;
+    sm_number = static_cast<int>(ticket / static_cast<unsigned>(n_seqs * heads));
+    sm_who = static_cast<int>(ticket) - sm_number * n_seqs * heads;
+    sm_entry = sm_who / heads;
+  };
+  auto take = [&]() {  // the piece that was handed out, and its indices under way
+    p.number = sm_number;
+    p.who = sm_who;
+    const int e = p.entry = sm_entry;
+    p.head = (p.who - e * heads) >> 1;
     p.of_v = p.who & 1;
     p.t0 = p.number * kMove;
     const SeqDesc sq = seqs[e];
@@ -341,13 +348,13 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
   };
   pdl_wait();
   if (threadIdx.x == 0) {
-    sm_ticket = atomicAdd(x.ticket, 1u);
+    hand_out(atomicAdd(x.ticket, 1u));
     sm_failed = 0;
   }
   if (threadIdx.x < 2 * (kMove / 16)) sm_top[threadIdx.x / (kMove / 16)][threadIdx.x % (kMove / 16)] = 0u;
   __syncthreads();
   unsigned ticket = sm_ticket;
-  if (ticket < pieces) take(ticket);
+  if (ticket < pieces) take();
   for (int round = 0; ticket < pieces; ++round) {
     const Piece q = p;
     const int d = width(), per = d / 16, chunks = q.tokens * per;
@@ -374,7 +381,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
         ks[m] = exponent_of(sc[m]) + (from[m] == q.t0 + token_of(i, per) ? kStays : 0);
       }
     }
-    if (!q.of_v && static_cast<int>(threadIdx.x) < q.tokens) wt = w[kept[(static_cast<size_t>(q.who / heads) * c.H + q.head) * keep + q.t0 + threadIdx.x]];
+    if (!q.of_v && static_cast<int>(threadIdx.x) < q.tokens) wt = w[kept[(static_cast<size_t>(q.entry) * c.H + q.head) * keep + q.t0 + threadIdx.x]];
     unsigned next = 0;
     if (threadIdx.x == 0) next = atomicAdd(x.ticket, 1u);
 #pragma unroll
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
         atomicMax(&top[block], bits);
       }
     }
-    if (threadIdx.x == 0) sm_ticket = next;
+    if (threadIdx.x == 0) hand_out(next);
     asm volatile("" ::"f"(wt) : "memory");
     __syncthreads();  // every load of the CTA has arrived: what they gave has been used
     unsigned* flags = x.loaded + q.who;
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cach
     // (nothing written is told by this flag, only that the reads are done: no fence, which would wait for the last piece's stores)
     if (threadIdx.x == 0 && q.tokens > 0) asm volatile("st.relaxed.gpu.global.u32 [%0], 1;" ::"l"(flags + q.number * stride) : "memory");
     ticket = sm_ticket;
-    if (ticket < pieces) take(ticket);
+    if (ticket < pieces) take();
     if (threadIdx.x < 32 && q.tokens > 0) {
       bool fine = true;
       uint64_t since = 0;

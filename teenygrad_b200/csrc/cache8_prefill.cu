@@ -52,32 +52,38 @@ __global__ void __launch_bounds__(256) cache8_widen_kernel(const Cache8 c, const
   const float* scales = (of_v ? c.vs : c.ks) + row * c.blocks;
   uint4* dst = reinterpret_cast<uint4*>((of_v ? to.v : to.k) + (static_cast<size_t>(head) * to.n_seqs * to.key_rows + static_cast<size_t>(blockIdx.z) * to.key_rows + t0) * d);
   bool nan = false;
-  const int chunks = kTile * per;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < chunks; i += 256) {
-    const int t = t0 + (per == 8 ? i >> 3 : i / per);
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    float scale = 0.0f;
-    if (t < live) {
-      w = src[i];
-      scale = scales[t >> c.shift];
-    }
-    if (of_v && t >= sq.pos) {
-      uint32_t word[4] = {w.x, w.y, w.z, w.w};
+  // four 16-byte pieces of codes at a time, straight-line code up to the stores: a piece behind the live tokens reads the last one's place
+  const int chunks = kTile * per, last = (live - t0) * per - 1;
+  for (int i0 = threadIdx.x; i0 < chunks; i0 += 4 * 256) {
+    uint4 w[4];
+    float scale[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t is = ((word[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bytes 0x7f, 0xff
-        if (is) {
-          nan = true;
+    for (int m = 0; m < 4; ++m) {
+      const int i = min(i0 + 256 * m, last), t = t0 + (per == 8 ? i >> 3 : i / per);
+      w[m] = src[i];
+      scale[m] = scales[t >> c.shift];
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int i = i0 + 256 * m, t = t0 + (per == 8 ? i >> 3 : i / per);
+      if (i >= chunks) break;
+      uint32_t word[4] = {w[m].x, w[m].y, w[m].z, w[m].w};
+      const bool there = i <= last;
+      if (of_v && t >= sq.pos) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t is = ((word[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bytes 0x7f, 0xff
+          nan = nan || (is && there);
           word[k] &= ~((is >> 7) * 0xffu);
         }
       }
-      w = make_uint4(word[0], word[1], word[2], word[3]);
+      uint4 o[2];
+      widen16(make_uint4(word[0], word[1], word[2], word[3]), scale[m], o);
+      if (!there) o[0] = o[1] = make_uint4(0u, 0u, 0u, 0u);
+      // (whole sectors: as two 16-byte stores a sector is written in halves)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                   ::"l"(dst + 2 * i), "r"(o[0].x), "r"(o[0].y), "r"(o[0].z), "r"(o[0].w), "r"(o[1].x), "r"(o[1].y), "r"(o[1].z), "r"(o[1].w) : "memory");
     }
-    uint4 o[2];
-    widen16(w, scale, o);
-    dst[2 * i] = o[0];
-    dst[2 * i + 1] = o[1];
   }
   if (of_v) {
     const int any = __syncthreads_or(nan);
