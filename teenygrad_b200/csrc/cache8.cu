@@ -144,7 +144,8 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 }
 
 // One CTA for the new tokens of one entry in one block of the cache: blockIdx = (block counted from the entry's first, 2 * head + (values), entry).
-// A thread holds the 16-element pieces that it reads (up to NCH) until the scale is known: each number is read once.
+// A thread holds the 16-element pieces that it reads (up to NCH) until the scale is known: each number is read once.  Bound by HBM for prompts (16 of
+// up to 2048 tokens, eight heads of 128, 130 MB: 23.3 us, 5.6 TB/s), by a launch's latency for single tokens (64 of them: 3.0 us).
 template <typename T, int NCH>
 __global__ void __launch_bounds__(kThreads) cache8_append_kernel(const Cache8 c, const Cache8Append a, const SeqDesc* seqs, int max_len, int vec) {
   __shared__ float sh[kThreads / 32];
@@ -219,7 +220,7 @@ struct EvictScratch {
 
 // The kept tokens of one (entry, head), in order.  The smallest kept weight is found by digits, 11, 11 and 10 bits from the top: a histogram of
 // the next digit of the keys that agree with the digits found so far.  Each warp has a stretch of the candidates, in registers up to 32 PER of them (of
-// more they are read again for every digit).
+// more they are read again for every digit).  A chain of short steps: 700 candidates 5.6 us, 16 x 8 heads of up to 7680 14 us.
 template <int PER>
 __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8 c, int keep, int recent, int* kept, const EvictScratch x, const SeqDesc* seqs) {
   __shared__ int hist[kBins], sums[32], found[2], warp_gt[32], warp_eq[32];
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8
 // their order: a CTA reads its tokens into registers, says so, and waits, before it writes, for those in front; whoever has one of these either has
 // said so or is about to, waiting at most for pieces further in front.  Each byte is read once and written once; tokens that stay where and what
 // they are are not written.  A piece is a chain of dependent accesses (number, indices, tokens, flags, writes; 17000 clocks with a CTA for
-// each), so CTAs stay, and ask for the next piece and its indices while they work on one.
+// each, 88 us for 16 x 8 heads of up to 4096 kept tokens), so CTAs stay, and ask for the next piece and its indices while they work on one: 62 us.
 __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cache8 c, int keep, int n_seqs, unsigned pieces, const int* kept, const EvictScratch x,
                                                                       const SeqDesc* seqs, int* err) {
   constexpr int kMost = kMove * kCache8Head / 16 / kMoveThreads;

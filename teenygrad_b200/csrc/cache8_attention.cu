@@ -14,7 +14,8 @@
 // group, each CTA takes the same number of consecutive slices of all of them, whatever the lengths, and its warps take them in turn.  Where
 // a sequence ends or a share does, the warps' sums are added through shared memory.  A sequence that lies in several CTAs' shares leaves partial
 // results in scratch, at most two for each CTA; the last one to have stored its part adds them (a second kernel for it cost 4 to 10 us a
-// call; parts of single warps, four times as many, up to 14 us).  No CTA waits for another.
+// call; parts of single warps, four times as many, up to 14 us).  No CTA waits for another.  64 sequences of 1500 to 6000 tokens, 32 / 8 heads of 128, 500 MB:
+// 91 us, 5.5 TB/s; one of 701 tokens: 9.8 us, a chain of latencies.
 #include <atomic>
 #include <type_traits>
 
