@@ -11,9 +11,10 @@
  *
  * Step tables are those of teeny_hybrid.h: seqs, device int32 [n_seqs][4] = {slot, position, first row, tokens}; max_len: the longest
  * entry.  host_seqs: the same table in host memory, or null.  With it an entry that does not fit (slot, position + tokens, rows) and
- * a slot that comes twice in a call that writes to it are refused; without it the kernels leave out entries that do not fit (the
- * table may be written on the device, by a replayed graph for instance).  A position is the index of a token's row in the cache; after an eviction
- * that is no longer its position in the text, which only the caller's rotations need.
+ * a slot that comes twice in a call that writes to it are refused.  The kernels go by the device's table, which a replayed graph may
+ * have moved on since the call was made, and leave out entries that do not fit; one longer than max_len does not.  A position is the
+ * index of a token's row in the cache; after an eviction that is no longer its position in the text, which only the caller's
+ * rotations need.
  *
  * f32: element type of k, v, q, out and gate (0 bf16, 1 f32).  Row strides are in elements, heads lie side by side within a row.
  * dim and vdim are multiples of 16 up to 128, block is 16, 32, 64 or 128, the caches' bases are 16-byte aligned.

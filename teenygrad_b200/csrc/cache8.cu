@@ -575,8 +575,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
     return TEENY_ERR_BAD_ARG;
   if (const int rc = bind_cache(&c, const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scale), const_cast<float*>(v_scale), weights))
     return rc;
-  const SeqDesc* host = reinterpret_cast<const SeqDesc*>(host_seqs);
-  if (host) {
+  if (const SeqDesc* host = reinterpret_cast<const SeqDesc*>(host_seqs)) {
     if (!all_fit(host, n_seqs, c, rows, max_len)) return TEENY_ERR_BAD_ARG;
     if (const int rc = check_table(host, n_seqs, c, weights != nullptr, true)) return rc;
   }
@@ -585,7 +584,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
   if (reinterpret_cast<uintptr_t>(scratch) & 15) return TEENY_ERR_ALIGNMENT;
   const Cache8Attn a{f32 != 0, q, ldq, out, ldo, rows, heads, score_scale, softcap, sink, gate, ldg, lse, weights != nullptr, weight_decay,
                      scratch, scratch_bytes};
-  return cache8_attention(c, a, reinterpret_cast<const SeqDesc*>(seqs), host, n_seqs, max_len, reinterpret_cast<cudaStream_t>(stream));
+  return cache8_attention(c, a, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, max_len, reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t teeny_cache8_evict_scratch_bytes(const teeny_cache8_shape* shape, int n_seqs, int keep) {

@@ -982,18 +982,13 @@ size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows
   return plan_of(c, f32, Hq, rows, n_seqs, max_len, max_len, weights).bytes;
 }
 
-int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int call_len, cudaStream_t st) {
+int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, int n_seqs, int call_len, cudaStream_t st) {
   if (const int rc = prepare()) return rc;
-  // Entries of many tokens go to the kernels of cache8_prefill.cu, the others to this file's: by their lengths on the device, the host only
-  // leaves out a launch that has nothing to do.
+  // Entries of many tokens go to the kernels of cache8_prefill.cu, the others to this file's: by their lengths on the device, which a replayed graph may
+  // have changed since the call was captured, so that both are launched wherever an entry can be long.
   const int min_len = cache8_prefill_min_len(c, a.Hq);
   const bool prompts = cache8_prefill_takes(c, a, call_len);
-  const int max_len = prompts && min_len - 1 < call_len ? min_len - 1 : call_len;
-  bool any_long = prompts, any_short = true;
-  if (host && prompts) {
-    any_long = any_short = false;
-    for (int i = 0; i < n_seqs; ++i) (host[i].len >= min_len ? any_long : any_short) |= host[i].len > 0;
-  }
+  const int max_len = prompts ? min_len - 1 : call_len;
   const Plan p = plan_of(c, a.f32, a.Hq, a.rows, n_seqs, max_len, call_len, a.weights != 0);
   // the kernels count slices in 32 bits
   if (static_cast<double>(call_len) * (a.Hq / c.H) > 2e9 || static_cast<double>(n_seqs) * c.H * p.groups * ((c.cap + kSlice - 1) / kSlice) > 2e9)
@@ -1026,15 +1021,18 @@ int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, 
   s.vec_o = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) & 15) == 0;
   s.err = device_error_word();
   if (!s.err) return TEENY_ERR_DRIVER;
-  if (any_long) {
+  if (prompts) {
     if (const int rc = cache8_prefill(c, a, s.lse2, scratch + p.widened, seqs, n_seqs, call_len, st)) return rc;
   }
-  if (any_short)
+  {
+    PdlScope behind;
+    if (!prompts) pdl_set_enabled(behind.was);  // (the call's first launch)
     for_variant(p.kind, [&](auto v) {
       using V = decltype(v);
       launch_kernel(cache8_attention_kernel<V>, dim3(p.parts), dim3(32 * kWarps), V::kBytes, st, 1, mk, mv, s);
     });
-  if (a.weights && any_short) {
+  }
+  if (a.weights) {
     const PdlScope behind;
     // warps for the same keys: as many as share rows usefully
     const long long eights = (static_cast<long long>(s.G) * max_len + 7) / 8;

@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(256) cache8_widen_kernel(const Cache8 c, const
 // Puts the NaN values back: column d of an output row is NaN from the first token on whose value is NaN there.  blockIdx = (head, entry).
 __global__ void __launch_bounds__(128) cache8_nan_kernel(const Cache8 c, const Cache8Attn a, const Widened w, const SeqDesc* seqs, int min_len, int max_len) {
   pdl_wait();
+  pdl_trigger();
   const SeqDesc sq = seqs[blockIdx.y];
   if (sq.len < min_len || !cache8_fits(sq, c, a.rows, max_len)) return;
   const int live = sq.pos + sq.len, head = blockIdx.x;

@@ -544,7 +544,7 @@ struct Cache8Attn {
   size_t scratch_bytes;
 };
 size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights);
-int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, const SeqDesc* host, int n_seqs, int max_len, cudaStream_t st);
+int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, int n_seqs, int max_len, cudaStream_t st);
 // Causal attention of the entries with at least min_len tokens (128 entries at most) over bf16 keys and values [kv heads, n_seqs * key_rows, .], entry e's
 // from row e * key_rows on (attention_prefill.cu).  lse2 [rows, Hq] or null: like t.lse, base 2.
 int attention_prefill_ragged(const Cache8& c, const Cache8Attn& t, const bf16* k, const bf16* v, int key_rows, float* lse2, const SeqDesc* seqs,

@@ -543,7 +543,8 @@ def latent_attention(q, cache, vdim, score_scale, seqs, max_len, out=None, scrat
 class StepTable:
     """A step's entries on the device (``seqs`` int32 [n, 4]) and in host memory (``host``), with what the calls need to know of
     them.  A program that advances ``seqs`` on the device (a replayed graph) passes the table all the same: the kernels go by
-    ``seqs``, the host's copy serves the checks of arguments and the choice of kernels when a call is made or captured."""
+    ``seqs``, whose entries may be shorter than the host's ``longest`` but not longer (such an entry is left out); the host's copy serves the
+    checks of arguments and the choice of kernels when a call is made or captured."""
 
     def __init__(self, entries, device="cuda"):
         rows = [tuple(int(x) for x in e) for e in entries]

@@ -278,7 +278,7 @@ def test_an_entry_that_does_not_fit_is_left_out(dtype):
     (BF, (8, 2, 128, 128, 64), [1, 1], True, {"cache8_attention_kernel", "cache8_weights_kernel"}),
     (F32, (8, 2, 64, 64, 64), [130, 1], True, {"cache8_attention_kernel", "cache8_rows_weights_kernel"}),
     (BF, (8, 2, 128, 128, 64), [9, 1], True, {"cache8_attention_kernel", "cache8_rows_weights_kernel"}),
-    (BF, (8, 2, 128, 128, 64), [130, 140], False, {"cache8_widen_kernel", "attention_prefill_kernel", "cache8_nan_kernel"}),
+    (BF, (8, 2, 128, 128, 64), [130, 140], False, {"cache8_widen_kernel", "attention_prefill_kernel", "cache8_nan_kernel", "cache8_attention_kernel"}),
     (BF, (8, 2, 128, 128, 64), [130, 1], True, {"cache8_widen_kernel", "attention_prefill_kernel", "cache8_nan_kernel", "cache8_prompt_weights_kernel",
                                                 "cache8_attention_kernel", "cache8_rows_weights_kernel"}),
 ])
@@ -569,6 +569,38 @@ def test_a_captured_step_follows_its_table(dtype):
         for a, b in ((one.k, two.k), (one.v, two.v)):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
         assert torch.equal(one.k_scale, two.k_scale) and torch.equal(one.weights, two.weights)
+
+
+@DTYPES
+@pytest.mark.parametrize("lens", [[150, 140], [9, 9]])
+def test_a_captured_call_follows_its_tables_lengths(dtype, lens):
+    """Entries that were captured long and are short when the graph is replayed, and the other way round."""
+    from teenygrad_b200 import ops
+    heads, kv, dim = 8, 2, 128
+    table, rows = rows_of(lens, [1, 0], [40, 7])
+    on, q = ops.step_table(table), rnd(81, rows, heads, dim).to(dtype)
+    cache, _ = filled(82, 2, kv, 200, dim, dim, 32, weights=True)
+    x, out = q.cuda(), torch.zeros(rows, heads, dim, dtype=dtype, device="cuda")
+    ops.cache8_attention(x, cache, 0.1, on, weight_decay=0.5, out=out)  # (loads the kernels)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.cache8_attention(x, cache, 0.1, on, weight_decay=0.5, out=out)
+    for now in ([1, 1], [lens[0], 1], [2, lens[1]], lens, [0, 3]):
+        fresh, want = filled(82, 2, kv, 200, dim, dim, 32, weights=True)
+        cache.weights.copy_(fresh.weights)
+        entries = [(s, p, row, n) for (s, p, row, _), n in zip(table, now)]
+        on.seqs.copy_(torch.tensor(entries, dtype=torch.int32))
+        out.fill_(5.0)
+        graph.replay()
+        ref = want.attention(q, 0.1, entries, decay=0.5)
+        check(out, None, ref, dtype, q, dim, 200, 0.0, entries)
+        _, _, p = bounds(dtype, ref, q, dim, 200, 0.0)
+        near = float(p.max()) + (max(lens) * heads // kv + 4) * 2.0 ** -24
+        assert float(((cache.weights.double().cpu() - want.weights).abs() - near * want.weights).max()) <= 0.0, now
+        mine = torch.zeros(rows, dtype=torch.bool)
+        for _, _, row, n in entries:
+            mine[row:row + n] = True
+        assert bool((out.cpu()[~mine] == 5.0).all())
 
 
 @DTYPES
