@@ -48,7 +48,8 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
  * denominator; gate [rows, ldg] (heads vdim apart) or null: the output is multiplied by sigmoid(gate).  lse [rows, heads] or
  * null: logarithm of the denominator, the sink's part included.  weights (or null): for every live token of the entries' slots
  * weights <- weight_decay * weights + the probabilities that the entry's tokens and query heads gave it; with weight_decay 0 what
- * was there is not read.  The gate does not count there.  Rows of out that belong to no entry stay as they are.  Sums are made in
+ * was there is not read.  The gate does not count there.  Rows of out that belong to no entry stay as they are; no two entries have
+ * a row in common (refused where host_seqs shows it).  Sums are made in
  * a fixed order: the same call gives the same bits.
  * scratch: its first TEENY_CACHE8_COUNTER_BYTES are zero before the first call, and every call leaves them zero (after a device error they have to be
  * made zero again).  Calls of any sizes may share it, evictions among them, as long as they follow one another.  out must not overlap q. */

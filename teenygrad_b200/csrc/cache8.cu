@@ -531,6 +531,23 @@ bool all_fit(const SeqDesc* t, int n, const Cache8& c, int rows, int max_len) {
     if (!cache8_fits(t[i], c, rows, max_len) && !(t[i].len == 0 && t[i].pos >= 0 && t[i].pos <= c.cap)) return false;
   return true;
 }
+// No row is two entries' (both would write its results).
+bool rows_apart(const SeqDesc* t, int n, int rows) {
+  int end = 0, i = 0;
+  for (; i < n && (t[i].len == 0 || t[i].row0 >= end); ++i)
+    if (t[i].len > 0) end = t[i].row0 + t[i].len;
+  if (i == n) return true;
+  // (not in order)
+  unsigned char* seen = static_cast<unsigned char*>(calloc(rows, 1));
+  bool apart = seen != nullptr;
+  for (i = 0; i < n && apart; ++i)
+    for (int r = t[i].row0; r < t[i].row0 + t[i].len && apart; ++r) {
+      apart = !seen[r];
+      seen[r] = 1;
+    }
+  free(seen);
+  return apart;
+}
 bool step_sizes(int rows, int n_seqs, int max_len) { return rows > 0 && n_seqs > 0 && n_seqs <= 65535 && max_len > 0; }
 
 }  // namespace
@@ -576,7 +593,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
   if (const int rc = bind_cache(&c, const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scale), const_cast<float*>(v_scale), weights))
     return rc;
   if (const SeqDesc* host = reinterpret_cast<const SeqDesc*>(host_seqs)) {
-    if (!all_fit(host, n_seqs, c, rows, max_len)) return TEENY_ERR_BAD_ARG;
+    if (!all_fit(host, n_seqs, c, rows, max_len) || !rows_apart(host, n_seqs, rows)) return TEENY_ERR_BAD_ARG;
     if (const int rc = check_table(host, n_seqs, c, weights != nullptr, true)) return rc;
   }
   const size_t need = cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, weights != nullptr);

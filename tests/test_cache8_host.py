@@ -56,6 +56,17 @@ def test_tables(lib, table):
         assert attention(lib, sh, host(*table), len(table)) == BAD
 
 
+@pytest.mark.parametrize("table", [[(0, 0, 0, 2), (1, 0, 1, 2)], [(0, 0, 4, 2), (1, 0, 0, 5)], [(0, 0, 3, 1), (1, 5, 3, 1)], [(0, 0, 6, 2), (1, 0, 0, 0), (2, 0, 0, 7)]], ids=str)
+def test_rows_of_two_entries(lib, table):
+    assert attention(lib, shape(lib), host(*table), len(table)) == BAD
+
+
+@pytest.mark.parametrize("table", [[(0, 0, 0, 2), (1, 0, 2, 2)], [(0, 0, 4, 2), (1, 0, 0, 4)], [(0, 0, 3, 1), (1, 5, 3, 0)], [(0, 0, 6, 2), (1, 0, 7, 0), (2, 0, 0, 6)]], ids=str)
+def test_rows_apart_in_any_order(lib, table):
+    """(Scratch is asked for behind the table.)"""
+    assert attention(lib, shape(lib), host(*table), len(table), weights=P, size=3) == SCRATCH
+
+
 def test_arguments(lib):
     sh = shape(lib)
     assert append(lib, sh, kn=None) == BAD and append(lib, sh, k=None) == BAD and append(lib, sh, ks=None) == BAD and append(lib, sh, ldk=127) == BAD
