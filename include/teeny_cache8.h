@@ -10,7 +10,7 @@
  * weight that each cached token received, summed over the query heads of its kv head.
  *
  * Step tables are those of teeny_hybrid.h: seqs, device int32 [n_seqs][4] = {slot, position, first row, tokens}; max_len: the longest
- * entry.  host_seqs: the same table in host memory, or null.  With it an entry that does not fit (slot, position + tokens, rows) and
+ * entry, or anything above it.  host_seqs: the same table in host memory, or null.  With it an entry that does not fit (slot, position + tokens, rows) and
  * a slot that comes twice in a call that writes to it are refused.  The kernels go by the device's table, which a replayed graph may
  * have moved on since the call was made, and leave out entries that do not fit; one longer than max_len does not.  A position is the
  * index of a token's row in the cache; after an eviction that is no longer its position in the text, which only the caller's

@@ -2,6 +2,7 @@
 //
 // Scales are powers of two, so that holding a code at another scale is a shift of its exponent, exact unless the result leaves E4M3's
 // normal range.  A block's scale is 2^k with the smallest k >= -126 for which its largest number is at most 448 * 2^k.
+#include <algorithm>
 #include <cstdlib>
 
 #include "../../include/teeny_cache8.h"
@@ -549,6 +550,8 @@ bool rows_apart(const SeqDesc* t, int n, int rows) {
   free(seen);
   return apart;
 }
+// The longest entry that can fit, where the caller's bound is above it.
+int longest_of(int max_len, const Cache8& c, int rows) { return std::min(max_len, std::min(c.cap, rows)); }
 bool step_sizes(int rows, int n_seqs, int max_len) { return rows > 0 && n_seqs > 0 && n_seqs <= 65535 && max_len > 0; }
 
 }  // namespace
@@ -571,14 +574,14 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
     if (const int rc = check_table(host, n_seqs, c, true, true)) return rc;
   }
   const Cache8Append a{f32 != 0, k_new, v_new, ldk, ldv, rows};
-  return cache8_append(c, a, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, max_len, reinterpret_cast<cudaStream_t>(stream));
+  return cache8_append(c, a, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, longest_of(max_len, c, rows), reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int f32, int heads, int rows, int n_seqs, int max_len,
                                             int with_weights) {
   Cache8 c;
   if (!cache_of(shape, &c) || heads <= 0 || heads % c.H || !step_sizes(rows, n_seqs, max_len)) return 0;
-  return cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, with_weights != 0);
+  return cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, longest_of(max_len, c, rows), with_weights != 0);
 }
 
 int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void* k, const void* v, const float* k_scale,
@@ -597,6 +600,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
     if (!all_fit(host, n_seqs, c, rows, max_len) || !rows_apart(host, n_seqs, rows)) return TEENY_ERR_BAD_ARG;
     if (const int rc = check_table(host, n_seqs, c, weights != nullptr, true)) return rc;
   }
+  max_len = longest_of(max_len, c, rows);
   const size_t need = cache8_attention_scratch_bytes(c, f32 != 0, heads, rows, n_seqs, max_len, weights != nullptr);
   if (need && (!scratch || scratch_bytes < need)) return TEENY_ERR_SCRATCH;
   if (reinterpret_cast<uintptr_t>(scratch) & 15) return TEENY_ERR_ALIGNMENT;

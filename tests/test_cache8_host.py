@@ -82,6 +82,13 @@ def test_arguments(lib):
     assert evict(lib, sh, host((0, 101, 0, 0))) == BAD and evict(lib, sh, host((0, 5, 0, 0), (0, 6, 0, 0)), 2) == BAD and evict(lib, sh, host((4, 5, 0, 0))) == BAD
 
 
+def test_scratch_for_a_bound_that_nothing_reaches(lib):
+    """max_len may be anything above the longest entry, which has to fit the rows and the cache."""
+    size = lambda rows, longest, f32: lib.lib.teeny_cache8_attention_scratch_bytes(C.addressof(shape(lib)), f32, 4, rows, 2, longest, 1)  # noqa: E731
+    for f32 in (0, 1):
+        assert size(8, 2 ** 31 - 1, f32) == size(8, 8, f32) and size(900, 2 ** 31 - 1, f32) == size(900, 100, f32)
+
+
 def test_the_wrappers_checks(lib):
     import torch
     from teenygrad_b200 import ops

@@ -394,6 +394,29 @@ def test_without_the_hosts_table(dtype, lens):
 
 
 @DTYPES
+@pytest.mark.parametrize("lens", [[1, 3], [140, 2]])
+def test_a_bound_that_nothing_reaches(dtype, lens):
+    """max_len far above the longest entry, without the host's table."""
+    from teenygrad_b200 import ops
+    from teenygrad_b200._lib import lib
+    heads, kv, dim, most = 8, 2, 64, 2 ** 31 - 1
+    cache, want = filled(17, 2, kv, 200, dim, dim, 32)
+    table, rows = rows_of(lens, [1, 0], [40, 7])
+    on = ops.step_table(table)
+    q, k, v = (rnd(18 + i, rows, h, dim).to(dtype) for i, h in enumerate((heads, kv, kv)))
+    x, kx, vx, out = q.cuda(), k.cuda(), v.cuda(), torch.zeros(rows, heads, dim, dtype=dtype, device="cuda")
+    f32, tail = int(dtype == F32), [on.seqs.data_ptr(), None, on.n, most, ops._stream()]
+    assert lib.teeny_cache8_append(f32, *cache._at, None, kx.data_ptr(), kv * dim, vx.data_ptr(), kv * dim, rows, *tail) == 0
+    want.append(k, v, table)
+    same(cache, want)
+    size = lib.teeny_cache8_attention_scratch_bytes(cache._shape_at, f32, heads, rows, on.n, most, 0)
+    scratch = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    assert lib.teeny_cache8_attention(f32, *cache._at, None, 0.0, x.data_ptr(), heads * dim, out.data_ptr(), heads * dim, rows, heads, 0.1, 0.0, None, None, 0,
+                                      None, scratch.data_ptr(), size, *tail) == 0
+    check(out, None, want.attention(q, 0.1, table), dtype, q, dim, 200, 0.0, table)
+
+
+@DTYPES
 def test_calls_of_any_sizes_share_scratch(dtype):
     from teenygrad_b200 import ops
     cache, want = filled(17, 6, 2, 700, 64, 64, 16, weights=True)
