@@ -44,7 +44,7 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
                         const int* host_seqs, int n_seqs, int max_len, teeny_stream_t stream);
 
 /* Causal grouped-query attention of every entry's tokens over the cache, which holds their own keys and values already: score =
- * (q . k) * score_scale, with softcap > 0 softcap * tanh(score / softcap); sink [heads] or null: exp(sink) joins the softmax
+ * (q . k) * score_scale, with softcap > 0 softcap * tanh(score / softcap) (from 1e-30 to 1e30); sink [heads] or null: exp(sink) joins the softmax
  * denominator; gate [rows, ldg] (heads vdim apart) or null: the output is multiplied by sigmoid(gate).  lse [rows, heads] or
  * null: logarithm of the denominator, the sink's part included.  weights (or null): for every live token of the entries' slots
  * weights <- weight_decay * weights + the probabilities that the entry's tokens and query heads gave it; with weight_decay 0 what

@@ -901,7 +901,7 @@ void set_softcap(PrefillArgs* a, float softcap, float scale) {
   const float x = scale / softcap;
   float power = x * a->cap_l2;
   for (int i = 0; i < 4; ++i, power *= x * x) a->cap_c[i] = kTanh[i] * power;
-  a->small = a->cap_c[3] < -1e-30f ? 0.5f / x : -1.0f;  // (coefficients near the end of f32's range: exponential and reciprocal only)
+  a->small = a->cap_c[3] < -1e-30f && a->cap_c[3] > -1e30f ? 0.5f / x : -1.0f;  // (coefficients near the end of f32's range: exponential and reciprocal only)
 }
 
 // `d` < 128: the copies fill the columns beyond with zeros (loads) or leave them out (stores)
@@ -1041,7 +1041,7 @@ int attention_prefill_ragged(const Cache8& c, const Cache8Attn& t, const bf16* k
   if (!a.err) return TEENY_ERR_DRIVER;
   auto kernel = t.softcap > 0.0f ? attention_prefill_kernel<2, false, true>
                 : t.gate || t.sink ? attention_prefill_kernel<1, false, true> : attention_prefill_kernel<0, false, true>;
-  launch_kernel(kernel, dim3(static_cast<unsigned>(sm_count() / 2 * 2)), dim3(kThreads), Smem<false>::kSmemTotal, stream, 2, mk, mv, mq, mo, mg, a);
+  launch_kernel(kernel, dim3(static_cast<unsigned>(sm_count() < 4 ? 2 : sm_count() / 2 * 2)), dim3(kThreads), Smem<false>::kSmemTotal, stream, 2, mk, mv, mq, mo, mg, a);
   return static_cast<int>(cudaGetLastError());
 }
 

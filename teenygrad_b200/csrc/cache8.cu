@@ -592,7 +592,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
   Cache8 c;
   if (!cache_of(shape, &c) || !q || !out || !seqs || !step_sizes(rows, n_seqs, max_len) || heads <= 0 || heads % c.H ||
       ldq < static_cast<long long>(heads) * c.D || ldo < static_cast<long long>(heads) * c.V ||
-      (gate && ldg < static_cast<long long>(heads) * c.V) || !(softcap >= 0.0f && softcap < 1e30f) || !(score_scale > -1e30f && score_scale < 1e30f))
+      (gate && ldg < static_cast<long long>(heads) * c.V) || !(softcap == 0.0f || (softcap > 1e-30f && softcap < 1e30f)) || !(score_scale > -1e30f && score_scale < 1e30f))
     return TEENY_ERR_BAD_ARG;
   if (const int rc = bind_cache(&c, const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(k_scale), const_cast<float*>(v_scale), weights))
     return rc;

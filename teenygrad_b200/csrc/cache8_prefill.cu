@@ -392,7 +392,7 @@ int cache8_prefill_min_len(const Cache8& c, int Hq) {
 bool cache8_prefill_takes(const Cache8& c, const Cache8Attn& a, int max_len) {
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.gate);
   return !a.f32 && max_len >= cache8_prefill_min_len(c, a.Hq) && (bases & 15) == 0 && ((a.ldq | a.ldo | a.ldg) & 7) == 0 && a.scale > 0.0f &&
-         a.scale < 1e30f;
+         a.scale < 1e30f && (a.softcap == 0.0f || a.scale / a.softcap < 1e30f);
 }
 size_t cache8_prefill_scratch_bytes(const Cache8& c, int n_seqs) {
   size_t n;

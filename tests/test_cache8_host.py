@@ -74,6 +74,7 @@ def test_arguments(lib):
     assert append(lib, sh, rows=0) == BAD
     assert attention(lib, sh, heads=3) == BAD and attention(lib, sh, heads=0) == BAD and attention(lib, sh, q=None) == BAD and attention(lib, sh, out=None) == BAD
     assert attention(lib, sh, ldq=255) == BAD and attention(lib, sh, softcap=-1.0) == BAD and attention(lib, sh, softcap=float("nan")) == BAD
+    assert attention(lib, sh, softcap=1e-39) == BAD and attention(lib, sh, softcap=float("inf")) == BAD
     assert attention(lib, sh, gate=P, ldg=100) == BAD and attention(lib, sh, scale=float("nan")) == BAD
     assert attention(lib, sh, weights=P, scratch=None, size=0) == SCRATCH and attention(lib, sh, weights=P, size=3) == SCRATCH
     assert attention(lib, sh, weights=P, scratch=P + 4) == ALIGN

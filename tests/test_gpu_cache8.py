@@ -473,6 +473,14 @@ def test_a_soft_cap_far_above_the_scores():
                 assert float(((a - b).abs() / b).max()) < near
 
 
+@DTYPES
+@pytest.mark.parametrize("lens", [[1, 1], [5, 1], [130, 1]])
+@pytest.mark.parametrize("softcap", [2e-30, 1e-6])
+def test_a_soft_cap_far_below_the_scores(dtype, lens, softcap):
+    """Every score is the cap or its negative: nearly equal probabilities."""
+    attend(dtype, (4, 2, 64, 64, 32), lens, [60, 150][:len(lens)], 200, softcap, decay=0.5, seed=19)
+
+
 # ------------------------------------------------------------------------------------------------ evict
 @pytest.mark.parametrize("block", [16, 64, 128])
 @pytest.mark.parametrize("keep,recent", [(1, 0), (1, 1), (50, 0), (50, 50), (130, 17), (299, 5), (300, 10)])
