@@ -7,7 +7,7 @@
 // so that few query heads waste nothing.  A query row is scaled by a power of two so that its largest number is in [2^14, 2^15): a bf16
 // number below 2^-28 of that loses bits, no other.  f32 rows are two f16 terms, 22 bits, in two column tiles whose sums lie in the same thread's
 // registers.  Probabilities are f16 numbers times 2^14 (f32: two terms as well), so that a key is lost only 2^-38 below the row's
-// maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to the largest so far, the probabilities.
+// maximum so far.  Scales of key blocks multiply the scores; those of value blocks, relative to the largest so far (2^-112 at least), the probabilities.
 //
 // The call is bound by reading the cache.  A CTA is four warps, each with slices of 32 keys of its own in flight (keys and values by TMA, their scales by
 // 4-byte asynchronous copies on the same barrier).  Work is divided evenly by slices: entry after entry, head after head, row group after row
@@ -33,6 +33,9 @@ constexpr int kSlice = 32;                     // keys that a warp takes at a ti
 constexpr int kBox = kSlice * kCache8Head;     // 4 KB: their keys, or their values (narrower heads are filled up with zeros by the copies)
 constexpr int kStage = 2 * kBox;
 constexpr int kWarps = 4;                      // of a CTA
+// The values' reference begins here: a block of zeros has the scale 2^-126, and 2^14 over that is no f32 number, while 2^14 / kLeastRef and kLeastRef / 2^14 are
+// normal ones.  Blocks of smaller scales (numbers below 2^-103) lose bits where a probability is below 2^-14.
+constexpr float kLeastRef = 0x1p-112f;
 
 // Variant of the kernel: RT tiles of eight query rows in TERMS f16 terms (bf16: 1, f32: 2).  One tile in one term fits 168 registers, with which an SM
 // has three CTAs; more take two.
@@ -399,7 +402,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
     // acc[tile][j]: dimensions 16 g + 2j (rows 2c, 2c + 1), 16 g + 2j + 1 (the same), in units of vref * 2^-14
     float m[RT][2], l[RT][2], acc[NT][8][4];
-    float vref = 0.0f;  // largest scale of the values so far
+    float vref = kLeastRef;  // largest scale of the values so far
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -462,7 +465,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
               for (int z = 0; z < 4; ++z) acc[nt][j][z] *= down;
         }
-        const float inv = vref > 0.0f ? 16384.0f / vref : 0.0f, r0 = vs0 * inv, r1 = vs1 * inv;
+        const float inv = 16384.0f / vref, r0 = vs0 * inv, r1 = vs1 * inv;
         float y[RT][4][2];  // [row tile][keys 8 t + g][rows 2c, 2c + 1]
         bool grows = false;
 #pragma unroll
