@@ -414,7 +414,8 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.0f;
-    for (int sj = p.j + ((warp - done) & (kWarps - 1)); sj < p.end && ok; sj += kWarps, ++count) {
+    int half = 0;  // 1, 2: only the slice's first, second 16 keys count
+    for (int sj = p.j + ((warp - done) & (kWarps - 1)); sj < p.end && ok;) {
       const int st = count & (ST - 1), kb = sj * kSlice;
       if (!mbar_wait(bars + 8 * st, count / ST & 1, s.err, DEVERR_ATTN_SOFTMAX)) {
         ok = false;
@@ -423,8 +424,12 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       if (kb < p.limit) {
         const uint8_t *kt = gen + warp * (ST * kStage) + st * kStage + g * 128, *vt = gen + warp * (ST * kStage) + st * kStage + kBox;
         const float4 scales = *reinterpret_cast<const float4*>(gen + V::kScales + (warp * ST + st) * 16);
-        const float ks0 = scales.x, ks1 = scales.y, vs0 = scales.z, vs1 = scales.w;
+        const float ks0 = scales.x, ks1 = scales.y, vs0 = scales.z;
+        float vs1 = scales.w;
         const bool masked = kb + kSlice > p.sq.pos + 1;
+        // Two blocks of 16, the later one of much larger values, which not all rows see: one block at a time, so that it takes no bits from the rows before it.
+        if (masked && p.sq.len > 1 && half == 0 && vs1 > 16.0f * vs0) half = 1;
+        if (half == 1) vs1 = 0.0f;
         // ---- scores: keys 16 u + g and 16 u + 8 + g of the slice are rows g and g + 8 of tile u; lane c reads the dimensions that it holds of the query ----
         float x[NT][2][4];
 #pragma unroll
@@ -493,7 +498,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) y[rt][t][z] = kb + 8 * t + g < rows_limit[rt][z] ? y[rt][t][z] : -INFINITY;
+              for (int z = 0; z < 2; ++z) y[rt][t][z] = kb + 8 * t + g < rows_limit[rt][z] && half != (t < 2 ? 2 : 1) ? y[rt][t][z] : -INFINITY;
         }
         if (s.scores) {
 #pragma unroll
@@ -603,8 +608,15 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                 mma_f16_16816(acc[nt][2 * k + j], a[j][0], a[j][1], a[j][2], a[j][3], pb[nt][2 * kk], pb[nt][2 * kk + 1]);
           }
       }
+      if (half == 1) {  // (the stage once more)
+        half = 2;
+        continue;
+      }
+      half = 0;
       __syncwarp();
       load_next();
+      sj += kWarps;
+      ++count;
     }
 
     // ---- the warps' sums together, and the rows' results or this CTA's part of them ----

@@ -152,6 +152,23 @@ def test_values_of_small_and_large_scales(dtype, lens, pos, exponents):
 
 
 @DTYPES
+@pytest.mark.parametrize("lens,pos", [([20, 9], [8, 41]), ([40, 3], [0, 14]), ([140, 150], [5, 0])])
+@pytest.mark.parametrize("up", [40, 100])
+@pytest.mark.parametrize("off16", [False, True])
+def test_values_that_a_row_does_not_see_are_of_no_scale_to_it(dtype, lens, pos, up, off16):
+    """The entry's later blocks are 2^up larger than what its first rows see."""
+    heads, kv, dim, block, cap = 8, 2, 64, 16, 190
+    cache, want = filled(67, 2, kv, cap, dim, 48, block, weights=True)
+    table, rows = rows_of(lens, [1, 0], pos)
+    for slot, p, _, n in table:
+        at = min(-(-(p + 2) // block) * block, cap // block * block)  # the first block that the entry's first row does not see
+        for h in range(kv):
+            for b in range(at // block, -(-cap // block)):
+                put(cache, want, "v", slot, h, slice(b * block, min(cap, (b + 1) * block)), scale=2.0 ** (up - 9 + (b & 1)))
+    run(dtype, cache, want, table, rows, heads, 68, off16=off16)
+
+
+@DTYPES
 @pytest.mark.parametrize("lens,pos", LENS)
 @pytest.mark.parametrize("heads,kv,dim,block,off16", [(8, 2, 128, 64, False), (4, 4, 80, 16, True), (24, 2, 16, 32, True)])
 def test_bounds_of_the_kernels_own_roundings(dtype, lens, pos, heads, kv, dim, block, off16):
