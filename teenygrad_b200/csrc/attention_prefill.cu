@@ -792,10 +792,18 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
         if (ok) ok = mbar_wait(bar(PV_DONE + (glast & 1)), (glast >> 1) & 1, err, DEVERR_ATTN_SOFTMAX);
         if (ok) {
           tc_fence_after();
-          if (OPT > 0) l += fast_exp2(fmaf(sink, 1.4426950408889634f, -m_fin));
+          const float over = OPT > 0 ? fmaf(sink, 1.4426950408889634f, -m_fin) : 0.0f;
+          float sum_from = m_fin, out_scale = args.out_scale;  // what l is relative to
+          if (RAGGED && OPT > 0 && over > 0.0f) {  // the sink: its exponential relative to the scores may be no f32 number, and lse is one
+            out_scale *= fast_exp2(-over);
+            l = fmaf(l, fast_exp2(-over), 1.0f);
+            sum_from = sink * 1.4426950408889634f;
+          } else if (OPT > 0) {
+            l += fast_exp2(over);
+          }
           float inv;
           asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(l));  // l >= 1 (the row's maximum contributes 2^0); 1 ulp
-          inv *= args.out_scale;
+          inv *= out_scale;
           const float2 inv2 = {inv, inv};
           const bool valid = qi < rows_of(it);
           uint32_t t[4][32];  // the whole row in flight, so that the accumulator is free for the next item at once
@@ -851,7 +859,7 @@ attention_prefill_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gri
           }
           if constexpr (RAGGED) {
             const size_t at = (static_cast<size_t>(row0_of(it)) + qi) * args.Hq + it.h;
-            const float lse2 = m_fin + log2f(l);
+            const float lse2 = sum_from + log2f(l);
             if (valid && args.lse2) args.lse2[at] = lse2;
             if (valid && args.lse) args.lse[at] = 0.6931471805599453f * lse2;
           } else if (valid && args.lse)

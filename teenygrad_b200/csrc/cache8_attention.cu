@@ -147,10 +147,20 @@ template <typename T>
 __device__ __forceinline__ void finish_row(const Shared& s, const SeqDesc& sq, int hk, int r, int lane, const float4& x, float m, float l) {
   const int i = r / s.G, hq = hk * s.G + r - i * s.G;
   const size_t row = static_cast<size_t>(sq.row0) + i;
-  if (s.a.sink) l += ex2(fmaf(s.a.sink[hq], kLog2e, -m));
+  float inv = 1.0f;
+  if (s.a.sink) {
+    const float sink = s.a.sink[hq], over = fmaf(sink, kLog2e, -m);
+    if (over > 0.0f) {  // relative to the sink: its exponential relative to the scores may be no f32 number
+      inv = ex2(-over);
+      l = fmaf(l, inv, 1.0f);
+      m = sink * kLog2e;
+    } else {
+      l += ex2(over);
+    }
+  }
   if (lane == 0) note_lse(s, row, hq, m + log2f(l));
   if (4 * lane >= s.c.V) return;
-  const float inv = 1.0f / l;
+  inv /= l;
   float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
   if (s.a.gate) {
     const T* gate = static_cast<const T*>(s.a.gate) + row * s.a.ldg + static_cast<size_t>(hq) * s.c.V + 4 * lane;

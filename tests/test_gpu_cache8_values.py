@@ -170,6 +170,19 @@ def test_values_that_a_row_does_not_see_are_of_no_scale_to_it(dtype, lens, pos, 
 
 @DTYPES
 @pytest.mark.parametrize("lens,pos", LENS)
+@pytest.mark.parametrize("sink", [60.0, 95.0, 150.0, 3e4, -150.0, float("inf"), -float("inf")])
+def test_sinks_far_from_the_scores(dtype, lens, pos, sink):
+    """lse is the sink's value where that is far above the scores, and theirs where it is far below."""
+    heads, kv, dim = 8, 2, 64
+    cache, want = filled(69, 3, kv, 190, dim, 48, 32, weights=True)
+    table, rows = rows_of(lens, [1, 2, 0], pos)
+    sinks = rnd(70, heads)
+    sinks[1], sinks[3], sinks[6] = sink, sink, sink + 1.0
+    run(dtype, cache, want, table, rows, heads, 71, sink=sinks)
+
+
+@DTYPES
+@pytest.mark.parametrize("lens,pos", LENS)
 @pytest.mark.parametrize("heads,kv,dim,block,off16", [(8, 2, 128, 64, False), (4, 4, 80, 16, True), (24, 2, 16, 32, True)])
 def test_bounds_of_the_kernels_own_roundings(dtype, lens, pos, heads, kv, dim, block, off16):
     """Ordinary numbers: probabilities in f16 (prompts: bf16) or two terms of it, and nothing coarser."""
