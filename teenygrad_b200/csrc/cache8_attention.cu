@@ -215,7 +215,8 @@ __device__ __forceinline__ float split_row(const float (&x)[32], float scale_log
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   int p = 0;
-  if (amax > 0.0f && amax < INFINITY) p = min(100, max(-100, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23)));
+  // (from -113 on, for the largest f32 numbers; with more than 118 the factor would be subnormal, and rows below 2^-104 are left smaller instead)
+  if (amax > 0.0f && amax < INFINITY) p = min(118, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23));
   const float up = __uint_as_float(static_cast<unsigned>(127 + p) << 23), down = __uint_as_float(static_cast<unsigned>(127 - p) << 23);
 #pragma unroll
   for (int w = 0; w < 16; ++w) {

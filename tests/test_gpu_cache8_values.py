@@ -183,6 +183,21 @@ def test_sinks_far_from_the_scores(dtype, lens, pos, sink):
 
 @DTYPES
 @pytest.mark.parametrize("lens,pos", LENS)
+@pytest.mark.parametrize("q_exp,k_exp", [(117, -118), (124, -118), (-110, 100), (-100, 80)])
+def test_queries_of_any_size(dtype, lens, pos, q_exp, k_exp):
+    """Rows of queries near both ends of their type, over keys that make ordinary scores of them."""
+    heads, kv, dim, cap = 8, 2, 64, 190
+    cache, want = filled(72, 3, kv, cap, dim, 48, 32, weights=True)
+    for s in range(3):
+        for h in range(kv):
+            put(cache, want, "k", s, h, slice(0, cap), scale=2.0 ** k_exp)
+    table, rows = rows_of(lens, [1, 2, 0], pos)
+    # (score_scale takes what is left: dots of about 2^(3 + 6.5 + q_exp + k_exp))
+    run(dtype, cache, want, table, rows, heads, 73, factor=2.0 ** q_exp, scale=2.0 ** min(-9 - q_exp - k_exp, 20))
+
+
+@DTYPES
+@pytest.mark.parametrize("lens,pos", LENS)
 @pytest.mark.parametrize("heads,kv,dim,block,off16", [(8, 2, 128, 64, False), (4, 4, 80, 16, True), (24, 2, 16, 32, True)])
 def test_bounds_of_the_kernels_own_roundings(dtype, lens, pos, heads, kv, dim, block, off16):
     """Ordinary numbers: probabilities in f16 (prompts: bf16) or two terms of it, and nothing coarser."""
