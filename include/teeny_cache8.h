@@ -51,7 +51,7 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
  * was there is not read.  The gate does not count there.  Rows of out that belong to no entry stay as they are; no two entries have
  * a row in common (refused where host_seqs shows it).  Sums are made in
  * a fixed order: the same call gives the same bits.
- * scratch: its first TEENY_CACHE8_COUNTER_BYTES are zero before the first call, and every call leaves them zero (after a device error they have to be
+ * scratch, on 32 bytes: its first TEENY_CACHE8_COUNTER_BYTES are zero before the first call, and every call leaves them zero (after a device error they have to be
  * made zero again).  Calls of any sizes may share it, evictions among them, as long as they follow one another.  out must not overlap q. */
 size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int f32, int heads, int rows, int n_seqs, int max_len,
                                             int with_weights);
@@ -65,7 +65,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
  * head keeps its last `recent` tokens and those of the others with the largest weights (equal ones: the lowest index; NaN counts as the
  * least), `keep` in all, and they move to the front in their order, with scales made anew from what is kept.  A slot with at most
  * `keep` tokens keeps them all.  The slot's next token belongs at min(position, keep).  kept [n_seqs, kv_heads, keep]: the kept
- * tokens' indices before, -1 behind the last.  Rows of the cache behind the kept tokens, and their weights, stay as they are. */
+ * tokens' indices before, -1 behind the last.  Rows of the cache behind the kept tokens, and their weights, stay as they are.  scratch: on 16 bytes. */
 size_t teeny_cache8_evict_scratch_bytes(const teeny_cache8_shape* shape, int n_seqs, int keep);
 int teeny_cache8_evict(const teeny_cache8_shape* shape, void* k, void* v, float* k_scale, float* v_scale, float* weights, int keep,
                        int recent, int* kept, void* scratch, size_t scratch_bytes, const int* seqs, const int* host_seqs, int n_seqs,

@@ -107,3 +107,12 @@ def test_the_wrappers_checks(lib):
     assert ops._head_rows(z(5, 100)[:, 8:72].unflatten(1, (4, 16)), 4, 16, "q") == 100
     t = ops.step_table([(0, 3, 0, 2), (1, 0, 2, 5)], "cpu")
     assert (t.n, t.longest, list(t.host)) == (2, 5, [0, 3, 0, 2, 1, 0, 2, 5]) and t.seqs.tolist() == [[0, 3, 0, 2], [1, 0, 2, 5]]
+
+
+@pytest.mark.parametrize("f32,longest", [(0, 8), (0, 600), (1, 600)])
+def test_scratch_off_its_alignment(lib, f32, longest):
+    """Prompts' tokens are widened into scratch by stores of 32 bytes: scratch that begins in the middle of 32 is refused, whatever the call's lengths."""
+    sh = shape(lib, cap=1000)
+    for off in (4, 8, 16, 24, 48, 112):
+        assert lib.lib.teeny_cache8_attention(f32, C.addressof(sh), P, P, P, P, None, 0.0, P, 256, P, 256, 700, 4, 0.1, 0.0, None, None, 0, None,
+                                              P + off, 1 << 40, P, host((0, 3, 0, longest)), 1, longest, None) == ALIGN
