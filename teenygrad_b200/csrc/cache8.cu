@@ -605,7 +605,7 @@ int teeny_cache8_attention(int f32, const teeny_cache8_shape* shape, const void*
   if (need && (!scratch || scratch_bytes < need)) return TEENY_ERR_SCRATCH;
   if (reinterpret_cast<uintptr_t>(scratch) & 31) return TEENY_ERR_ALIGNMENT;  // (prompts' tokens are widened by stores of 32 bytes)
   const Cache8Attn a{f32 != 0, q, ldq, out, ldo, rows, heads, score_scale, softcap, sink, gate, ldg, lse, weights != nullptr, weight_decay,
-                     scratch, scratch_bytes};
+                     scratch};
   return cache8_attention(c, a, reinterpret_cast<const SeqDesc*>(seqs), n_seqs, max_len, reinterpret_cast<cudaStream_t>(stream));
 }
 

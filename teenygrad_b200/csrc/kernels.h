@@ -513,7 +513,6 @@ struct Cache8 {
   int slots, H, cap, D, V, B, blocks, shift;  // B = 2^shift tokens a block, `blocks` of them a slot and head
 };
 constexpr int kCache8Head = 128;   // largest dim and vdim
-constexpr int kCache8Block = 128;  // largest block
 // An entry that the kernels leave out: they read and write nothing of it.
 __host__ __device__ inline bool cache8_fits(const SeqDesc& s, const Cache8& c, int rows, int max_len) {
   return s.slot >= 0 && s.slot < c.slots && s.pos >= 0 && s.len > 0 && s.len <= max_len && s.len <= c.cap && s.pos <= c.cap - s.len &&
@@ -541,7 +540,6 @@ struct Cache8Attn {
   int weights;     // add to the cache's weights
   float decay;
   void* scratch;
-  size_t scratch_bytes;
 };
 size_t cache8_attention_scratch_bytes(const Cache8& c, int f32, int Hq, int rows, int n_seqs, int max_len, bool weights);
 int cache8_attention(const Cache8& c, const Cache8Attn& a, const SeqDesc* seqs, int n_seqs, int max_len, cudaStream_t st);
