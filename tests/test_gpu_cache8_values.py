@@ -81,8 +81,8 @@ def run(dtype, cache, want, table, rows, heads, seed, factor=1.0, scale=None, si
         gw, ww = cache.weights[slot].double().cpu(), want.weights[slot]
         assert torch.equal(gw[:, pos + n:], was[slot, :, pos + n:])
         far = (gw - ww).abs()[:, :pos + n]
-        finite = p[at][~inf]
-        assert bool((far <= (float(finite.max() if finite.numel() else 0.0) + (n * heads // kv + 4) * 2.0 ** -24) * ww[:, :pos + n] + 2.0 ** -120).all())
+        finite, least = p[at][~inf], n * heads // kv * 2.0 ** -126  # (a subnormal probability counts as none)
+        assert bool((far <= (float(finite.max() if finite.numel() else 0.0) + (n * heads // kv + 4) * 2.0 ** -24) * ww[:, :pos + n] + least).all())
     same(cache, want, weights=False)
     return got, z
 
