@@ -10,8 +10,8 @@
  * weight that each cached token received, summed over the query heads of its kv head.
  *
  * Step tables are those of teeny_hybrid.h: seqs, device int32 [n_seqs][4] = {slot, position, first row, tokens}; max_len: the longest
- * entry, or anything above it.  host_seqs: the same table in host memory, or null.  With it an entry that does not fit (slot, position + tokens, rows) and
- * a slot that comes twice in a call that writes to it are refused.  The kernels go by the device's table, which a replayed graph may
+ * entry, or anything above it, and at least 1 (a call whose entries are all empty is refused).  host_seqs: the same table in host memory, or
+ * null.  With it an entry that does not fit (slot, position + tokens, rows) and a slot that comes twice in a call that writes to it are refused.  The kernels go by the device's table, which a replayed graph may
  * have moved on since the call was made, and leave out entries that do not fit; one longer than max_len does not.  A position is the
  * index of a token's row in the cache; after an eviction that is no longer its position in the text, which only the caller's
  * rotations need.
@@ -51,6 +51,10 @@ int teeny_cache8_append(int f32, const teeny_cache8_shape* shape, void* k, void*
  * was there is not read.  The gate does not count there.  Rows of out that belong to no entry stay as they are; no two entries have
  * a row in common (refused where host_seqs shows it).  Sums are made in
  * a fixed order: the same call gives the same bits.
+ * Sums and statistics are f32.  Before the product with the values a probability is rounded to f16 (f32 calls: to 22 bits), and to bf16 in the entries of bf16
+ * calls with max(32, 192 / (heads / kv_heads)) tokens and more whose rows lie on 16 bytes, which the tcgen05 kernel takes.  In f16 a probability
+ * stands multiplied by its value block's scale, relative to the largest scale that the row sees: below 2^-28 that loses bits, below 2^-38 it is lost (f32 calls:
+ * 2^-39, 2^-49).
  * scratch, on 32 bytes: its first TEENY_CACHE8_COUNTER_BYTES are zero before the first call, and every call leaves them zero (after a device error they have to be
  * made zero again).  Calls of any sizes may share it, evictions among them, as long as they follow one another.  out must not overlap q. */
 size_t teeny_cache8_attention_scratch_bytes(const teeny_cache8_shape* shape, int f32, int heads, int rows, int n_seqs, int max_len,

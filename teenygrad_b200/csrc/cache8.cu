@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(kSelThreads) cache8_select_kernel(const Cache8
 // their order: a CTA reads its tokens into registers, says so, and waits, before it writes, for those in front; whoever has one of these either has
 // said so or is about to, waiting at most for pieces further in front.  Each byte is read once and written once; tokens that stay where and what
 // they are are not written.  A piece is a chain of dependent accesses (number, indices, tokens, flags, writes; 17000 clocks with a CTA for
-// each, 88 us for 16 x 8 heads of up to 4096 kept tokens), so CTAs stay, and ask for the next piece and its indices while they work on one: 67 us.
+// each, 88 us for 16 x 8 heads of up to 4096 kept tokens), so CTAs stay, and ask for the next piece and its indices while they work on one: 62 us, 67
+// with the flags released.
 __global__ void __launch_bounds__(kMoveThreads, 4) cache8_move_kernel(const Cache8 c, int keep, int n_seqs, unsigned pieces, const int* kept, const EvictScratch x,
                                                                       const SeqDesc* seqs, int* err) {
   constexpr int kMost = kMove * kCache8Head / 16 / kMoveThreads;

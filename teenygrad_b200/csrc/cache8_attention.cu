@@ -15,7 +15,7 @@
 // a sequence ends or a share does, the warps' sums are added through shared memory.  A sequence that lies in several CTAs' shares leaves partial
 // results in scratch, at most two for each CTA; the last one to have stored its part adds them (a second kernel for it cost 4 to 10 us a
 // call; parts of single warps, four times as many, up to 14 us).  No CTA waits for another.  64 sequences of 1500 to 6000 tokens, 32 / 8 heads of 128, 500 MB:
-// 91 us, 5.5 TB/s; one of 701 tokens: 9.8 us, a chain of latencies.
+// 92 us, 5.4 TB/s; one of 701 tokens: 10.0 us, a chain of latencies.
 #include <atomic>
 #include <type_traits>
 
@@ -117,7 +117,7 @@ __device__ __forceinline__ EntryShape entry_shape(const Shared& s, const SeqDesc
 // How the slices are shared.  With many units each of the CTAs takes the same number of consecutive slices, whatever units they are of: the first `more`
 // take one more than the others' `each`.  With few units, a unit is cut into parts of `cut` slices and each CTA takes one: the end
 // of a unit inside a share costs a CTA 5000 clocks (eight kv heads, one sequence of 701 tokens: 12.9 us without, 9.8 with; four of 14050: 27.1 and 21.8; four of
-// 40001 with weights: 82.3 and 80.3; 16 x 5 tokens, ragged: 41.8 and 38.2).  No share is less than a slice for each warp (unless its unit is), nor are there many more than 64 to a
+// 40001 with weights: 82.3 and 80.3; 16 x 5 tokens, ragged: 41.8 and 38.2, by now 39.0).  No share is less than a slice for each warp (unless its unit is), nor are there many more than 64 to a
 // unit, whose parts have to be added again.
 struct Shares {
   int parts, each, more, cut;
@@ -439,6 +439,7 @@ cache8_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         float vs1 = scales.w;
         const bool masked = kb + kSlice > p.sq.pos + 1;
         // Two blocks of 16, the later one of much larger values, which not all rows see: one block at a time, so that it takes no bits from the rows before it.
+        // (16 entries of five tokens: 39.2 us without, 39.9 with the loop's way back; a reference for each row 43.2.)
         if (masked && p.sq.len > 1 && half == 0 && vs1 > 16.0f * vs0) half = 1;
         if (half == 1) vs1 = 0.0f;
         // ---- scores: keys 16 u + g and 16 u + 8 + g of the slice are rows g and g + 8 of tile u; lane c reads the dimensions that it holds of the query ----

@@ -635,7 +635,7 @@ _CACHE8_COUNTER_BYTES = 4096  # TEENY_CACHE8_COUNTER_BYTES
 
 def cache8_attention_scratch(cache, table, q, weights=False):
     """Scratch for calls with this many entries and rows.  Calls that follow one another in a stream may share the largest one's, evictions among
-    them."""
+    them.  (A part of a larger buffer: on 32 bytes, the first 4096 bytes zero.)"""
     out = torch.empty(lib.teeny_cache8_attention_scratch_bytes(cache._shape_at, _f32_flag(q), q.shape[1], q.shape[0], table.n, table.longest, int(weights)),
                       dtype=torch.uint8, device=cache.device)
     out[:_CACHE8_COUNTER_BYTES].zero_()
